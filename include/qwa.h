@@ -5,7 +5,8 @@
  * ragged micro-batches.
  *
  * Shapes are fixed by the model: 16 query heads, 8 key/value heads,
- * head_dim 128, f16 storage, fp32 softmax and accumulation.
+ * head_dim 128, f16 storage, fp32 softmax and accumulation. The rotary, cache
+ * and shared-prefix entry points take other head counts, and bf16 too.
  *
  * Reference interface replaced (shihanqu/qwen3-embedding-webgpu-prepacked):
  *   QKNormRopeKernel.createRun + encodeRun     src/webgpu/ops.ts:152-166, :15-19
@@ -305,6 +306,157 @@ QWA_API qwa_status qwa_q40_qkv_projection(qwa_ctx *ctx, const void *input, const
  * during stream capture): the memory is released by the next Q4_0 call made
  * outside a capture, or by qwa_destroy. */
 QWA_API qwa_status qwa_q40_forget(qwa_ctx *ctx, const void *packed);
+
+/* ------------------------------------------------------------------------
+ * Requests behind a shared prefix: rotary positions, a key/value cache in 8
+ * bits, and attention over both. No counterpart in the reference, whose every
+ * request is computed whole (src/webgpu/embedding-engine.ts:56-75). */
+
+typedef enum qwa_dtype { QWA_F16 = 0, QWA_BF16 = 1 } qwa_dtype;
+
+typedef enum qwa_rope_layout {
+  QWA_ROPE_HALF = 0,        /* pairs (x[i], x[i + rotary_dim/2]), as ops.ts:104-150 */
+  QWA_ROPE_INTERLEAVED = 1  /* pairs (x[2i], x[2i+1]) */
+} qwa_rope_layout;
+
+/* Frequencies f_i = theta^(-2i/rotary_dim), i < rotary_dim/2, for longer contexts:
+ *   LINEAR  f_i / factor
+ *   NTK     theta * factor^(rotary_dim / (rotary_dim - 2)) in theta's place
+ *   YARN    f_i / factor * r_i + f_i * (1 - r_i), r_i the ramp from 0 to 1
+ *           between the dimensions that turn beta_fast and beta_slow times over
+ *           original_positions; cos and sin times attention_factor, or, if
+ *           that is <= 0, 0.1 ln(factor) + 1 (1 where factor <= 1)
+ *   LLAMA3  f_i / factor * (1 - s_i) + f_i * s_i, s_i from 0 to 1 while the
+ *           turns over original_positions go from low_ to high_freq_factor */
+typedef enum qwa_rope_scaling_kind {
+  QWA_ROPE_SCALING_NONE = 0,
+  QWA_ROPE_SCALING_LINEAR = 1,
+  QWA_ROPE_SCALING_NTK = 2,
+  QWA_ROPE_SCALING_YARN = 3,
+  QWA_ROPE_SCALING_LLAMA3 = 4
+} qwa_rope_scaling_kind;
+
+typedef struct qwa_rope_scaling {
+  int kind;
+  double factor;
+  double original_positions;                /* YARN, LLAMA3 */
+  double beta_fast, beta_slow;              /* YARN; usually 32 and 1 */
+  double attention_factor;                  /* YARN; <= 0: the rule above */
+  double low_freq_factor, high_freq_factor; /* LLAMA3; usually 1 and 4 */
+} qwa_rope_scaling;
+
+/* Rotary table: table[p][i] = (m cos a, m sin a), a = (first_position + p) *
+ * f_i in 64 bits, f32 [positions, rotary_dim/2, 2]; scaling NULL: none. With
+ * rotary_dim 128 the rows from P on are a rope_table argument for
+ * qwa_qk_norm_rope and qwa_qkv_projection whose requests begin at position P.
+ * rotary_dim even, 2..256; theta > 1; table 16-byte aligned. */
+QWA_API qwa_status qwa_rope_table(qwa_ctx *ctx, float *table, int64_t first_position,
+                                  int positions, int rotary_dim, double theta,
+                                  const qwa_rope_scaling *scaling, void *stream);
+
+/* 16-bit [tokens, heads, head_dim] in and out; strides in elements, a head's
+ * values contiguous. out may be in (with the same strides); otherwise they must not overlap. */
+typedef struct qwa_rope_tensor {
+  const void *in;
+  int64_t in_stride, in_head_stride;
+  void *out;
+  int64_t out_stride, out_head_stride;
+  int heads;
+} qwa_rope_tensor;
+
+/* Rotates the first rotary_dim values of every head of q and k (either may be
+ * NULL) by the table's row at each token's position and copies the rest:
+ *   y1 = x1 c - x2 s,  y2 = x2 c + x1 s
+ * in f32, rounded once. inverse != 0 takes -s: the way back, which is also the
+ * gradient (dx from dy). positions_device: DEVICE int32 [tokens]; a token
+ * whose position is not in 0..table_rows-1 is skipped, nothing of it is
+ * written. head_dim 2..1024; rotary_dim even, at most head_dim and 256. Rows,
+ * strides and pointers in multiples of 16 bytes take the fast path. */
+QWA_API qwa_status qwa_rope(qwa_ctx *ctx, int dtype, const qwa_rope_tensor *q,
+                            const qwa_rope_tensor *k, int tokens, int head_dim, int rotary_dim,
+                            int layout, int inverse, const int32_t *positions_device,
+                            const float *table, int table_rows, void *stream);
+
+typedef enum qwa_kv_format {
+  QWA_KV_PLAIN = 0, /* the 16-bit values themselves */
+  QWA_KV_E4M3 = 1,
+  QWA_KV_INT8 = 2
+} qwa_kv_format;
+
+/* Key/value cache, all device memory of the caller: k, v [slots, heads,
+ * head_dim] of 16-bit values or 8-bit codes; k_scale, v_scale (8-bit formats)
+ * [slots, heads] bytes e + 127. A value is code * 2^e. dtype: of the 16-bit values that
+ * are written and read. head_dim a power of two in 16..256; k and v 16-byte
+ * aligned. */
+typedef struct qwa_kv_cache {
+  int dtype;  /* qwa_dtype */
+  int format; /* qwa_kv_format */
+  int heads, head_dim;
+  int64_t slots;
+  void *k, *v;
+  uint8_t *k_scale, *v_scale;
+} qwa_kv_cache;
+
+/* Quantises rows k, v (16-bit [tokens, heads, head_dim], k_stride / v_stride
+ * elements a token) into slots slots_device[t] (DEVICE int32; a slot that is not
+ * in 0..slots-1 skips its row). Per (row, head): 2^e the least power of two
+ * for which the largest magnitude is at most 448 * 2^e (E4M3) or 127 * 2^e
+ * (INT8), 2^0 for a row of zeros; code = x * 2^-e rounded to nearest, ties to even.
+ * An infinity is stored as the largest code; NaN stays NaN in E4M3 and becomes 0 in
+ * INT8, and does not count for e. e is at least -15 / -24 (f16) and -117 / -126 (bf16),
+ * and where 256 * 2^e (64 * 2^e) is out of the 16-bit type's range, codes end at 240 (63): what
+ * is read back is always finite unless a NaN was written. Slots of one call must
+ * differ: of two rows for one slot, values of both may remain. */
+QWA_API qwa_status qwa_kv_cache_write(qwa_ctx *ctx, const qwa_kv_cache *cache, const void *k,
+                                      int64_t k_stride, const void *v, int64_t v_stride,
+                                      const int32_t *slots_device, int tokens, void *stream);
+
+/* Values of slots slots_device[t] as 16-bit rows [tokens, heads, head_dim]; a
+ * slot that is not in the cache gives zeros. */
+QWA_API qwa_status qwa_kv_cache_read(qwa_ctx *ctx, const qwa_kv_cache *cache,
+                                     const int32_t *slots_device, int tokens, void *k_out,
+                                     void *v_out, void *stream);
+
+/* Work lists of a shared-prefix attention for given lengths: `batch` requests
+ * with cu_seqlens_q_host queries and cu_seqlens_k_host own keys (HOST, packed
+ * back to back; NULL: as many keys as queries). A request's queries are the
+ * last of its own keys, so it has at least as many keys as queries; the
+ * shared prefix of prefix_len keys stands before all of them. mode: QWA_MODE_*,
+ * the sparse rule on absolute positions (AUTO: sparse iff prefix_len + the most own keys <=
+ * 8192); sparse_prefix / window as prefix / window of qwa_attention. q_heads a
+ * multiple of kv_heads, at most 128 times. The plan belongs to the
+ * context's device and lives until it is destroyed, which waits for the device;
+ * destroy it after the graphs that captured its use. Not during stream capture
+ * (it allocates). */
+typedef struct qwa_prefix_plan qwa_prefix_plan;
+QWA_API qwa_status qwa_prefix_plan_create(qwa_ctx *ctx, const int32_t *cu_seqlens_q_host,
+                                          const int32_t *cu_seqlens_k_host, int batch, int q_heads,
+                                          int kv_heads, int prefix_len, int mode,
+                                          int sparse_prefix, int window, qwa_prefix_plan **out);
+QWA_API qwa_status qwa_prefix_plan_destroy(qwa_prefix_plan *plan);
+
+/* Attention of the plan's requests behind the prefix held in the cache's slots
+ * first_slot .. first_slot + prefix_len - 1 (cache may be NULL if prefix_len is 0):
+ * every query sees the prefix and its request's own keys up to itself,
+ *   out = softmax(q k / sqrt(128)) v.
+ * q 16-bit [queries, q_heads, 128], k / v [own keys, kv_heads, 128], strides in
+ * elements a token (multiples of 8), out [queries, q_heads, 128] contiguous; all
+ * 16-byte aligned, head_dim 128. The prefix is read and multiplied once for
+ * the rows of all requests together. A value of v that is not finite reaches only the
+ * queries that see it. */
+QWA_API qwa_status qwa_prefix_attention(qwa_ctx *ctx, const qwa_prefix_plan *plan, int dtype,
+                                        const void *q, int64_t q_stride, const void *k,
+                                        int64_t k_stride, const void *v, int64_t v_stride,
+                                        void *out, const qwa_kv_cache *cache, int64_t first_slot,
+                                        void *stream);
+
+/* Work of such a call: kept (query, key) pairs of one query head (FLOPs = 512 *
+ * q_heads * pairs), and key tiles visited over all kv heads. */
+QWA_API qwa_status qwa_prefix_attention_work(const int32_t *cu_seqlens_q_host,
+                                             const int32_t *cu_seqlens_k_host, int batch,
+                                             int q_heads, int kv_heads, int prefix_len, int mode,
+                                             int sparse_prefix, int window, int64_t *kept_pairs,
+                                             int64_t *visited_tiles);
 
 #ifdef __cplusplus
 }

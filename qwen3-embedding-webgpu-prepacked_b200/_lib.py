@@ -20,6 +20,36 @@ I32, I64, F32 = ctypes.c_int, ctypes.c_int64, ctypes.c_float
 I32P = ctypes.POINTER(ctypes.c_int32)
 I64P = ctypes.POINTER(ctypes.c_int64)
 
+F64 = ctypes.c_double
+
+# qwa_dtype, qwa_kv_format, qwa_rope_layout, qwa_rope_scaling_kind
+DTYPE_F16, DTYPE_BF16 = 0, 1
+KV_PLAIN, KV_E4M3, KV_INT8 = 0, 1, 2
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1
+ROPE_SCALING = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3, "llama3": 4}
+
+
+class RopeScalingStruct(ctypes.Structure):
+    """qwa_rope_scaling"""
+    _fields_ = [("kind", I32), ("factor", F64), ("original_positions", F64), ("beta_fast", F64),
+                ("beta_slow", F64), ("attention_factor", F64), ("low_freq_factor", F64),
+                ("high_freq_factor", F64)]
+
+
+class RopeTensor(ctypes.Structure):
+    """qwa_rope_tensor"""
+    _fields_ = [("in_", P), ("in_stride", I64), ("in_head_stride", I64), ("out", P),
+                ("out_stride", I64), ("out_head_stride", I64), ("heads", I32)]
+
+
+class KvCacheStruct(ctypes.Structure):
+    """qwa_kv_cache"""
+    _fields_ = [("dtype", I32), ("format", I32), ("heads", I32), ("head_dim", I32),
+                ("slots", I64), ("k", P), ("v", P), ("k_scale", P), ("v_scale", P)]
+
+
+RopeTensorP, KvCacheP = ctypes.POINTER(RopeTensor), ctypes.POINTER(KvCacheStruct)
+
 # name -> (restype, argtypes); the exported surface of include/qwa.h
 SIGNATURES = {
     "qwa_create": (I32, [I32, ctypes.POINTER(P)]),
@@ -50,6 +80,16 @@ SIGNATURES = {
     "qwa_embedding_lookup_q6k": (I32, [P, P, P, I32, P, I32, I32, P]),
     "qwa_last_token_pool": (I32, [P, P, I32, P, I32P, I32, P]),
     "qwa_last_token_pool_padded": (I32, [P, P, P, P, I32, I32, I32, P]),
+    "qwa_rope_table": (I32, [P, P, I64, I32, I32, F64, ctypes.POINTER(RopeScalingStruct), P]),
+    "qwa_rope": (I32, [P, I32, RopeTensorP, RopeTensorP, I32, I32, I32, I32, I32, P, P, I32, P]),
+    "qwa_kv_cache_write": (I32, [P, KvCacheP, P, I64, P, I64, P, I32, P]),
+    "qwa_kv_cache_read": (I32, [P, KvCacheP, P, I32, P, P, P]),
+    "qwa_prefix_plan_create": (I32, [P, I32P, I32P, I32, I32, I32, I32, I32, I32, I32,
+                                     ctypes.POINTER(P)]),
+    "qwa_prefix_plan_destroy": (I32, [P]),
+    "qwa_prefix_attention": (I32, [P, P, I32, P, I64, P, I64, P, I64, P, KvCacheP, I64, P]),
+    "qwa_prefix_attention_work": (I32, [I32P, I32P, I32, I32, I32, I32, I32, I32, I32, I64P,
+                                        I64P]),
 }
 
 _lib = None

@@ -76,9 +76,9 @@ def _ptr(t: Optional[torch.Tensor]):
     return ctypes.c_void_p(t.data_ptr()) if t is not None else None
 
 
-def _stream(stream) -> int:
+def _stream(stream, device=None) -> int:
     if stream is None:
-        return torch.cuda.current_stream().cuda_stream
+        return torch.cuda.current_stream(device).cuda_stream
     return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
 
 
@@ -115,8 +115,9 @@ class AttentionRun:
 
 
 def encode_run(stream, run: EncodableRun) -> None:
-    """encodeRun (ops.ts:15-19): issue the run on ``stream`` (None = current)."""
-    _lib.check(run.launch(_stream(stream)), run.ctx.handle)
+    """encodeRun (ops.ts:15-19): issue the run on ``stream`` (None = the current
+    stream of the run's device)."""
+    _lib.check(run.launch(_stream(stream, run.ctx.device)), run.ctx.handle)
 
 
 class QKNormRopeKernel:

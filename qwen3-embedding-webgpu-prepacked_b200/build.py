@@ -14,8 +14,10 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libqwa.so")
-SOURCES = ["api.cu", "attention.cu", "prologue.cu", "noalloc.cu", "pool.cu", "rmsnorm.cu", "gemm.cu", "q40.cu", "ffn.cu", "q40_small.cu"]
-HEADERS = ["ptx.cuh", "internal.h", "attn_common.cuh", os.path.join("..", "..", "include", "qwa.h")]
+SOURCES = ["api.cu", "attention.cu", "prologue.cu", "noalloc.cu", "pool.cu", "rmsnorm.cu", "gemm.cu", "q40.cu", "ffn.cu", "q40_small.cu",
+           "rope.cu", "kv_cache.cu", "prefix_attention.cu"]
+HEADERS = ["ptx.cuh", "internal.h", "attn_common.cuh", "convert.cuh", "prefix_plan.h",
+           "prefix_attention.h", os.path.join("..", "..", "include", "qwa.h")]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",

@@ -16,6 +16,8 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <exception>
+#include <functional>
 #include <map>
 #include <memory>
 #include <string>
@@ -24,6 +26,7 @@
 
 #include "../../include/qwa.h"
 #include "internal.h"
+#include "prefix_attention.h"
 #include "ptx.cuh"
 
 using namespace qwa;
@@ -69,6 +72,20 @@ struct qwa_ctx {
   int skip_load = -1;                             // test hook, see qwa_set_debug
   float* small_ws = nullptr;                      // partial sums of the small-M Q4_0 path
   size_t small_ws_bytes = 0;
+  cudaStream_t upload = nullptr;  // copies of prefix plans, waited for before they are used
+};
+
+// Work lists of a shared-prefix attention, owned by the caller.
+struct qwa_prefix_plan {
+  int device = 0;
+  PrefixShape shape{};
+  int total_q = 0, total_k = 0;
+  void* memory = nullptr;  // items, tiles, rows, offsets
+  const PrefixItem* items = nullptr;
+  const PrefixTile* tiles = nullptr;
+  const PrefixRow* rows = nullptr;
+  const int* offsets = nullptr;
+  int grid = 0, splits = 1;
 };
 
 namespace {
@@ -106,16 +123,20 @@ qwa_status ensure_encode(qwa_ctx* ctx) {
   return QWA_OK;
 }
 
-// 3-D f16 map {128 dims, heads, rows}: head stride 256 B, row stride
-// row_stride_bytes; box {64, 1, 128} with 128-byte swizzle, so one load
-// lands as 128 rows x 128 B (the canonical SW128 K-major atom layout).
+// 3-D 16-bit map {128 dims, heads, rows}: head stride 256 B, row stride
+// row_stride_bytes; box {64, box_heads, box_rows} with 128-byte swizzle, so one
+// load lands as box_rows * box_heads rows x 128 B (the canonical SW128 K-major
+// atom layout), heads innermost.
 qwa_status make_map(qwa_ctx* ctx, CUtensorMap* map, const void* base, int heads, int64_t rows,
-                    int64_t row_stride_bytes, uint32_t box_rows = 128) {
+                    int64_t row_stride_bytes, uint32_t box_rows = 128, uint32_t box_heads = 1,
+                    bool bf16 = false) {
   cuuint64_t dims[3] = {128, static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(rows)};
   cuuint64_t strides[2] = {256, static_cast<cuuint64_t>(row_stride_bytes)};
-  cuuint32_t box[3] = {64, 1, box_rows};
+  cuuint32_t box[3] = {64, box_heads, box_rows};
   cuuint32_t elem[3] = {1, 1, 1};
-  CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims,
+  const CUtensorMapDataType type =
+      bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  CUresult r = g_encode(map, type, 3, const_cast<void*>(base), dims,
                         strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -484,6 +505,7 @@ qwa_status qwa_destroy(qwa_ctx* ctx) {
     if (ctx->d_rope) cudaFree(ctx->d_rope);
     if (ctx->d_status) cudaFree(ctx->d_status);
     if (ctx->small_ws) cudaFree(ctx->small_ws);
+    if (ctx->upload) cudaStreamDestroy(ctx->upload);
   }
   delete ctx;
   return QWA_OK;
@@ -996,6 +1018,511 @@ qwa_status qwa_selftest_tile(qwa_ctx* ctx, const void* a, const void* b, const v
   QWA_CUDA(ctx, launch_selftest_tile(ta, tb, tv, c, d, ctx->d_status,
                                      static_cast<cudaStream_t>(stream)));
   return QWA_OK;
+}
+
+// ------------------------------------------------------------ rotary positions
+namespace {
+
+// Frequencies (radians a position) and the factor of every cos and sin.
+qwa_status rope_frequencies(qwa_ctx* ctx, int rotary, double theta, const qwa_rope_scaling* s,
+                            RopeFrequencies* out) {
+  const int kind = s ? s->kind : QWA_ROPE_SCALING_NONE;
+  const int half = rotary / 2;
+  if (rotary < 2 || rotary > kMaxRotary || rotary % 2 != 0)
+    return fail(ctx, QWA_ERR_INVALID_ARG, "rotary_dim must be even and in 2..%d (got %d)",
+                kMaxRotary, rotary);
+  if (!(theta > 1.0) || !std::isfinite(theta))
+    return fail(ctx, QWA_ERR_INVALID_ARG, "theta must be a finite number above 1");
+  if (kind < QWA_ROPE_SCALING_NONE || kind > QWA_ROPE_SCALING_LLAMA3)
+    return fail(ctx, QWA_ERR_INVALID_ARG, "unknown rope scaling %d", kind);
+  if (kind != QWA_ROPE_SCALING_NONE && (!(s->factor > 0.0) || !std::isfinite(s->factor)))
+    return fail(ctx, QWA_ERR_INVALID_ARG, "the scaling factor must be a finite number above 0");
+  const bool parts = kind == QWA_ROPE_SCALING_YARN || kind == QWA_ROPE_SCALING_LLAMA3;
+  if (parts && (!(s->original_positions > 0.0) || !std::isfinite(s->original_positions)))
+    return fail(ctx, QWA_ERR_INVALID_ARG, "original_positions must be above 0");
+  const double pi = 3.14159265358979323846;
+  const double factor = s ? s->factor : 1.0;
+  out->half = half;
+  out->m = 1.0;
+  double base = theta;
+  if (kind == QWA_ROPE_SCALING_NTK)
+    base = theta * std::pow(factor, double(rotary) / std::max(rotary - 2, 1));
+  double low = 0.0, high = 0.0;
+  if (kind == QWA_ROPE_SCALING_YARN) {
+    if (!(s->beta_slow > 0.0) || !(s->beta_fast >= s->beta_slow) || !std::isfinite(s->beta_fast))
+      return fail(ctx, QWA_ERR_INVALID_ARG, "beta_fast >= beta_slow > 0 is required");
+    // the dimension that turns `turns` times over the original positions
+    auto at = [&](double turns) {
+      return half * std::log(s->original_positions / (turns * 2.0 * pi)) / std::log(theta);
+    };
+    low = std::max(std::floor(at(s->beta_fast)), 0.0);
+    high = std::min(std::ceil(at(s->beta_slow)), rotary - 1.0);
+    if (s->attention_factor > 0.0) out->m = s->attention_factor;
+    else if (factor > 1.0) out->m = 0.1 * std::log(factor) + 1.0;
+  }
+  if (kind == QWA_ROPE_SCALING_LLAMA3 && !(s->high_freq_factor > s->low_freq_factor))
+    return fail(ctx, QWA_ERR_INVALID_ARG, "high_freq_factor > low_freq_factor is required");
+  for (int i = 0; i < half; ++i) {
+    double f = std::pow(base, -double(i) / half);
+    if (kind == QWA_ROPE_SCALING_LINEAR) {
+      f /= factor;
+    } else if (kind == QWA_ROPE_SCALING_YARN) {
+      const double ramp =
+          std::min(std::max((i - low) / std::max(high - low, 0.001), 0.0), 1.0);
+      f = f / factor * ramp + f * (1.0 - ramp);
+    } else if (kind == QWA_ROPE_SCALING_LLAMA3) {
+      const double turns = s->original_positions * f / (2.0 * pi);
+      const double smooth = std::min(
+          std::max((turns - s->low_freq_factor) / (s->high_freq_factor - s->low_freq_factor), 0.0),
+          1.0);
+      f = (1.0 - smooth) * f / factor + smooth * f;
+    }
+    out->f[i] = f;
+  }
+  return QWA_OK;
+}
+
+bool good_dtype(int dtype) { return dtype == QWA_F16 || dtype == QWA_BF16; }
+
+// One of rope's tensors: its pointers and strides, in 16-bit values.
+qwa_status check_rope_side(qwa_ctx* ctx, const qwa_rope_tensor* t, int tokens, int head_dim,
+                           const char* name) {
+  if (t->heads < 1) return fail(ctx, QWA_ERR_INVALID_ARG, "%s: heads must be >= 1", name);
+  if (!t->in || !t->out) return fail(ctx, QWA_ERR_INVALID_ARG, "%s: NULL tensor pointer", name);
+  if ((reinterpret_cast<uintptr_t>(t->in) & 1u) || (reinterpret_cast<uintptr_t>(t->out) & 1u))
+    return fail(ctx, QWA_ERR_INVALID_ARG, "%s: pointers must be 2-byte aligned", name);
+  if (t->in_stride < 0 || t->in_head_stride < 0 || t->out_stride < 0 || t->out_head_stride < 0)
+    return fail(ctx, QWA_ERR_INVALID_ARG, "%s: strides must be >= 0", name);
+  // heads inside a token's row, or tokens inside a head's
+  const bool token_major =
+      (t->heads == 1 || t->out_head_stride >= head_dim) &&
+      (tokens == 1 || t->out_stride >= (t->heads - 1) * t->out_head_stride + head_dim);
+  const bool head_major =
+      (tokens == 1 || t->out_stride >= head_dim) &&
+      (t->heads == 1 || t->out_head_stride >= (tokens - 1) * t->out_stride + head_dim);
+  if (!token_major && !head_major)
+    return fail(ctx, QWA_ERR_INVALID_ARG, "%s: output strides let rows overlap", name);
+  if (t->in == t->out &&
+      (t->in_stride != t->out_stride || t->in_head_stride != t->out_head_stride))
+    return fail(ctx, QWA_ERR_INVALID_ARG, "%s: in place needs equal strides", name);
+  return QWA_OK;
+}
+
+RopeSide rope_side(const qwa_rope_tensor* t) {
+  if (!t) return RopeSide{};
+  return {static_cast<const uint16_t*>(t->in), static_cast<uint16_t*>(t->out), t->in_stride,
+          t->in_head_stride, t->out_stride, t->out_head_stride, t->heads};
+}
+
+}  // namespace
+
+qwa_status qwa_rope_table(qwa_ctx* ctx, float* table, int64_t first_position, int positions,
+                          int rotary_dim, double theta, const qwa_rope_scaling* scaling,
+                          void* stream) {
+  if (!ctx) return QWA_ERR_INVALID_ARG;
+  DeviceGuard guard(ctx->device);
+  RopeFrequencies fr;
+  qwa_status st = rope_frequencies(ctx, rotary_dim, theta, scaling, &fr);
+  if (st != QWA_OK) return st;
+  if (positions < 0 || first_position < 0 || first_position > 0x7fffffff)
+    return fail(ctx, QWA_ERR_INVALID_ARG, "positions must be >= 0 and first_position in 0..2^31-1");
+  if (positions == 0) return QWA_OK;
+  if (!table || !aligned16(table))
+    return fail(ctx, QWA_ERR_INVALID_ARG, "table must be a 16-byte aligned pointer");
+  QWA_CUDA(ctx, launch_rope_table(fr, reinterpret_cast<float2*>(table), first_position, positions,
+                                  static_cast<cudaStream_t>(stream)));
+  return QWA_OK;
+}
+
+qwa_status qwa_rope(qwa_ctx* ctx, int dtype, const qwa_rope_tensor* q, const qwa_rope_tensor* k,
+                    int tokens, int head_dim, int rotary_dim, int layout, int inverse,
+                    const int32_t* positions_device, const float* table, int table_rows,
+                    void* stream) {
+  if (!ctx) return QWA_ERR_INVALID_ARG;
+  DeviceGuard guard(ctx->device);
+  if (!good_dtype(dtype)) return fail(ctx, QWA_ERR_UNSUPPORTED, "dtype must be f16 or bf16");
+  if (layout != QWA_ROPE_HALF && layout != QWA_ROPE_INTERLEAVED)
+    return fail(ctx, QWA_ERR_INVALID_ARG, "unknown rope layout %d", layout);
+  if (tokens < 0) return fail(ctx, QWA_ERR_INVALID_ARG, "tokens must be >= 0");
+  if (head_dim < 2 || head_dim > 1024)
+    return fail(ctx, QWA_ERR_INVALID_ARG, "head_dim must be in 2..1024 (got %d)", head_dim);
+  if (rotary_dim < 2 || rotary_dim % 2 != 0 || rotary_dim > std::min(head_dim, kMaxRotary))
+    return fail(ctx, QWA_ERR_INVALID_ARG,
+                "rotary_dim must be even, >= 2 and at most head_dim and %d (got %d)", kMaxRotary,
+                rotary_dim);
+  if (!q && !k) return fail(ctx, QWA_ERR_INVALID_ARG, "one of q and k is required");
+  if (tokens == 0) return QWA_OK;
+  qwa_status st = QWA_OK;
+  if (q && (st = check_rope_side(ctx, q, tokens, head_dim, "q")) != QWA_OK) return st;
+  if (k && (st = check_rope_side(ctx, k, tokens, head_dim, "k")) != QWA_OK) return st;
+  if (!positions_device || (reinterpret_cast<uintptr_t>(positions_device) & 3u) || !table ||
+      !aligned16(table) || table_rows < 1)
+    return fail(ctx, QWA_ERR_INVALID_ARG,
+                "positions must be 4-byte aligned, table 16-byte aligned with >= 1 rows");
+  RopeArgs a{};
+  a.q = rope_side(q);
+  a.k = rope_side(k);
+  a.positions = positions_device;
+  a.table = reinterpret_cast<const float2*>(table);
+  a.table_rows = table_rows;
+  a.tokens = tokens;
+  a.head_dim = head_dim;
+  a.rotary = rotary_dim;
+  a.layout = layout;
+  a.inverse = inverse != 0;
+  QWA_CUDA(ctx, launch_rope(a, dtype == QWA_BF16, static_cast<cudaStream_t>(stream)));
+  return QWA_OK;
+}
+
+// ------------------------------------------------------------- 8-bit cache
+namespace {
+
+qwa_status check_cache(qwa_ctx* ctx, const qwa_kv_cache* c) {
+  if (!c) return fail(ctx, QWA_ERR_INVALID_ARG, "cache is NULL");
+  if (!good_dtype(c->dtype)) return fail(ctx, QWA_ERR_UNSUPPORTED, "dtype must be f16 or bf16");
+  if (c->format < QWA_KV_PLAIN || c->format > QWA_KV_INT8)
+    return fail(ctx, QWA_ERR_INVALID_ARG, "unknown cache format %d", c->format);
+  if (c->head_dim < 16 || c->head_dim > 256 || (c->head_dim & (c->head_dim - 1)))
+    return fail(ctx, QWA_ERR_UNSUPPORTED, "head_dim must be a power of two in 16..256 (got %d)",
+                c->head_dim);
+  if (c->heads < 1 || c->slots < 0 || c->slots > 0x7fffffff)
+    return fail(ctx, QWA_ERR_INVALID_ARG, "heads must be >= 1 and slots in 0..2^31-1");
+  if (c->slots > 0 && (!c->k || !c->v || !aligned16(c->k) || !aligned16(c->v)))
+    return fail(ctx, QWA_ERR_INVALID_ARG, "the cache's k and v must be 16-byte aligned pointers");
+  if (c->slots > 0 && c->format != QWA_KV_PLAIN && (!c->k_scale || !c->v_scale))
+    return fail(ctx, QWA_ERR_INVALID_ARG, "an 8-bit cache needs k_scale and v_scale");
+  return QWA_OK;
+}
+
+qwa_status cache_args(qwa_ctx* ctx, const qwa_kv_cache* c, const int32_t* slots_device, int tokens,
+                      KvCacheArgs* a) {
+  if (tokens < 0) return fail(ctx, QWA_ERR_INVALID_ARG, "tokens must be >= 0");
+  if (tokens > 0 && (!slots_device || (reinterpret_cast<uintptr_t>(slots_device) & 3u)))
+    return fail(ctx, QWA_ERR_INVALID_ARG, "slots must be a 4-byte aligned pointer");
+  if (static_cast<int64_t>(tokens) * c->heads > (1ll << 31))
+    return fail(ctx, QWA_ERR_INVALID_ARG, "tokens * heads must be at most 2^31");
+  *a = KvCacheArgs{};
+  a->k = c->k;
+  a->v = c->v;
+  a->k_scale = c->k_scale;
+  a->v_scale = c->v_scale;
+  a->slots = c->slots;
+  a->heads = c->heads;
+  a->head_dim = c->head_dim;
+  a->tokens = tokens;
+  a->slot_of = slots_device;
+  return QWA_OK;
+}
+
+}  // namespace
+
+qwa_status qwa_kv_cache_write(qwa_ctx* ctx, const qwa_kv_cache* cache, const void* k,
+                              int64_t k_stride, const void* v, int64_t v_stride,
+                              const int32_t* slots_device, int tokens, void* stream) {
+  if (!ctx) return QWA_ERR_INVALID_ARG;
+  DeviceGuard guard(ctx->device);
+  KvCacheArgs a;
+  qwa_status st = check_cache(ctx, cache);
+  if (st == QWA_OK) st = cache_args(ctx, cache, slots_device, tokens, &a);
+  if (st != QWA_OK) return st;
+  if (tokens == 0 || cache->slots == 0) return QWA_OK;
+  const int64_t width = static_cast<int64_t>(cache->heads) * cache->head_dim;
+  if (!k || !v || !aligned16(k) || !aligned16(v))
+    return fail(ctx, QWA_ERR_INVALID_ARG, "k and v must be 16-byte aligned pointers");
+  if (k_stride < width || k_stride % 8 != 0 || v_stride < width || v_stride % 8 != 0)
+    return fail(ctx, QWA_ERR_INVALID_ARG,
+                "k_stride and v_stride must be multiples of 8 and >= heads * head_dim");
+  a.k_in = k;
+  a.v_in = v;
+  a.k_stride = k_stride;
+  a.v_stride = v_stride;
+  QWA_CUDA(ctx, launch_kv_write(a, cache->dtype == QWA_BF16, cache->format,
+                                static_cast<cudaStream_t>(stream)));
+  return QWA_OK;
+}
+
+qwa_status qwa_kv_cache_read(qwa_ctx* ctx, const qwa_kv_cache* cache, const int32_t* slots_device,
+                             int tokens, void* k_out, void* v_out, void* stream) {
+  if (!ctx) return QWA_ERR_INVALID_ARG;
+  DeviceGuard guard(ctx->device);
+  KvCacheArgs a;
+  qwa_status st = check_cache(ctx, cache);
+  if (st == QWA_OK) st = cache_args(ctx, cache, slots_device, tokens, &a);
+  if (st != QWA_OK) return st;
+  if (tokens == 0) return QWA_OK;
+  if (!k_out || !v_out || !aligned16(k_out) || !aligned16(v_out))
+    return fail(ctx, QWA_ERR_INVALID_ARG, "k_out and v_out must be 16-byte aligned pointers");
+  a.k_out = k_out;
+  a.v_out = v_out;
+  QWA_CUDA(ctx, launch_kv_read(a, cache->dtype == QWA_BF16, cache->format,
+                               static_cast<cudaStream_t>(stream)));
+  return QWA_OK;
+}
+
+// ------------------------------------------------- shared-prefix attention
+namespace {
+
+qwa_status prefix_shape(qwa_ctx* ctx, const int32_t* cu_q, const int32_t* cu_k, int batch,
+                        int q_heads, int kv_heads, int prefix_len, int mode, int sparse_prefix,
+                        int window, PrefixShape* out) {
+  int total_q = 0, total_k = 0, max_q = 0, max_k = 0;
+  qwa_status st = check_cu(ctx, cu_q, batch, &total_q, &max_q);
+  if (st == QWA_OK) st = check_cu(ctx, cu_k, batch, &total_k, &max_k);
+  if (st != QWA_OK) return st;
+  for (int b = 0; b < batch; ++b)
+    if (cu_k[b + 1] - cu_k[b] < cu_q[b + 1] - cu_q[b])
+      return fail(ctx, QWA_ERR_INVALID_ARG,
+                  "request %d has more queries than own keys (a query is its own key)", b);
+  if (kv_heads < 1 || q_heads < kv_heads || q_heads % kv_heads != 0 || q_heads / kv_heads > 128)
+    return fail(ctx, QWA_ERR_UNSUPPORTED,
+                "q_heads must be a multiple of kv_heads, at most 128 times (got %d / %d)", q_heads,
+                kv_heads);
+  if (mode < QWA_MODE_AUTO || mode > QWA_MODE_SPARSE)
+    return fail(ctx, QWA_ERR_INVALID_ARG, "unknown mode %d", mode);
+  if (prefix_len < 0 || static_cast<int64_t>(prefix_len) + max_k > (1 << 30))
+    return fail(ctx, QWA_ERR_INVALID_ARG, "prefix_len must be >= 0, positions at most 2^30");
+  if (sparse_prefix < 0 || sparse_prefix > (1 << 30) || window < 1 || window > (1 << 30))
+    return fail(ctx, QWA_ERR_INVALID_ARG,
+                "sparse_prefix must be in 0..2^30 and window in 1..2^30");
+  const int group = q_heads / kv_heads;
+  *out = PrefixShape{batch, q_heads, kv_heads, prefix_len,
+                     resolve_sparse(mode, prefix_len + max_k), sparse_prefix, window,
+                     128 / group, 2 * (128 / group)};
+  return QWA_OK;
+}
+
+// CTAs of a cluster that share a block's tiles: as many as keep the SMs busy,
+// each with a tile at least.
+int prefix_splits(const PrefixWork& w, int items, int sms) {
+  int least = 1 << 30;
+  for (const PrefixItem& i : w.items) least = std::min(least, i.tile_end - i.tile_beg);
+  const int s = std::min(std::min(8, sms / std::max(items, 1)), least);
+  return std::max(s, 1);
+}
+
+qwa_status create_prefix_plan(qwa_ctx* ctx, const int32_t* cu_q, const int32_t* cu_k,
+                              const PrefixShape& shape, qwa_prefix_plan** out) {
+  auto plan = std::make_unique<qwa_prefix_plan>();
+  plan->device = ctx->device;
+  plan->shape = shape;
+  plan->total_q = cu_q[shape.batch];
+  plan->total_k = cu_k[shape.batch];
+  if (plan->total_q > 0) {
+    const PrefixWork w = build_prefix_work(shape, cu_q, cu_k);
+    const int blocks = static_cast<int>(w.items.size());
+    const int64_t n = static_cast<int64_t>(blocks) * shape.kv_heads;
+    if (n > 0x7fffffff / 8)
+      return fail(ctx, QWA_ERR_UNSUPPORTED, "too many blocks of rows (%lld)",
+                  static_cast<long long>(n));
+    std::vector<PrefixItem> items;
+    items.reserve(n);
+    std::vector<int> offsets(1, 0);
+    plan->splits = prefix_splits(w, static_cast<int>(n), ctx->sms);
+    if (plan->splits > 1) {
+      for (int i = 0; i < blocks; ++i)
+        for (int g = 0; g < shape.kv_heads; ++g) {
+          items.push_back(w.items[i]);
+          items.back().head = g;
+        }
+      plan->grid = static_cast<int>(n) * plan->splits;
+    } else {
+      // list scheduling: the longest block first, to the least loaded CTA
+      std::vector<int> order(blocks);
+      for (int i = 0; i < blocks; ++i) order[i] = i;
+      std::stable_sort(order.begin(), order.end(),
+                       [&](int a, int b) { return w.cost[a] > w.cost[b]; });
+      const int ctas = static_cast<int>(std::min<int64_t>(n, ctx->sms));
+      std::vector<std::vector<std::pair<int, int>>> per_cta(ctas);
+      std::vector<std::pair<double, int>> heap;
+      for (int c = 0; c < ctas; ++c) heap.push_back({0.0, c});
+      const auto later = std::greater<std::pair<double, int>>();
+      for (int i : order)
+        for (int g = 0; g < shape.kv_heads; ++g) {
+          std::pop_heap(heap.begin(), heap.end(), later);
+          per_cta[heap.back().second].push_back({i, g});
+          heap.back().first += w.cost[i];
+          std::push_heap(heap.begin(), heap.end(), later);
+        }
+      for (int c = 0; c < ctas; ++c) {
+        for (const auto& ig : per_cta[c]) {
+          items.push_back(w.items[ig.first]);
+          items.back().head = ig.second;
+        }
+        offsets.push_back(static_cast<int>(items.size()));
+      }
+      plan->grid = ctas;
+    }
+    const size_t b_items = items.size() * sizeof(PrefixItem);
+    const size_t b_tiles = w.tiles.size() * sizeof(PrefixTile);
+    const size_t b_rows = w.rows.size() * sizeof(PrefixRow);
+    const size_t b_off = offsets.size() * sizeof(int);
+    std::vector<uint8_t> host(b_items + b_tiles + b_rows + b_off);
+    std::memcpy(host.data(), items.data(), b_items);
+    std::memcpy(host.data() + b_items, w.tiles.data(), b_tiles);
+    std::memcpy(host.data() + b_items + b_tiles, w.rows.data(), b_rows);
+    std::memcpy(host.data() + b_items + b_tiles + b_rows, offsets.data(), b_off);
+    if (!ctx->upload)
+      QWA_CUDA(ctx, cudaStreamCreateWithFlags(&ctx->upload, cudaStreamNonBlocking));
+    QWA_CUDA(ctx, cudaMalloc(&plan->memory, host.size()));
+    cudaError_t e = cudaMemcpyAsync(plan->memory, host.data(), host.size(),
+                                    cudaMemcpyHostToDevice, ctx->upload);
+    // waited for here, so that any stream may use the plan
+    if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->upload);
+    if (e != cudaSuccess) {
+      cudaFree(plan->memory);
+      return fail(ctx, QWA_ERR_CUDA, "copying a prefix plan failed: %s", cudaGetErrorString(e));
+    }
+    uint8_t* p = static_cast<uint8_t*>(plan->memory);
+    plan->items = reinterpret_cast<const PrefixItem*>(p);
+    plan->tiles = reinterpret_cast<const PrefixTile*>(p + b_items);
+    plan->rows = reinterpret_cast<const PrefixRow*>(p + b_items + b_tiles);
+    plan->offsets = reinterpret_cast<const int*>(p + b_items + b_tiles + b_rows);
+  }
+  *out = plan.release();
+  return QWA_OK;
+}
+
+}  // namespace
+
+qwa_status qwa_prefix_plan_create(qwa_ctx* ctx, const int32_t* cu_seqlens_q_host,
+                                  const int32_t* cu_seqlens_k_host, int batch, int q_heads,
+                                  int kv_heads, int prefix_len, int mode, int sparse_prefix,
+                                  int window, qwa_prefix_plan** out) {
+  if (!ctx || !out) return QWA_ERR_INVALID_ARG;
+  *out = nullptr;
+  DeviceGuard guard(ctx->device);
+  try {
+    const int32_t* cu_k = cu_seqlens_k_host ? cu_seqlens_k_host : cu_seqlens_q_host;
+    PrefixShape shape;
+    qwa_status st = prefix_shape(ctx, cu_seqlens_q_host, cu_k, batch, q_heads, kv_heads,
+                                 prefix_len, mode, sparse_prefix, window, &shape);
+    if (st != QWA_OK) return st;
+    return create_prefix_plan(ctx, cu_seqlens_q_host, cu_k, shape, out);
+  } catch (const std::exception&) {
+    return fail(ctx, QWA_ERR_CUDA, "out of host memory for a prefix plan");
+  }
+}
+
+qwa_status qwa_prefix_plan_destroy(qwa_prefix_plan* plan) {
+  if (!plan) return QWA_OK;
+  {
+    DeviceGuard guard(plan->device);
+    if (plan->memory) cudaFree(plan->memory);  // waits for launches that read it
+  }
+  delete plan;
+  return QWA_OK;
+}
+
+qwa_status qwa_prefix_attention(qwa_ctx* ctx, const qwa_prefix_plan* plan, int dtype,
+                                const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+                                const void* v, int64_t v_stride, void* out,
+                                const qwa_kv_cache* cache, int64_t first_slot, void* stream) {
+  if (!ctx) return QWA_ERR_INVALID_ARG;
+  if (!plan) return fail(ctx, QWA_ERR_INVALID_ARG, "plan is NULL");
+  if (plan->device != ctx->device)
+    return fail(ctx, QWA_ERR_INVALID_ARG, "the plan belongs to device %d, the context to %d",
+                plan->device, ctx->device);
+  if (!good_dtype(dtype)) return fail(ctx, QWA_ERR_UNSUPPORTED, "dtype must be f16 or bf16");
+  DeviceGuard guard(ctx->device);
+  const PrefixShape& s = plan->shape;
+  if (plan->total_q == 0) return QWA_OK;
+  if (!q || !k || !v || !out) return fail(ctx, QWA_ERR_INVALID_ARG, "NULL tensor pointer");
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out))
+    return fail(ctx, QWA_ERR_INVALID_ARG, "q, k, v and out must be 16-byte aligned");
+  const int64_t q_width = static_cast<int64_t>(s.q_heads) * kHeadDim;
+  const int64_t kv_width = static_cast<int64_t>(s.kv_heads) * kHeadDim;
+  if (q_stride < q_width || q_stride % 8 != 0 || k_stride < kv_width || k_stride % 8 != 0 ||
+      v_stride < kv_width || v_stride % 8 != 0)
+    return fail(ctx, QWA_ERR_INVALID_ARG,
+                "strides must be multiples of 8 and at least heads * 128");
+  qwa_status st;
+  int format = QWA_KV_PLAIN;
+  if (s.prefix_len > 0) {
+    if ((st = check_cache(ctx, cache)) != QWA_OK) return st;
+    if (cache->dtype != dtype || cache->heads != s.kv_heads || cache->head_dim != kHeadDim)
+      return fail(ctx, QWA_ERR_INVALID_ARG,
+                  "the cache must have q's dtype, %d heads and head_dim 128", s.kv_heads);
+    if (first_slot < 0 || first_slot + s.prefix_len > cache->slots)
+      return fail(ctx, QWA_ERR_INVALID_ARG, "the prefix's slots %lld..%lld are not in the cache",
+                  static_cast<long long>(first_slot),
+                  static_cast<long long>(first_slot + s.prefix_len - 1));
+    format = cache->format;
+  }
+  if ((st = ensure_encode(ctx)) != QWA_OK) return st;
+  const bool bf16 = dtype == QWA_BF16;
+  PrefixMaps m;
+  const uint32_t group = static_cast<uint32_t>(s.q_heads / s.kv_heads);
+  if ((st = make_map(ctx, &m.q, q, s.q_heads, plan->total_q, q_stride * 2,
+                     static_cast<uint32_t>(s.tile_tokens), group, bf16)) != QWA_OK)
+    return st;
+  if ((st = make_map(ctx, &m.k, k, s.kv_heads, plan->total_k, k_stride * 2, 128, 1, bf16)) !=
+      QWA_OK)
+    return st;
+  if ((st = make_map(ctx, &m.v, v, s.kv_heads, plan->total_k, v_stride * 2, 128, 1, bf16)) !=
+      QWA_OK)
+    return st;
+  m.pk = m.k;
+  m.pv = m.v;
+  PrefixArgs a{};
+  if (s.prefix_len > 0) {
+    const int64_t at = first_slot * kv_width * (format == QWA_KV_PLAIN ? 2 : 1);
+    a.k_prefix = static_cast<const uint8_t*>(cache->k) + at;
+    a.v_prefix = static_cast<const uint8_t*>(cache->v) + at;
+    if (format == QWA_KV_PLAIN) {
+      if ((st = make_map(ctx, &m.pk, a.k_prefix, s.kv_heads, s.prefix_len, kv_width * 2, 128, 1,
+                         bf16)) != QWA_OK)
+        return st;
+      if ((st = make_map(ctx, &m.pv, a.v_prefix, s.kv_heads, s.prefix_len, kv_width * 2, 128, 1,
+                         bf16)) != QWA_OK)
+        return st;
+    } else {
+      a.k_scale = cache->k_scale + first_slot * s.kv_heads;
+      a.v_scale = cache->v_scale + first_slot * s.kv_heads;
+    }
+  }
+  a.items = plan->items;
+  a.tiles = plan->tiles;
+  a.rows = plan->rows;
+  a.cta_offsets = plan->offsets;
+  a.splits = plan->splits;
+  a.v_own = static_cast<const uint16_t*>(v);
+  a.v_stride = v_stride;
+  a.out = static_cast<uint16_t*>(out);
+  a.q_heads = s.q_heads;
+  a.kv_heads = s.kv_heads;
+  a.group = static_cast<int>(group);
+  a.tile_tokens = s.tile_tokens;
+  a.prefix_len = s.prefix_len;
+  a.sparse = s.sparse;
+  a.sparse_prefix = s.sparse_prefix;
+  a.window = s.window;
+  a.scale_log2 = kScale * kLog2e;
+  a.status = ctx->d_status;
+  a.wait_ns = ctx->wait_ns;
+  QWA_CUDA(ctx, launch_prefix_attention(m, a, bf16, format, plan->grid,
+                                        static_cast<cudaStream_t>(stream)));
+  return QWA_OK;
+}
+
+qwa_status qwa_prefix_attention_work(const int32_t* cu_seqlens_q_host,
+                                     const int32_t* cu_seqlens_k_host, int batch, int q_heads,
+                                     int kv_heads, int prefix_len, int mode, int sparse_prefix,
+                                     int window, int64_t* kept_pairs, int64_t* visited_tiles) {
+  try {
+    const int32_t* cu_k = cu_seqlens_k_host ? cu_seqlens_k_host : cu_seqlens_q_host;
+    PrefixShape s;
+    qwa_status st = prefix_shape(nullptr, cu_seqlens_q_host, cu_k, batch, q_heads, kv_heads,
+                                 prefix_len, mode, sparse_prefix, window, &s);
+    if (st != QWA_OK) return st;
+    if (kept_pairs) *kept_pairs = prefix_kept_pairs(s, cu_seqlens_q_host, cu_k);
+    if (visited_tiles)
+      *visited_tiles = static_cast<int64_t>(
+                           build_prefix_work(s, cu_seqlens_q_host, cu_k).tiles.size()) *
+                       kv_heads;
+    return QWA_OK;
+  } catch (const std::exception&) {
+    return QWA_ERR_CUDA;
+  }
 }
 
 #ifdef QWA_TRACE

@@ -230,4 +230,52 @@ cudaError_t launch_swiglu(const __half* combined, __half* out, int rows, int wid
 cudaError_t launch_q6k_embedding(const uint32_t* ids, const uint8_t* table, int vocab,
                                  __half* out, int tokens, int width, cudaStream_t stream);
 
+// ------------------------------------------- rotary positions (rope.cu)
+constexpr int kMaxRotary = 256;
+struct RopeFrequencies {
+  double f[kMaxRotary / 2];  // radians a position
+  double m;                  // factor of every cos and sin
+  int half;                  // rotary / 2
+};
+cudaError_t launch_rope_table(const RopeFrequencies& fr, float2* table, int64_t first,
+                              int positions, cudaStream_t stream);
+
+struct RopeSide {  // q or k: [tokens, heads, head_dim] of 16-bit values, strides in elements
+  const uint16_t* in;
+  uint16_t* out;
+  int64_t in_stride, in_head_stride, out_stride, out_head_stride;
+  int heads;
+};
+struct RopeArgs {
+  RopeSide q, k;
+  const int32_t* positions;
+  const float2* table;  // [table_rows, rotary / 2]
+  int table_rows, tokens, head_dim, rotary, layout, inverse;
+  int smem_heads;  // heads a block stages at a time
+  __device__ __forceinline__ const uint16_t* in_row(int64_t t, int h) const {
+    return h < q.heads ? q.in + t * q.in_stride + h * q.in_head_stride
+                       : k.in + t * k.in_stride + (h - q.heads) * k.in_head_stride;
+  }
+  __device__ __forceinline__ uint16_t* out_row(int64_t t, int h) const {
+    return h < q.heads ? q.out + t * q.out_stride + h * q.out_head_stride
+                       : k.out + t * k.out_stride + (h - q.heads) * k.out_head_stride;
+  }
+};
+cudaError_t launch_rope(RopeArgs args, int bf16, cudaStream_t stream);
+
+// ------------------------------------------------ 8-bit cache (kv_cache.cu)
+enum KvFormat : int { kKvPlain = 0, kKvE4M3 = 1, kKvInt8 = 2 };  // qwa_kv_format
+struct KvCacheArgs {
+  void *k, *v;                 // [slots, heads, head_dim] codes
+  uint8_t *k_scale, *v_scale;  // [slots, heads] exponent + 127
+  int64_t slots;
+  int heads, head_dim, tokens;
+  const int32_t* slot_of;  // [tokens]
+  const void *k_in, *v_in;
+  int64_t k_stride, v_stride;  // elements a token
+  void *k_out, *v_out;
+};
+cudaError_t launch_kv_write(const KvCacheArgs& args, int bf16, int format, cudaStream_t stream);
+cudaError_t launch_kv_read(const KvCacheArgs& args, int bf16, int format, cudaStream_t stream);
+
 }  // namespace qwa

@@ -1,0 +1,978 @@
+// Attention of a batch of requests behind one cached prefix (tcgen05 + TMA).
+//
+//   o_r = sum_j p_rj v_j / sum_j p_rj,  p_rj = exp(q_r . k_j / sqrt(128) - m_r)
+//
+// over the keys j that row r keeps: the prefix's, then its request's own up to
+// itself (prefix_plan.h has the rule and the lists of work).
+//
+// A block of work is `tile_tokens` x 2 packed query tokens x the `group` query
+// heads of one kv head: two 128-row tiles A and B, row = token * group + head.
+// Rows of different requests share a tile, so the prefix is read and
+// multiplied once for the whole block; own keys of other requests are masked.
+//
+// Warp roles (384 threads):
+//   warp 0      TMA producer: Q tiles, then K_j / V_j into a 3-slot ring
+//   warp 1      TMEM owner; lane 0 issues every tcgen05.mma and commit
+//   warps 2-3   prepare tiles: 8-bit prefix tiles are read with plain loads,
+//               converted and written to their slot; V tiles with masked keys
+//               are cleared of values that are not finite (guard, below)
+//   warps 4-7   softmax of tile A, one thread a row
+//   warps 8-11  softmax of tile B
+// TMEM: S_A, S_B (P over them, as 16-bit pairs), O_A, O_B; 512 columns.
+// MMA order per key tile: S_A(j), PV_B(j-1), S_B(j), PV_A(j), so the softmax of
+// one tile runs under the MMAs of the other.
+//
+// Guard. A masked key has p = 0, but the MMA still multiplies: 0 * inf = NaN
+// would reach rows of other requests. So V tiles in which some row drops a key
+// are searched, values that are not finite replaced by 0, and the rows that
+// keep such a key get it back in the epilogue (found again by a slow search).
+//
+// Split. With few blocks the tiles of a block are dealt to a cluster of 2, 4 or
+// 8 CTAs, each with its own running maximum and sum; at the end every CTA
+// leaves its O, m and l in shared memory and merges a share of the rows from
+// all of them. No workspace, one launch, and an order that does not vary.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "attn_common.cuh"
+#include "convert.cuh"
+#include "internal.h"
+#include "prefix_attention.h"
+#include "ptx.cuh"
+
+namespace qwa {
+namespace {
+using namespace attn;
+
+constexpr int kThreads = 384;
+constexpr int kSoftmaxWarp0 = 4;
+constexpr int kRegsSupport = 104;
+constexpr int kRegsSoftmax = 200;
+static_assert(128 * kRegsSupport + 256 * kRegsSoftmax <= kThreads * 168, "register split");
+constexpr uint32_t kQEmptyArrivals = 8;
+constexpr uint32_t kSlotFullArrivals = 2;  // the two preparing warps, or the producer twice
+constexpr int kSlots = 3;
+constexpr uint32_t kQBufBytes = 2 * kTileBytes;
+constexpr uint32_t kSlotOff = 2 * kQBufBytes;
+constexpr uint32_t kStatOff = kSlotOff + kSlots * kTileBytes;  // split: (m, l) of 256 rows
+constexpr uint32_t kBarOff = kStatOff + 256 * 8;
+enum Bar : int {
+  kQFull = 0,
+  kQEmpty = kQFull + 2,
+  kSlotFull = kQEmpty + 2,
+  kSlotEmpty = kSlotFull + kSlots,
+  kRawFull = kSlotEmpty + kSlots,  // a guarded V tile has landed, not yet searched
+  kSFull = kRawFull + kSlots,
+  kPLo = kSFull + 2,
+  kPHi = kPLo + 2,
+  kOFinal = kPHi + 2,
+  kDrain = kOFinal + 2,
+  kNumBars = kDrain + 1
+};
+constexpr uint32_t kHolderOff = kBarOff + 8 * kNumBars;
+constexpr uint32_t kAbortOff = kHolderOff + 4;
+constexpr uint32_t kLimitOff = (kHolderOff + 8 + 7) / 8 * 8;
+// li + 1 of the last item with values put aside, by li % 4: the preparing
+// warps run at most two items ahead of an epilogue
+constexpr uint32_t kBadOff = kLimitOff + 8;
+constexpr uint32_t kSmemUsed = kBadOff + 16;
+constexpr uint32_t kSmemBytes = 232448;  // all of it: what is over covers the alignment to 1024
+static_assert(kSmemUsed + 768 <= kSmemBytes, "shared memory budget");
+
+template <bool kBf16>
+__host__ __device__ constexpr uint32_t idesc_16(uint32_t m, uint32_t n, bool b_mn_major) {
+  // A and B format: 0 = f16, 1 = bf16
+  return idesc_f16_f32(m, n, b_mn_major) | (kBf16 ? (1u << 7) | (1u << 10) : 0u);
+}
+
+// One half of PV (keys 0..63 or 64..127): at most `nk` steps of 16 in all.
+template <bool kBf16>
+__device__ __forceinline__ void issue_pv_part(uint32_t d_tmem, uint32_t p_tmem, uint64_t v_desc,
+                                              bool accumulate, int nk, int half) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int kk = 4 * half + i;
+    if (kk < nk)
+      mma_ts(d_tmem, p_tmem + kk * 8, v_desc + ((kk * 2048) >> 4), idesc_16<kBf16>(128, 128, true),
+             (accumulate || kk > 0) ? 1u : 0u);
+  }
+}
+
+// exp2(a * scale - m) of 32 scores, packed to 16-bit pairs in a[0..15]; returns
+// their sum (of the unrounded values, in f32).
+template <bool kBf16>
+__device__ __forceinline__ float exp_pack(uint32_t (&a)[32], float scale, float m) {
+  const uint64_t s2 = f2_pack(scale, scale), nm2 = f2_pack(-m, -m);
+  uint64_t sum2 = f2_pack(0.f, 0.f);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    float y0, y1;
+    f2_unpack(fma2(f2_pack(__uint_as_float(a[2 * i]), __uint_as_float(a[2 * i + 1])), s2, nm2),
+              y0, y1);
+    const float e0 = ex2(y0), e1 = ex2(y1);
+    sum2 = add2(sum2, f2_pack(e0, e1));
+    a[i] = pack2<kBf16>(e0, e1);
+  }
+  float sum0, sum1;
+  f2_unpack(sum2, sum0, sum1);
+  return sum0 + sum1;
+}
+
+// The keys that a row keeps, in the numbering of one key tensor: [lo, hi], of
+// those (sparse) only < cut or >= wlo.
+struct Kept {
+  int lo, hi, cut, wlo;
+};
+__device__ __forceinline__ Kept kept_keys(const PrefixArgs& a, bool own, PrefixRow r) {
+  if (own) {
+    const int own_prefix = max(0, a.sparse_prefix - a.prefix_len);
+    return {r.lo, r.hi, r.lo + own_prefix, max(0, r.hi - a.window + 1)};
+  }
+  return {0, a.prefix_len - 1, a.sparse_prefix,
+          max(0, a.prefix_len + r.hi - r.lo - a.window + 1)};
+}
+__device__ __forceinline__ uint32_t kept_bits(const Kept& k, int k0, int sparse) {
+  uint32_t m = low_bits(k.hi - k0 + 1) & ~low_bits(k.lo - k0);
+  if (sparse) m &= low_bits(k.cut - k0) | ~low_bits(k.wlo - k0);
+  return m;
+}
+__device__ __forceinline__ void mask_keys(uint32_t (&a)[32], const Kept& k, int k0, int sparse) {
+  const uint32_t m = kept_bits(k, k0, sparse);
+  if (__all_sync(0xffffffffu, m == 0xffffffffu)) return;
+#pragma unroll
+  for (int c = 0; c < 32; ++c)
+    if (!((m >> c) & 1u)) a[c] = __float_as_uint(-INFINITY);
+}
+
+// ------------------------------------------------------------- 8-bit tiles
+// 2^e as two equal 16-bit (f16) values; out of f16's range it is 0 or inf.
+__device__ __forceinline__ uint32_t half2_pow2(int e) {
+  uint32_t h;
+  if (e > 15) h = 0x7c00u;
+  else if (e >= -14) h = static_cast<uint32_t>(e + 15) << 10;
+  else if (e >= -24) h = 1u << (e + 24);
+  else h = 0u;
+  return h | (h << 16);
+}
+
+// Two codes (the low 16 bits) -> the 16-bit pair of values that they stand for.
+template <bool kBf16, int kFormat>
+__device__ __forceinline__ uint32_t code_pair(uint32_t codes, uint32_t scale_h2, float scale_a,
+                                              float scale_b) {
+  uint32_t h;
+  if constexpr (kFormat == kKvE4M3) {
+    h = e4m3x2_to_half2(codes);
+  } else {
+    // 1024 + (code + 128) has the code's bits in an f16's low byte
+    const uint32_t u = __byte_perm(codes ^ 0x8080u, 0x64646464u, 0x4140);
+    const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&u),
+                              __floats2half2_rn(1152.f, 1152.f));
+    h = *reinterpret_cast<const uint32_t*>(&v);
+  }
+  if constexpr (kBf16) {
+    const float2 f = unpack2<false>(h);
+    return pack2<true>(f.x * scale_a * scale_b, f.y * scale_a * scale_b);
+  } else {
+    const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&h),
+                              *reinterpret_cast<const __half2*>(&scale_h2));
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+
+// Clears the halves of w whose exponent is all ones (inf, NaN).
+template <bool kBf16>
+__device__ __forceinline__ uint32_t finite_only(uint32_t w, bool& bad) {
+  constexpr uint32_t kExp = kBf16 ? 0x7f807f80u : 0x7c007c00u;
+  const uint32_t hit = __vcmpeq2(w & kExp, kExp);
+  bad |= hit != 0;
+  return w & ~hit;
+}
+
+__device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t x, uint32_t y, uint32_t z,
+                                             uint32_t w) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y), "r"(z),
+               "r"(w)
+               : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
+// The raw codes of one prefix tile, held by 64 threads: thread (w, lane) has
+// the 16 codes of unit lane % 8 in the rows 8 i + 4 w + lane / 8.
+struct RawTile {
+  uint4 code[16];
+  uint32_t scale;  // bytes of rows i = lane / 4 (low) and i = 8 + lane / 4, sub-row lane % 4
+};
+__device__ __forceinline__ void load_raw(RawTile& raw, const uint8_t* codes, const uint8_t* scales,
+                                         int kv_heads, int head, int key, int rows, int w,
+                                         int lane) {
+  const int64_t stride = static_cast<int64_t>(kv_heads) * kHeadDim;
+  const uint8_t* src = codes + key * stride + head * kHeadDim + (lane & 7) * 16;
+  const int r0 = 4 * w + (lane >> 3);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int r = r0 + 8 * i;
+    raw.code[i] = r < rows ? __ldg(reinterpret_cast<const uint4*>(src + r * stride))
+                           : make_uint4(0u, 0u, 0u, 0u);
+  }
+  raw.scale = 0x7f7fu;  // 2^0 for rows that do not exist
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = 8 * (8 * i + (lane >> 2)) + 4 * w + (lane & 3);
+    if (r < rows) {
+      const uint32_t s = __ldg(scales + static_cast<int64_t>(key + r) * kv_heads + head);
+      raw.scale = (raw.scale & ~(0xffu << (8 * i))) | (s << (8 * i));
+    }
+  }
+}
+// Converts it into the slot's swizzled layout. guard: values that are not
+// finite become 0; returns whether there were any.
+template <bool kBf16, int kFormat>
+__device__ __forceinline__ bool store_raw(const RawTile& raw, uint32_t slot, bool guard, int w,
+                                          int lane) {
+  bool bad = false;
+  const int u = lane & 7;                       // dims 16 u .. 16 u + 15
+  const uint32_t half_base = slot + (u >> 2) * kHalfBytes;
+  const int first = u >> 2;  // lanes of the second half write their odd unit first (banks)
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int r = 8 * i + 4 * w + (lane >> 3);
+    const uint32_t both = __shfl_sync(0xffffffffu, raw.scale, (i & 7) * 4 + (lane >> 3));
+    const int e = static_cast<int>((both >> (8 * (i >> 3))) & 0xffu) - 127;
+    const uint32_t h2 = half2_pow2(e);
+    const float sa = pow2f(e / 2), sb = pow2f(e - e / 2);
+    const uint32_t c[4] = {raw.code[i].x, raw.code[i].y, raw.code[i].z, raw.code[i].w};
+    uint32_t v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      v[j] = code_pair<kBf16, kFormat>((c[j >> 1] >> (16 * (j & 1))) & 0xffffu, h2, sa, sb);
+      if (guard) v[j] = finite_only<kBf16>(v[j], bad);
+    }
+    const uint32_t row = half_base + r * 128;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int which = j ^ first;
+      const uint32_t unit = static_cast<uint32_t>((u & 3) * 2 + which) ^ (r & 7);
+      if (which == 0) st_shared_v4(row + unit * 16, v[0], v[1], v[2], v[3]);
+      else st_shared_v4(row + unit * 16, v[4], v[5], v[6], v[7]);
+    }
+  }
+  return bad;
+}
+// Clears a landed V tile (rows [0, width)) of values that are not finite.
+template <bool kBf16>
+__device__ __forceinline__ bool guard_tile(uint32_t slot, int width, int w, int lane) {
+  bool bad = false;
+  for (int r = 4 * w + (lane >> 3); r < width; r += 8) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t at = slot + h * kHalfBytes + r * 128 + (lane & 7) * 16;
+      uint4 v = ld_shared_v4(at);
+      bool hit = false;
+      v.x = finite_only<kBf16>(v.x, hit);
+      v.y = finite_only<kBf16>(v.y, hit);
+      v.z = finite_only<kBf16>(v.z, hit);
+      v.w = finite_only<kBf16>(v.w, hit);
+      if (hit) st_shared_v4(at, v.x, v.y, v.z, v.w);
+      bad |= hit;
+    }
+  }
+  return bad;
+}
+
+// What a row gets back for the values that the guard put aside: per dim of a
+// 32-dim chunk whether it keeps a key with +inf, -inf or NaN there.
+struct Aside {
+  uint32_t pos, neg, nan;
+};
+template <bool kBf16, int kFormat>
+__device__ __noinline__ Aside find_aside(const PrefixArgs& a, int tile_beg, int tile_end,
+                                         PrefixRow row, int head, int chunk) {
+  Aside s{0u, 0u, 0u};
+  for (int j = tile_beg; j < tile_end; ++j) {
+    const PrefixTile tile = a.tiles[j];
+    if (!(tile.info & kTileGuard)) continue;
+    const bool own = tile.info & kTileOwn;
+    const Kept k = kept_keys(a, own, row);
+    const int width = tile.info & kTileWidthMask;
+    for (int c = 0; c < width; c += 32) {
+      uint32_t bits = kept_bits(k, tile.key + c, a.sparse);
+      if (width - c < 32) bits &= low_bits(width - c);
+      for (; bits; bits &= bits - 1) {
+        const int64_t key = tile.key + c + __ffs(bits) - 1;
+        for (int d = 0; d < 32; ++d) {
+          const int dim = chunk * 32 + d;
+          uint32_t v;
+          if (own) {
+            v = a.v_own[key * a.v_stride + head * kHeadDim + dim];
+          } else if (kFormat == kKvPlain) {
+            v = static_cast<const uint16_t*>(
+                a.v_prefix)[(key * a.kv_heads + head) * kHeadDim + dim];
+          } else {
+            const int64_t at = key * a.kv_heads + head;
+            const int e = static_cast<int>(a.v_scale[at]) - 127;
+            const uint32_t code = static_cast<const uint8_t*>(a.v_prefix)[at * kHeadDim + dim];
+            v = code_pair<kBf16, kFormat>(code, half2_pow2(e), pow2f(e / 2), pow2f(e - e / 2)) &
+                0xffffu;
+          }
+          constexpr uint32_t kExp = kBf16 ? 0x7f80u : 0x7c00u;
+          if ((v & kExp) != kExp) continue;
+          if ((v & 0x7fffu) != kExp) s.nan |= 1u << d;
+          else if (v & 0x8000u) s.neg |= 1u << d;
+          else s.pos |= 1u << d;
+        }
+      }
+    }
+  }
+  return s;
+}
+__device__ __forceinline__ float with_aside(float o, const Aside& s, int d) {
+  if ((s.nan >> d) & 1u) o += NAN;
+  if ((s.pos >> d) & 1u) o += INFINITY;
+  if ((s.neg >> d) & 1u) o -= INFINITY;
+  return o;
+}
+
+__device__ __forceinline__ float4 ld_cluster_v4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 ld_cluster_v2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+
+// The work of one CTA: items [beg, end) of the list with all their tiles, or
+// (split) the share `rank` of `ranks` of one item's tiles.
+struct Share {
+  int beg, end, rank, ranks;
+};
+template <bool kSplit>
+__device__ __forceinline__ Share my_share(const PrefixArgs& a) {
+  if constexpr (kSplit) {
+    const int item = blockIdx.x / a.splits;
+    return {item, item + 1, static_cast<int>(cluster_ctarank()), a.splits};
+  } else {
+    return {a.cta_offsets[blockIdx.x], a.cta_offsets[blockIdx.x + 1], 0, 1};
+  }
+}
+template <bool kSplit>
+__device__ __forceinline__ void share_tiles(const Share& s, const PrefixItem& item, int& beg,
+                                            int& end) {
+  beg = item.tile_beg;
+  end = item.tile_end;
+  if constexpr (kSplit) {
+    const int n = end - beg;
+    end = beg + n * (s.rank + 1) / s.ranks;
+    beg = beg + n * s.rank / s.ranks;
+  }
+}
+
+template <bool kBf16, int kFormat, bool kSplit>
+__global__ void __launch_bounds__(kThreads, 1)
+    prefix_attention_kernel(const __grid_constant__ CUtensorMap tm_q,
+                            const __grid_constant__ CUtensorMap tm_k,
+                            const __grid_constant__ CUtensorMap tm_v,
+                            const __grid_constant__ CUtensorMap tm_pk,
+                            const __grid_constant__ CUtensorMap tm_pv,
+                            const __grid_constant__ PrefixArgs args) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  if (smem - smem_raw + kSmemUsed > kSmemBytes) {  // the same in every CTA
+    if (threadIdx.x == 0) atomicCAS(args.status, 0, kDevSharedLayout);
+    return;
+  }
+  const uint32_t sbase = smem_addr(smem);
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + kHolderOff);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kAbortOff);
+  volatile unsigned long long* wait_limit =
+      reinterpret_cast<volatile unsigned long long*>(smem + kLimitOff);
+  volatile int* bad_item = reinterpret_cast<volatile int*>(smem + kBadOff);
+  auto bar = [&](int i) -> uint32_t { return sbase + kBarOff + 8u * i; };
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const Share share = my_share<kSplit>(args);
+
+  if (threadIdx.x == 0) {
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(bar(kQFull + b), 1);
+      mbar_init(bar(kQEmpty + b), kQEmptyArrivals);
+      bad_item[2 * b] = bad_item[2 * b + 1] = 0;
+    }
+    for (int s = 0; s < kSlots; ++s) {
+      mbar_init(bar(kSlotFull + s), kSlotFullArrivals);
+      mbar_init(bar(kSlotEmpty + s), 1);
+      mbar_init(bar(kRawFull + s), 1);
+    }
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(bar(kSFull + x), 1);
+      mbar_init(bar(kPLo + x), 128);
+      mbar_init(bar(kPHi + x), 128);
+      mbar_init(bar(kOFinal + x), 1);
+    }
+    mbar_init(bar(kDrain), 1);
+    *abort_flag = 0;
+    *wait_limit = args.wait_ns;
+    fence_mbar_init();
+    tma_prefetch_desc(&tm_q);
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+    if (kFormat == kKvPlain) {
+      tma_prefetch_desc(&tm_pk);
+      tma_prefetch_desc(&tm_pv);
+    }
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_addr(tmem_holder), kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+  // rows of a 128-row tile that a Q load fills
+  const int tile_rows = args.group * args.tile_tokens;
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsSupport));
+    if (warp == 0) {
+      // ---------------------------------------------------------- producer
+      if (lane == 0) {
+        int c = 0;
+        bool ok = true;
+        // phases whose copies may be in flight at the end: bit i + 8 valid, bit
+        // i parity; i = slot (full), 3 + slot (raw), 6 + Q buffer
+        uint32_t flying = 0;
+        uint32_t raw_uses = 0;  // bit s: parity of the next raw phase of slot s
+        auto fly = [&](int i, uint32_t parity) {
+          flying = (flying & ~(1u << i)) | (1u << (i + 16)) | (parity << i);
+        };
+        for (int it = share.beg, li = 0; ok && it < share.end; ++it, ++li) {
+          const PrefixItem item = args.items[it];
+          int tb, te;
+          share_tiles<kSplit>(share, item, tb, te);
+          const int qb = li & 1;
+          const int nx = item.tokens > args.tile_tokens ? 2 : 1;
+          if (!(ok = mbar_wait(bar(kQEmpty + qb), ((li >> 1) & 1) ^ 1, abort_flag, args.status,
+                               kDevTimeoutQ, wait_limit)))
+            break;
+          mbar_arrive_expect_tx(bar(kQFull + qb), nx * tile_rows * 256);
+          fly(2 * kSlots + qb, (li >> 1) & 1);
+          for (int x = 0; x < nx; ++x) {
+            const uint32_t dst = sbase + qb * kQBufBytes + x * kTileBytes;
+            const int t0 = item.row0 + x * args.tile_tokens;
+            tma_load_3d(dst, &tm_q, bar(kQFull + qb), 0, item.head * args.group, t0);
+            tma_load_3d(dst + kHalfBytes, &tm_q, bar(kQFull + qb), 64, item.head * args.group, t0);
+          }
+          for (int j = tb; ok && j < te; ++j) {
+            const PrefixTile tile = args.tiles[j];
+            const bool own = tile.info & kTileOwn;
+            for (int kv = 0; kv < 2; ++kv, ++c) {
+              const int s = c % kSlots;
+              if (!(ok = mbar_wait(bar(kSlotEmpty + s), ((c / kSlots) & 1) ^ 1, abort_flag,
+                                   args.status, kDevTimeoutSlotEmpty, wait_limit)))
+                break;
+              // what this slot held has been used, so it has landed
+              flying &= ~((1u << (s + 16)) | (1u << (s + kSlots + 16)));
+              if (kFormat != kKvPlain && !own) continue;  // the preparing warps fill it
+              const uint32_t dst = sbase + kSlotOff + s * kTileBytes;
+              const CUtensorMap* tm = own ? (kv ? &tm_v : &tm_k) : (kv ? &tm_pv : &tm_pk);
+              uint32_t full = bar(kSlotFull + s);
+              if (kv == 1 && (tile.info & kTileGuard)) {
+                full = bar(kRawFull + s);
+                fly(kSlots + s, (raw_uses >> s) & 1u);
+                raw_uses ^= 1u << s;
+                mbar_arrive_expect_tx(full, kTileBytes);
+              } else {
+                fly(s, (c / kSlots) & 1);
+                mbar_arrive_expect_tx(full, kTileBytes);
+                mbar_arrive(full);  // the second of kSlotFullArrivals
+              }
+              tma_load_3d(dst, tm, full, 0, item.head, tile.key);
+              tma_load_3d(dst + kHalfBytes, tm, full, 64, item.head, tile.key);
+            }
+          }
+        }
+        bool drained = true;
+        for (int i = 0; i < 2 * kSlots + 2; ++i)
+          if ((flying >> (i + 16)) & 1u) {
+            const int b = i < kSlots ? kSlotFull + i
+                                     : (i < 2 * kSlots ? kRawFull + i - kSlots
+                                                       : kQFull + i - 2 * kSlots);
+            drained &= mbar_drain(bar(b), (flying >> i) & 1u, *wait_limit);
+          }
+        if (!drained) atomicCAS(args.status, 0, kDevTimeoutDrain);
+      }
+    } else if (warp == 1) {
+      // -------------------------------------------------------- MMA issuer
+      if (lane == 0) {
+        const uint32_t t_s[2] = {tmem, tmem + 128};
+        const uint32_t t_o[2] = {tmem + 256, tmem + 384};
+        const uint64_t q_desc0 = smem_desc_sw128(sbase, 16, 1024);
+        const uint64_t k_desc0 = smem_desc_sw128(sbase + kSlotOff, 16, 1024);
+        const uint64_t v_desc0 = smem_desc_sw128(sbase + kSlotOff, kHalfBytes, 1024);
+        bool ok = true;
+        int t = 0;   // key tiles so far (tile A runs on all of them)
+        int tB = 0;  // those with a tile B
+        bool have_prev = false;  // PV_B of the previous tile still to issue
+        int prev_v = 0, prev_nk = 8;
+        bool prev_acc = false, prev_last = false;
+        // PV_B of the previous tile: its P has parity (tB - 1)
+        auto issue_prev = [&]() -> bool {
+          const uint64_t vd = v_desc0 + ((prev_v * kTileBytes) >> 4);
+          if (!mbar_wait(bar(kPLo + 1), (tB - 1) & 1, abort_flag, args.status, kDevTimeoutPFull,
+                         wait_limit))
+            return false;
+          tc_fence_after();
+          issue_pv_part<kBf16>(t_o[1], t_s[1], vd, prev_acc, prev_nk, 0);
+          if (!mbar_wait(bar(kPHi + 1), (tB - 1) & 1, abort_flag, args.status, kDevTimeoutPFull,
+                         wait_limit))
+            return false;
+          tc_fence_after();
+          issue_pv_part<kBf16>(t_o[1], t_s[1], vd, prev_acc, prev_nk, 1);
+          tc_commit(bar(kSlotEmpty + prev_v));
+          if (prev_last) tc_commit(bar(kOFinal + 1));
+          have_prev = false;
+          return true;
+        };
+        for (int it = share.beg, li = 0; ok && it < share.end; ++it, ++li) {
+          const PrefixItem item = args.items[it];
+          int tb, te;
+          share_tiles<kSplit>(share, item, tb, te);
+          const int nx = item.tokens > args.tile_tokens ? 2 : 1;
+          const int qb = li & 1;
+          const uint64_t qa = q_desc0 + ((qb * kQBufBytes) >> 4);
+          const uint64_t qbd = qa + (kTileBytes >> 4);
+          if (!(ok = mbar_wait(bar(kQFull + qb), (li >> 1) & 1, abort_flag, args.status,
+                               kDevTimeoutQ, wait_limit)))
+            break;
+          for (int j = tb; j < te; ++j, ++t) {
+            const int ck = 2 * t, sk = ck % kSlots;
+            const int cv = 2 * t + 1, sv = cv % kSlots;
+            const int width = args.tiles[j].info & kTileWidthMask;
+            const uint64_t k_desc = k_desc0 + ((sk * kTileBytes) >> 4);
+            if (!(ok = mbar_wait(bar(kSlotFull + sk), (ck / kSlots) & 1, abort_flag, args.status,
+                                 kDevTimeoutSlotFull, wait_limit)))
+              break;
+            tc_fence_after();
+            const uint32_t idesc = idesc_16<kBf16>(128, width, false);
+            issue_qk(t_s[0], qa, k_desc, idesc);
+            tc_commit(bar(kSFull + 0));
+            if (have_prev && !(ok = issue_prev())) break;
+            if (nx == 2) {
+              issue_qk(t_s[1], qbd, k_desc, idesc);
+              tc_commit(bar(kSFull + 1));
+            }
+            tc_commit(bar(kSlotEmpty + sk));
+            if (!(ok = mbar_wait(bar(kSlotFull + sv), (cv / kSlots) & 1, abort_flag, args.status,
+                                 kDevTimeoutSlotFull, wait_limit)))
+              break;
+            const uint64_t vd = v_desc0 + ((sv * kTileBytes) >> 4);
+            if (!(ok = mbar_wait(bar(kPLo + 0), t & 1, abort_flag, args.status, kDevTimeoutPFull,
+                                 wait_limit)))
+              break;
+            tc_fence_after();
+            issue_pv_part<kBf16>(t_o[0], t_s[0], vd, j > tb, width / 16, 0);
+            if (!(ok = mbar_wait(bar(kPHi + 0), t & 1, abort_flag, args.status, kDevTimeoutPFull,
+                                 wait_limit)))
+              break;
+            tc_fence_after();
+            issue_pv_part<kBf16>(t_o[0], t_s[0], vd, j > tb, width / 16, 1);
+            if (j == te - 1) tc_commit(bar(kOFinal + 0));
+            if (nx == 2) {
+              have_prev = true;
+              prev_v = sv;
+              prev_acc = j > tb;
+              prev_nk = width / 16;
+              prev_last = j == te - 1;
+              ++tB;
+            } else {
+              tc_commit(bar(kSlotEmpty + sv));
+            }
+          }
+        }
+        if (ok && have_prev) ok = issue_prev();
+        tc_commit(bar(kDrain));
+        if (!mbar_drain(bar(kDrain), 0, *wait_limit)) atomicCAS(args.status, 0, kDevTimeoutDrain);
+      }
+    } else {
+      // -------------------------------------------------- preparing warps
+      const int w = warp - 2;
+      int c = 0;
+      bool ok = true;
+      uint32_t raw_uses = 0;
+      RawTile raw;
+      // a warp-wide wait: every lane leaves it with the same answer
+      auto wait = [&](uint32_t b, uint32_t parity, int code) -> bool {
+        const bool got = mbar_wait(b, parity, abort_flag, args.status, code, wait_limit);
+        return __all_sync(0xffffffffu, got);
+      };
+      auto publish = [&](int s, bool bad, int li) {
+        if (__any_sync(0xffffffffu, bad) && lane == 0) bad_item[li & 3] = li + 1;
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(kSlotFull + s));
+      };
+      for (int it = share.beg, li = 0; ok && it < share.end; ++it, ++li) {
+        const PrefixItem item = args.items[it];
+        int tb, te;
+        share_tiles<kSplit>(share, item, tb, te);
+        // codes of the item's next 8-bit tile are fetched one tile ahead
+        auto fetch = [&](int j, int kv) {
+          const PrefixTile tile = args.tiles[j];
+          const int rows = min(tile.info & kTileWidthMask, args.prefix_len - tile.key);
+          load_raw(raw, static_cast<const uint8_t*>(kv ? args.v_prefix : args.k_prefix),
+                   kv ? args.v_scale : args.k_scale, args.kv_heads, item.head, tile.key, rows, w,
+                   lane);
+        };
+        if (kFormat != kKvPlain && tb < te && !(args.tiles[tb].info & kTileOwn)) fetch(tb, 0);
+        for (int j = tb; ok && j < te; ++j) {
+          const PrefixTile tile = args.tiles[j];
+          const bool own = tile.info & kTileOwn;
+          const bool guard = tile.info & kTileGuard;
+          for (int kv = 0; kv < 2; ++kv, ++c) {
+            const int s = c % kSlots;
+            const uint32_t slot = sbase + kSlotOff + s * kTileBytes;
+            if (kFormat != kKvPlain &&
+                !(ok = wait(bar(kSlotEmpty + s), ((c / kSlots) & 1) ^ 1, kDevTimeoutSlotEmpty)))
+              break;
+            if (kFormat != kKvPlain && !own) {
+              const bool bad =
+                  store_raw<kBf16, kFormat>(raw, slot, kv == 1 && guard, w, lane);
+              publish(s, bad, li);
+              if (kv == 0) fetch(j, 1);
+              else if (j + 1 < te && !(args.tiles[j + 1].info & kTileOwn)) fetch(j + 1, 0);
+            } else if (kv == 1 && guard) {
+              if (!(ok = wait(bar(kRawFull + s), (raw_uses >> s) & 1u, kDevTimeoutSlotFull)))
+                break;
+              raw_uses ^= 1u << s;
+              publish(s, guard_tile<kBf16>(slot, tile.info & kTileWidthMask, w, lane), li);
+            }
+          }
+        }
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+    // ----------------------------------------------------------- softmax
+    const int x = (warp - kSoftmaxWarp0) >> 2;
+    const int sub = warp & 3;
+    const int row = sub * 32 + lane;
+    const uint32_t t_lane = tmem + (static_cast<uint32_t>(sub * 32) << 16);
+    const uint32_t t_s = t_lane + x * 128;
+    const uint32_t t_o = t_lane + 256 + x * 128;
+    const float scale = args.scale_log2;
+    const int token = row / args.group;  // of this row in its tile
+    bool ok = true;
+    int t = 0, lx = 0;  // key tiles and items of this row tile so far
+    for (int it = share.beg, li = 0; ok && it < share.end; ++it, ++li) {
+      const PrefixItem item = args.items[it];
+      int tb, te;
+      share_tiles<kSplit>(share, item, tb, te);
+      const int qb = li & 1;
+      if (x == 1 && item.tokens <= args.tile_tokens) {
+        // no tile B: release the Q buffer once it is this item's
+        if (!(ok = mbar_wait(bar(kQFull + qb), (li >> 1) & 1, abort_flag, args.status,
+                             kDevTimeoutQ, wait_limit)))
+          break;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(kQEmpty + qb));
+        continue;
+      }
+      const bool valid = row < tile_rows && x * args.tile_tokens + token < item.tokens;
+      PrefixRow mine = {0, -1};
+      if (valid) mine = args.rows[item.row0 + x * args.tile_tokens + token];
+      float m_run = -INFINITY, l_run = 0.f;
+      for (int j = tb; j < te; ++j, ++t) {
+        const PrefixTile tile = args.tiles[j];
+        if (!(ok = mbar_wait(bar(kSFull + x), t & 1, abort_flag, args.status, kDevTimeoutSFull,
+                             wait_limit)))
+          break;
+        tc_fence_after();
+        const bool narrow = (tile.info & kTileWidthMask) <= 64;
+        uint32_t a0[32], a1[32], a2[32], a3[32];
+        tmem_ld32(t_s + 0, a0);
+        tmem_ld32(t_s + 32, a1);
+        if (!narrow) {
+          tmem_ld32(t_s + 64, a2);
+          tmem_ld32(t_s + 96, a3);
+        }
+        tmem_wait_ld();
+        reg_fence32(a0);
+        reg_fence32(a1);
+        if (!narrow) {
+          reg_fence32(a2);
+          reg_fence32(a3);
+        }
+        if (tile.info & kTileMask) {
+          const Kept kept = kept_keys(args, tile.info & kTileOwn, mine);
+          mask_keys(a0, kept, tile.key, args.sparse);
+          mask_keys(a1, kept, tile.key + 32, args.sparse);
+          if (!narrow) {
+            mask_keys(a2, kept, tile.key + 64, args.sparse);
+            mask_keys(a3, kept, tile.key + 96, args.sparse);
+          }
+        }
+        float tmax = fmaxf(chunk_max(a0), chunk_max(a1));
+        if (!narrow) tmax = fmaxf(tmax, fmaxf(chunk_max(a2), chunk_max(a3)));
+        tmax *= scale;
+        const float m_new = fmaxf(m_run, tmax);
+        bool need = false;
+        float f = 1.f;
+        if (j == tb) {
+          m_run = m_new;
+        } else if (m_new > m_run + 8.f) {
+          // lazy rescale: P stays <= 2^8 against a maximum that is out of date
+          need = true;
+          f = ex2(m_run - m_new);
+          l_run *= f;
+          m_run = m_new;
+        }
+        const float m_use = (m_run == -INFINITY) ? 0.f : m_run;
+        float sum = exp_pack<kBf16>(a0, scale, m_use) + exp_pack<kBf16>(a1, scale, m_use);
+        tmem_st16(t_s + 0, a0);
+        tmem_st16(t_s + 16, a1);
+        if (__any_sync(0xffffffffu, need)) {
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t o[32];
+            tmem_ld32(t_o + 32 * c, o);
+            tmem_wait_ld();
+            reg_fence32(o);
+            const uint64_t f2 = f2_pack(f, f);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              float r0, r1;
+              f2_unpack(mul2(f2_pack(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1])), f2),
+                        r0, r1);
+              o[2 * i] = __float_as_uint(r0);
+              o[2 * i + 1] = __float_as_uint(r1);
+            }
+            tmem_st32(t_o + 32 * c, o);
+          }
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(bar(kPLo + x));
+        if (!narrow) {
+          sum += exp_pack<kBf16>(a2, scale, m_use) + exp_pack<kBf16>(a3, scale, m_use);
+          tmem_st16(t_s + 32, a2);
+          tmem_st16(t_s + 48, a3);
+          tmem_wait_st();
+          tc_fence_before();
+        }
+        l_run += sum;
+        mbar_arrive(bar(kPHi + x));
+      }
+      // Epilogue: every MMA that reads this tile's Q rows has completed, so
+      // their buffer serves as staging.
+      if (!ok || !(ok = mbar_wait(bar(kOFinal + x), lx & 1, abort_flag, args.status,
+                                  kDevTimeoutOFinal, wait_limit)))
+        break;
+      ++lx;
+      tc_fence_after();
+      const bool aside = valid && bad_item[li & 3] == li + 1;
+      if constexpr (kSplit) {
+        // f32 rows of 512 bytes, their 16-byte units swizzled by the row
+        const uint32_t dst = sbase + x * kQBufBytes + row * 512;
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          uint32_t o[32];
+          tmem_ld32(t_o + 32 * c, o);
+          tmem_wait_ld();
+          reg_fence32(o);
+          if (aside) {
+            const Aside s = find_aside<kBf16, kFormat>(args, tb, te, mine, item.head, c);
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              o[i] = __float_as_uint(with_aside(__uint_as_float(o[i]), s, i));
+          }
+#pragma unroll
+          for (int v = 0; v < 8; ++v)
+            st_shared_v4(dst + (static_cast<uint32_t>(c * 8 + v) ^ lane) * 16, o[4 * v],
+                         o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
+        }
+        *reinterpret_cast<float2*>(smem + kStatOff + (x * 128 + row) * 8) =
+            make_float2(m_run, l_run);
+      } else {
+        const float inv_l = 1.f / l_run;
+        const uint32_t stage = sbase + qb * kQBufBytes + x * kTileBytes;
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          uint32_t o[32];
+          tmem_ld32(t_o + 32 * c, o);
+          tmem_wait_ld();
+          reg_fence32(o);
+          if (aside) {
+            const Aside s = find_aside<kBf16, kFormat>(args, tb, te, mine, item.head, c);
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              o[i] = __float_as_uint(with_aside(__uint_as_float(o[i]), s, i));
+          }
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            const uint32_t* p = o + 8 * v;
+            uint32_t y[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              y[i] = pack2<kBf16>(__uint_as_float(p[2 * i]) * inv_l,
+                                  __uint_as_float(p[2 * i + 1]) * inv_l);
+            st_shared_v4(stage + row * 256 + ((c * 4 + v) ^ (lane & 15)) * 16, y[0], y[1], y[2],
+                         y[3]);
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        // the warp's rows leave two at a time, 256 bytes each
+        for (int i = 0; i < 16; ++i) {
+          const int r = sub * 32 + 2 * i + (lane >> 4);
+          const int rt = r / args.group, rh = r - rt * args.group;
+          const int tok = x * args.tile_tokens + rt;
+          const uint4 v = ld_shared_v4(stage + r * 256 + ((lane & 15) ^ (r & 15)) * 16);
+          if (r < tile_rows && tok < item.tokens)
+            *reinterpret_cast<uint4*>(args.out +
+                                      (static_cast<int64_t>(item.row0 + tok) * args.q_heads +
+                                       item.head * args.group + rh) *
+                                          kHeadDim +
+                                      (lane & 15) * 8) = v;
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(kQEmpty + qb));
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncwarp();
+  if constexpr (kSplit) {
+    // the cluster's O, m and l are in shared memory: each CTA merges its share
+    // of the rows, a warp a row
+    cluster_sync();
+    if (warp >= kSoftmaxWarp0) {
+      const PrefixItem item = args.items[share.beg];
+      const int rows = item.tokens > args.tile_tokens ? 256 : 128;
+      const int per = (rows + share.ranks - 1) / share.ranks;
+      for (int i = warp - kSoftmaxWarp0; i < per; i += 8) {
+        const int r = share.rank * per + i;  // of the block's 128 or 256
+        const int x = r >> 7, rr = r & 127;
+        const int rt = rr / args.group, rh = rr - rt * args.group;
+        const int tok = x * args.tile_tokens + rt;
+        if (r >= rows || rr >= tile_rows || tok >= item.tokens) continue;
+        float2 ml = make_float2(-INFINITY, 0.f);
+        if (lane < share.ranks)
+          ml = ld_cluster_v2(mapa_shared(sbase + kStatOff + r * 8, lane));
+        float m = ml.x;
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        m = __shfl_sync(0xffffffffu, m, 0);
+        const float w = ml.x == -INFINITY ? 0.f : ex2(ml.x - m);
+        float l = w * ml.y;
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        l = __shfl_sync(0xffffffffu, l, 0);
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        const uint32_t at =
+            sbase + x * kQBufBytes + rr * 512 + (static_cast<uint32_t>(lane) ^ (rr & 31)) * 16;
+        for (int k = 0; k < share.ranks; ++k) {
+          const float wk = __shfl_sync(0xffffffffu, w, k);
+          const float4 v = ld_cluster_v4(mapa_shared(at, k));
+          if (wk != 0.f) {  // a rank in which the row keeps nothing adds nothing
+            acc.x = fmaf(wk, v.x, acc.x);
+            acc.y = fmaf(wk, v.y, acc.y);
+            acc.z = fmaf(wk, v.z, acc.z);
+            acc.w = fmaf(wk, v.w, acc.w);
+          }
+        }
+        const float inv_l = 1.f / l;
+        uint2 y;
+        y.x = pack2<kBf16>(acc.x * inv_l, acc.y * inv_l);
+        y.y = pack2<kBf16>(acc.z * inv_l, acc.w * inv_l);
+        *reinterpret_cast<uint2*>(args.out +
+                                  (static_cast<int64_t>(item.row0 + tok) * args.q_heads +
+                                   item.head * args.group + rh) *
+                                      kHeadDim +
+                                  lane * 4) = y;
+      }
+    }
+    __syncwarp();
+    cluster_sync();  // no CTA leaves while its shared memory is read
+  }
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+template <bool kBf16, int kFormat, bool kSplit>
+cudaError_t launch(const PrefixMaps& m, const PrefixArgs& args, int grid, int splits,
+                   cudaStream_t stream) {
+  static bool configured[kMaxDevices] = {};
+  auto kernel = prefix_attention_kernel<kBf16, kFormat, kSplit>;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
+  if (!configured[dev]) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    if (e != cudaSuccess) return e;
+    configured[dev] = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmemBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = static_cast<unsigned>(splits);
+  attr.val.clusterDim.y = 1;
+  attr.val.clusterDim.z = 1;
+  if (kSplit) {
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+  }
+  return cudaLaunchKernelEx(&cfg, kernel, m.q, m.k, m.v, m.pk, m.pv, args);
+}
+
+template <bool kBf16>
+cudaError_t launch_typed(const PrefixMaps& m, const PrefixArgs& a, int format, int grid, int splits,
+                         cudaStream_t stream) {
+  const bool split = splits > 1;
+  switch (format) {
+    case kKvE4M3:
+      return split ? launch<kBf16, kKvE4M3, true>(m, a, grid, splits, stream)
+                   : launch<kBf16, kKvE4M3, false>(m, a, grid, splits, stream);
+    case kKvInt8:
+      return split ? launch<kBf16, kKvInt8, true>(m, a, grid, splits, stream)
+                   : launch<kBf16, kKvInt8, false>(m, a, grid, splits, stream);
+    default:
+      return split ? launch<kBf16, kKvPlain, true>(m, a, grid, splits, stream)
+                   : launch<kBf16, kKvPlain, false>(m, a, grid, splits, stream);
+  }
+}
+
+}  // namespace
+
+cudaError_t launch_prefix_attention(const PrefixMaps& maps, const PrefixArgs& args, int bf16,
+                                    int format, int grid, cudaStream_t stream) {
+  if (grid <= 0) return cudaSuccess;
+  return bf16 ? launch_typed<true>(maps, args, format, grid, args.splits, stream)
+              : launch_typed<false>(maps, args, format, grid, args.splits, stream);
+}
+
+}  // namespace qwa

@@ -1,0 +1,201 @@
+"""Attention of a batch of requests that share a cached prefix.
+
+Requests of one service begin with the same text (an instruction, examples, a
+document). Its keys and values are computed once, kept in a ``KVCache``, and
+every request of a micro-batch attends to them and to its own keys:
+``prefix_attention`` packs the query rows of all requests into the tensor cores'
+tiles, so the prefix is read and multiplied once for the batch. It stands
+beside ``attention.CausalAttentionKernel`` (src/webgpu/ops.ts:320-345): with a
+prefix of length 0 both compute the same, and the sparse rule is the
+reference's, on absolute positions.
+
+Launches are the kernel of csrc/prefix_attention.cu through the C ABI. A
+``PrefixPlan`` holds the work lists of given lengths; ``prefix_attention``
+keeps the last few plans.
+"""
+from __future__ import annotations
+
+import ctypes
+import threading
+from collections import OrderedDict
+from typing import Optional, Sequence
+
+import torch
+
+from . import _lib
+from .attention import (HEAD_DIM, MODE_AUTO, PREFIX, WINDOW, AttentionRun, Context, EncodableRun,
+                        _need, _ptr, encode_run)
+from .kv_cache import _DTYPES, KVCache
+
+
+_retired: list = []  # lists of plans that ended during a capture
+
+
+class PrefixPlan:
+    """Work lists for requests of given lengths behind a prefix of ``prefix_len``
+    keys. A request's queries are the last of its own keys; ``cu_seqlens_k`` None: as
+    many keys as queries. A captured graph needs its plan for as long as it is
+    replayed."""
+
+    def __init__(self, cu_seqlens: Sequence[int], prefix_len: int, q_heads: int, kv_heads: int,
+                 cu_seqlens_k: Optional[Sequence[int]] = None, mode: int = MODE_AUTO,
+                 sparse_prefix: int = PREFIX, window: int = WINDOW, device=None,
+                 ctx: Optional[Context] = None):
+        self.ctx = ctx if ctx is not None else Context.for_device(device)
+        self.handle = None
+        cu_q = _lib.cu_array(cu_seqlens)
+        cu_k = _lib.cu_array(cu_seqlens_k) if cu_seqlens_k is not None else None
+        _need(len(cu_q) >= 2, "cu_seqlens needs at least one request")
+        _need(cu_k is None or len(cu_k) == len(cu_q),
+              "cu_seqlens and cu_seqlens_k must be of the same requests")
+        with torch.cuda.device(self.ctx.device):
+            _need(not torch.cuda.is_current_stream_capturing(),
+                  "a plan allocates memory: make it before the capture")
+        while _retired:
+            lib, old = _retired.pop()
+            lib.qwa_prefix_plan_destroy(old)
+        h = ctypes.c_void_p()
+        _lib.check(self.ctx.lib.qwa_prefix_plan_create(
+            self.ctx.handle, cu_q, cu_k, len(cu_q) - 1, q_heads, kv_heads, prefix_len, mode,
+            sparse_prefix, window, ctypes.byref(h)), self.ctx.handle)
+        self.handle = h
+        self.queries = cu_q[len(cu_q) - 1]
+        self.keys = cu_k[len(cu_k) - 1] if cu_k is not None else self.queries
+        self.prefix_len, self.q_heads, self.kv_heads = prefix_len, q_heads, kv_heads
+
+    def close(self) -> None:
+        """Release the lists; waits for the device. During a stream capture
+        (memory is not freed then) they are released by the next plan."""
+        if self.handle:
+            handle, self.handle = self.handle, None
+            if torch.cuda.is_current_stream_capturing():
+                _retired.append((self.ctx.lib, handle))
+            else:
+                self.ctx.lib.qwa_prefix_plan_destroy(handle)
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:  # at the interpreter's end
+            pass
+
+
+def _packed(t: torch.Tensor, name: str, tokens: int, heads: int, like: torch.Tensor) -> int:
+    """Checks a packed [tokens, heads, 128] operand; its token stride."""
+    _need(isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in _DTYPES and t.dim() == 3
+          and t.dtype == like.dtype and t.device == like.device,
+          f"{name} must be a CUDA float16 or bfloat16 tensor of q's dtype and device")
+    _need(tuple(t.shape) == (tokens, heads, HEAD_DIM),
+          f"{name} must be [{tokens}, {heads}, {HEAD_DIM}], got {tuple(t.shape)}")
+    _need(t.stride(2) == 1 and (heads == 1 or t.stride(1) == HEAD_DIM),
+          f"{name}: a token's heads must be contiguous")
+    return t.stride(0) if tokens > 1 else heads * HEAD_DIM
+
+
+class PrefixAttentionKernel:
+    """Shared-prefix attention, beside CausalAttentionKernel."""
+
+    def __init__(self, device=None):
+        self.ctx = Context.for_device(device)
+
+    def create_run(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, output: torch.Tensor,
+                   plan: PrefixPlan, cache: Optional[KVCache] = None,
+                   first_slot: int = 0) -> AttentionRun:
+        """q [queries, q_heads, 128], k, v [own keys, kv_heads, 128] packed
+        request after request, output as q, contiguous; the prefix is in the
+        cache's slots ``first_slot`` .. ``first_slot + plan.prefix_len - 1``."""
+        q_stride = _packed(q, "q", plan.queries, plan.q_heads, q)
+        k_stride = _packed(k, "k", plan.keys, plan.kv_heads, q)
+        v_stride = _packed(v, "v", plan.keys, plan.kv_heads, q)
+        _packed(output, "output", plan.queries, plan.q_heads, q)
+        _need(output.is_contiguous(), "output must be contiguous")
+        _need(q.device.index == self.ctx.device and plan.ctx.device == self.ctx.device,
+              "q and the plan must be on the kernel's device")
+        _need(plan.handle is not None, "the plan is closed")
+        _need(cache is not None or plan.prefix_len == 0, "a prefix needs its cache")
+        struct = None
+        if cache is not None:
+            _need(cache.device == q.device, "the cache must be on q's device")
+            struct = ctypes.byref(cache.struct)
+        lib, h = self.ctx.lib, self.ctx.handle
+        args = (_DTYPES[q.dtype], _ptr(q), q_stride, _ptr(k), k_stride, _ptr(v), v_stride,
+                _ptr(output), struct, first_slot)
+
+        def launch(stream):
+            _need(plan.handle is not None, "the plan is closed")
+            return lib.qwa_prefix_attention(h, plan.handle, *args, stream)
+
+        return AttentionRun([EncodableRun(launch, self.ctx, "shared-prefix attention")])
+
+    def encode(self, stream, run: AttentionRun) -> None:
+        for command in run.commands:
+            encode_run(stream, command)
+
+
+MAX_PLANS = 64
+_plans: "OrderedDict" = OrderedDict()
+_captured: dict = {}  # plans that a graph was captured with are kept
+_plans_lock = threading.Lock()
+
+
+def _plan_for(ctx: Context, key: tuple) -> PrefixPlan:
+    with torch.cuda.device(ctx.device):
+        capturing = torch.cuda.is_current_stream_capturing()
+    full = (ctx.device,) + key
+    with _plans_lock:
+        plan = _captured.get(full) or _plans.get(full)
+        if plan is not None:
+            if capturing:
+                _captured[full] = plan
+            elif full in _plans:
+                _plans.move_to_end(full)
+            return plan
+    cu_q, cu_k, prefix_len, q_heads, kv_heads, mode, sparse_prefix, window = key
+    plan = PrefixPlan(cu_q, prefix_len, q_heads, kv_heads, cu_k, mode, sparse_prefix, window,
+                      ctx=ctx)
+    with _plans_lock:
+        _plans[full] = plan
+        while len(_plans) > MAX_PLANS:
+            _plans.popitem(last=False)
+    return plan
+
+
+def prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                     cu_seqlens: Sequence[int], cache: Optional[KVCache] = None,
+                     prefix_len: int = 0, first_slot: int = 0,
+                     cu_seqlens_k: Optional[Sequence[int]] = None, mode: int = MODE_AUTO,
+                     sparse_prefix: int = PREFIX, window: int = WINDOW,
+                     out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+    """softmax(q k / sqrt(128)) v of packed requests behind the ``prefix_len``
+    keys in the cache's slots from ``first_slot`` on: q [queries, q_heads, 128], k, v
+    [own keys, kv_heads, 128]. ``cu_seqlens`` (host) cuts q into requests, ``cu_seqlens_k``
+    k and v (None: the same); a request's queries are the last of its keys.
+    Lengths met before reuse their plan; inside a capture they must have been
+    met before it."""
+    _need(isinstance(q, torch.Tensor) and q.is_cuda and q.dim() == 3
+          and isinstance(k, torch.Tensor) and k.dim() == 3,
+          "q and k must be CUDA tensors [tokens, heads, 128]")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    kern = PrefixAttentionKernel(q.device.index)
+    plan = _plan_for(kern.ctx, (tuple(cu_seqlens),
+                                tuple(cu_seqlens_k) if cu_seqlens_k is not None else None,
+                                prefix_len, q.shape[1], k.shape[1], mode, sparse_prefix, window))
+    kern.encode(stream, kern.create_run(q, k, v, out, plan, cache, first_slot))
+    return out
+
+
+def prefix_attention_work(cu_seqlens: Sequence[int], prefix_len: int, q_heads: int,
+                          kv_heads: int, cu_seqlens_k: Optional[Sequence[int]] = None,
+                          mode: int = MODE_AUTO, sparse_prefix: int = PREFIX,
+                          window: int = WINDOW):
+    """(kept pairs per query head, key tiles visited over all kv heads) of one call."""
+    cu_q = _lib.cu_array(cu_seqlens)
+    cu_k = _lib.cu_array(cu_seqlens_k) if cu_seqlens_k is not None else None
+    _need(cu_k is None or len(cu_k) == len(cu_q),
+          "cu_seqlens and cu_seqlens_k must be of the same requests")
+    pairs, tiles = ctypes.c_int64(), ctypes.c_int64()
+    _lib.check(_lib.load().qwa_prefix_attention_work(
+        cu_q, cu_k, len(cu_q) - 1, q_heads, kv_heads, prefix_len, mode, sparse_prefix, window,
+        ctypes.byref(pairs), ctypes.byref(tiles)))
+    return pairs.value, tiles.value

@@ -1,0 +1,147 @@
+"""Rotary positions on their own: the (cos, sin) table and its application.
+
+``QKNormRopeKernel`` rotates behind the Q/K norm, whole heads in halves, from
+position 0 (src/webgpu/ops.ts:104-166, table model.ts:76-83). This module has
+the rotation alone, for q and k that are normed already or not at all: both pair
+layouts, a part of the head, any positions, the way back (the gradient), and
+tables for contexts longer than the model's (linear, ntk, yarn, llama3). A
+table with ``rotary_dim`` 128 is also a ``rope_table`` for the fused kernels;
+its rows from P on serve requests that begin at position P.
+
+Launches are the kernels of csrc/rope.cu through the C ABI.
+"""
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib
+from .attention import ROPE_THETA, Context, EncodableRun, _need, _ptr, encode_run
+
+_DTYPES = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
+_LAYOUTS = {"half": _lib.ROPE_HALF, "interleaved": _lib.ROPE_INTERLEAVED}
+
+
+@dataclass(frozen=True)
+class RopeScaling:
+    """How frequencies change for longer contexts (include/qwa.h has the rules).
+    ``attention_factor`` None: yarn's own, 0.1 ln(factor) + 1."""
+    kind: str = "none"
+    factor: float = 1.0
+    original_positions: float = 0.0
+    beta_fast: float = 32.0
+    beta_slow: float = 1.0
+    attention_factor: Optional[float] = None
+    low_freq_factor: float = 1.0
+    high_freq_factor: float = 4.0
+
+    def struct(self) -> "_lib.RopeScalingStruct":
+        _need(self.kind in _lib.ROPE_SCALING,
+              f"scaling kind must be one of {sorted(_lib.ROPE_SCALING)}")
+        _need(self.attention_factor is None or self.attention_factor > 0,
+              "attention_factor must be above 0")
+        return _lib.RopeScalingStruct(_lib.ROPE_SCALING[self.kind], self.factor,
+                                      self.original_positions, self.beta_fast, self.beta_slow,
+                                      self.attention_factor or 0.0, self.low_freq_factor,
+                                      self.high_freq_factor)
+
+
+def rope_table(positions: int, rotary_dim: int = 128, theta: float = ROPE_THETA,
+               scaling: Optional[RopeScaling] = None, first: int = 0, device=None,
+               out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+    """f32 [positions, rotary_dim / 2, 2]: (cos, sin) of positions ``first``,
+    ``first`` + 1, ... with the angle in 64 bits."""
+    _need(positions >= 0 and rotary_dim >= 2, "positions must be >= 0 and rotary_dim >= 2")
+    if out is not None:
+        _need(out.is_cuda and out.dtype == torch.float32 and out.is_contiguous()
+              and out.numel() >= positions * (rotary_dim // 2) * 2,
+              "out must be a contiguous CUDA float32 tensor of [positions, rotary_dim / 2, 2]")
+        device = out.device
+    device = torch.device("cuda") if device is None else torch.device(device)
+    ctx = Context.for_device(device.index)
+    if out is None:
+        out = torch.empty(positions, rotary_dim // 2, 2, dtype=torch.float32,
+                          device=torch.device("cuda", ctx.device))
+    s = scaling.struct() if scaling is not None else None
+    lib, h = ctx.lib, ctx.handle
+    encode_run(stream, EncodableRun(
+        lambda st: lib.qwa_rope_table(h, _ptr(out), first, positions, rotary_dim, theta,
+                                      ctypes.byref(s) if s is not None else None, st),
+        ctx, "rotary table"))
+    return out
+
+
+def _heads(t: torch.Tensor, name: str, tokens: int, dim: int, dtype, device) -> None:
+    _need(isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in _DTYPES and t.dim() == 3,
+          f"{name} must be a CUDA float16 or bfloat16 tensor [tokens, heads, head_dim]")
+    _need(t.shape[0] == tokens and t.shape[2] == dim and t.dtype == dtype and t.device == device,
+          f"{name} must agree with the others in tokens, head_dim, dtype and device")
+    _need(t.stride(2) == 1 or dim == 1, f"{name}: a head's values must be contiguous")
+
+
+def _side(x: torch.Tensor, y: torch.Tensor) -> "_lib.RopeTensor":
+    return _lib.RopeTensor(x.data_ptr(), x.stride(0), x.stride(1), y.data_ptr(), y.stride(0),
+                           y.stride(1), x.shape[1])
+
+
+class RopeKernel:
+    """Rotation of q and k by a table (``rope_table``), beside QKNormRopeKernel."""
+
+    def __init__(self, device=None):
+        self.ctx = Context.for_device(device)
+
+    def create_run(self, q: Optional[torch.Tensor], k: Optional[torch.Tensor],
+                   table: torch.Tensor, positions: torch.Tensor,
+                   q_output: Optional[torch.Tensor], k_output: Optional[torch.Tensor],
+                   layout: str = "half", inverse: bool = False) -> EncodableRun:
+        """q, k: [tokens, heads, head_dim], any strides with contiguous heads;
+        either may be None. An output may be its input (in place). A token
+        whose position is not a row of the table is left unwritten."""
+        some = q if q is not None else k
+        _need(some is not None, "one of q and k is required")
+        _need(layout in _LAYOUTS, "layout must be 'half' or 'interleaved'")
+        _need(isinstance(some, torch.Tensor) and some.dim() == 3,
+              "q and k must be tensors [tokens, heads, head_dim]")
+        tokens, _, dim = some.shape
+        for x, y, name in ((q, q_output, "q"), (k, k_output, "k")):
+            if x is None:
+                continue
+            _heads(x, name, tokens, dim, some.dtype, some.device)
+            _need(y is not None, f"{name} needs an output")
+            _heads(y, name + "_output", tokens, dim, some.dtype, some.device)
+            _need(y.shape[1] == x.shape[1], f"{name}_output must have {name}'s heads")
+        _need(some.device.index == self.ctx.device, "q and k must be on the kernel's device")
+        _need(table.device == some.device and table.dtype == torch.float32 and table.dim() == 3
+              and table.shape[2] == 2 and table.is_contiguous(),
+              "table must be a contiguous float32 [rows, rotary_dim / 2, 2] on q's device")
+        _need(positions.device == some.device and positions.dtype == torch.int32
+              and positions.is_contiguous() and positions.numel() >= tokens,
+              "positions must be a contiguous int32 tensor of one position a token")
+        lib, h = self.ctx.lib, self.ctx.handle
+        qs = _side(q, q_output) if q is not None else None
+        ks = _side(k, k_output) if k is not None else None
+        args = (_DTYPES[some.dtype], ctypes.byref(qs) if qs is not None else None,
+                ctypes.byref(ks) if ks is not None else None, tokens, dim, 2 * table.shape[1],
+                _LAYOUTS[layout], 1 if inverse else 0, _ptr(positions), _ptr(table),
+                table.shape[0])
+        return EncodableRun(lambda s: lib.qwa_rope(h, *args, s), self.ctx, "rotary positions")
+
+
+def rope(q: Optional[torch.Tensor], k: Optional[torch.Tensor], table: torch.Tensor,
+         positions: torch.Tensor, layout: str = "half", inverse: bool = False,
+         q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None, stream=None
+         ) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
+    """(q, k) rotated at each token's position (the way back with ``inverse``)."""
+    if q is not None and q_out is None:
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if k is not None and k_out is None:
+        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    some = q if q is not None else k
+    _need(some is not None and some.is_cuda, "q or k must be a CUDA tensor")
+    run = RopeKernel(some.device.index).create_run(q, k, table, positions, q_out, k_out, layout,
+                                                   inverse)
+    encode_run(stream, run)
+    return q_out, k_out
