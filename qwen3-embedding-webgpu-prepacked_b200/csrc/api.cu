@@ -1291,6 +1291,24 @@ qwa_status prefix_shape(qwa_ctx* ctx, const int32_t* cu_q, const int32_t* cu_k, 
   return QWA_OK;
 }
 
+// 3-D map of 8-bit codes {128 dims, heads, rows}, box {128, 1, 128}: one load
+// lands as 128 rows x 128 B, not swizzled.
+qwa_status make_code_map(qwa_ctx* ctx, CUtensorMap* map, const void* base, int heads,
+                         int64_t rows) {
+  cuuint64_t dims[3] = {128, static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[2] = {128, static_cast<cuuint64_t>(heads) * 128};
+  cuuint32_t box[3] = {128, 1, 128};
+  cuuint32_t elem[3] = {1, 1, 1};
+  CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims,
+                        strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(ctx, QWA_ERR_CUDA, "cuTensorMapEncodeTiled (codes) failed (%d)",
+                static_cast<int>(r));
+  return QWA_OK;
+}
+
 // CTAs of a cluster that share a block's tiles: as many as keep the SMs busy,
 // each with a tile at least.
 int prefix_splits(const PrefixWork& w, int items, int sms) {
@@ -1468,16 +1486,20 @@ qwa_status qwa_prefix_attention(qwa_ctx* ctx, const qwa_prefix_plan* plan, int d
     const int64_t at = first_slot * kv_width * (format == QWA_KV_PLAIN ? 2 : 1);
     a.k_prefix = static_cast<const uint8_t*>(cache->k) + at;
     a.v_prefix = static_cast<const uint8_t*>(cache->v) + at;
-    if (format == QWA_KV_PLAIN) {
+    if (format != QWA_KV_PLAIN) {
+      if ((st = make_code_map(ctx, &m.pk, a.k_prefix, s.kv_heads, s.prefix_len)) != QWA_OK)
+        return st;
+      if ((st = make_code_map(ctx, &m.pv, a.v_prefix, s.kv_heads, s.prefix_len)) != QWA_OK)
+        return st;
+      a.k_scale = cache->k_scale + first_slot * s.kv_heads;
+      a.v_scale = cache->v_scale + first_slot * s.kv_heads;
+    } else {
       if ((st = make_map(ctx, &m.pk, a.k_prefix, s.kv_heads, s.prefix_len, kv_width * 2, 128, 1,
                          bf16)) != QWA_OK)
         return st;
       if ((st = make_map(ctx, &m.pv, a.v_prefix, s.kv_heads, s.prefix_len, kv_width * 2, 128, 1,
                          bf16)) != QWA_OK)
         return st;
-    } else {
-      a.k_scale = cache->k_scale + first_slot * s.kv_heads;
-      a.v_scale = cache->v_scale + first_slot * s.kv_heads;
     }
   }
   a.items = plan->items;

@@ -10,14 +10,15 @@
 // Rows of different requests share a tile, so the prefix is read and
 // multiplied once for the whole block; own keys of other requests are masked.
 //
-// Warp roles (384 threads):
+// Warp roles:
 //   warp 0      TMA producer: Q tiles, then K_j / V_j into a 3-slot ring
 //   warp 1      TMEM owner; lane 0 issues every tcgen05.mma and commit
-//   warps 2-3   prepare tiles: 8-bit prefix tiles are read with plain loads,
-//               converted and written to their slot; V tiles with masked keys
-//               are cleared of values that are not finite (guard, below)
 //   warps 4-7   softmax of tile A, one thread a row
 //   warps 8-11  softmax of tile B
+//   warps 2-3 (16-bit prefix) or 12-15 (8-bit) prepare tiles: 8-bit prefix tiles
+//               are read with plain loads, converted and written to their
+//               slot; V tiles with masked keys are cleared of values that are
+//               not finite (guard, below)
 // TMEM: S_A, S_B (P over them, as 16-bit pairs), O_A, O_B; 512 columns.
 // MMA order per key tile: S_A(j), PV_B(j-1), S_B(j), PV_A(j), so the softmax of
 // one tile runs under the MMAs of the other.
@@ -44,40 +45,62 @@ namespace qwa {
 namespace {
 using namespace attn;
 
-constexpr int kThreads = 384;
-constexpr int kSoftmaxWarp0 = 4;
-constexpr int kRegsSupport = 104;
-constexpr int kRegsSoftmax = 200;
-static_assert(128 * kRegsSupport + 256 * kRegsSoftmax <= kThreads * 168, "register split");
-constexpr uint32_t kQEmptyArrivals = 8;
-constexpr uint32_t kSlotFullArrivals = 2;  // the two preparing warps, or the producer twice
-constexpr int kSlots = 3;
-constexpr uint32_t kQBufBytes = 2 * kTileBytes;
-constexpr uint32_t kSlotOff = 2 * kQBufBytes;
-constexpr uint32_t kStatOff = kSlotOff + kSlots * kTileBytes;  // split: (m, l) of 256 rows
-constexpr uint32_t kBarOff = kStatOff + 256 * 8;
-enum Bar : int {
-  kQFull = 0,
-  kQEmpty = kQFull + 2,
-  kSlotFull = kQEmpty + 2,
-  kSlotEmpty = kSlotFull + kSlots,
-  kRawFull = kSlotEmpty + kSlots,  // a guarded V tile has landed, not yet searched
-  kSFull = kRawFull + kSlots,
-  kPLo = kSFull + 2,
-  kPHi = kPLo + 2,
-  kOFinal = kPHi + 2,
-  kDrain = kOFinal + 2,
-  kNumBars = kDrain + 1
+// Threads, registers and shared memory of a format. A 16-bit prefix needs no
+// conversion: warps 2-3 prepare, the softmax warps get 200 registers and the
+// ring four slots. For 8 bits a fourth warpgroup of four preparing warps joins
+// and takes its registers from the others, and raw tiles wait in a ring of
+// their own. (Two warps with the codes prefetched into registers took 6900 cycles for
+// a tile of 128 keys, three times its MMAs.)
+template <int kFormat>
+struct Layout {
+  static constexpr bool kConverts = kFormat != kKvPlain;
+  static constexpr int kThreads = kConverts ? 512 : 384;
+  static constexpr int kPrepWarp0 = kConverts ? 12 : 2;
+  static constexpr int kPrepWarps = kConverts ? 4 : 2;
+  static constexpr int kRegsLaunch = kConverts ? 128 : 168;
+  static constexpr int kRegsSupport = kConverts ? 72 : 104;  // producer and issuer
+  static constexpr int kRegsPrep = 72;                       // of the fourth warpgroup
+  static constexpr int kRegsSoftmax = kConverts ? 184 : 200;
+  static_assert(128 * kRegsSupport + 256 * kRegsSoftmax + (kConverts ? 128 * kRegsPrep : 0) <=
+                    kThreads * kRegsLaunch,
+                "register split");
+  static constexpr int kSlots = kConverts ? 3 : 4;   // K_j and V_j tiles in use
+  static constexpr int kStages = kConverts ? 3 : 0;  // raw 8-bit tiles on their way
+  static constexpr uint32_t kSlotOff = 2 * kTileBytes;  // after Q_A, Q_B
+  static constexpr uint32_t kStageOff = kSlotOff + kSlots * kTileBytes;
+  static constexpr uint32_t kEpiOff = kStageOff + kStages * (kTileBytes / 2);
+  static constexpr uint32_t kBarOff = kEpiOff + 8 * 2048;  // 2 KB for each softmax warp
+  enum Bar : int {
+    kQFull = 0,
+    kQEmpty,
+    kSlotEmpty,
+    kLanded = kSlotEmpty + kSlots,  // a tile has been copied into the slot
+    kReady = kLanded + kSlots,      // the preparing warps are done with it
+    kOwnGo = kReady + kSlots,       // 8 bits: an own tile may be copied into the slot
+    kStageFull = kOwnGo + kSlots,
+    kStageEmpty = kStageFull + kStages,
+    kSFull = kStageEmpty + kStages,
+    kPLo = kSFull + 2,
+    kPHi = kPLo + 2,
+    kOFinal = kPHi + 2,
+    kDrain = kOFinal + 2,
+    kNumBars
+  };
+  static constexpr uint32_t kHolderOff = kBarOff + 8 * kNumBars;
+  static constexpr uint32_t kAbortOff = kHolderOff + 4;
+  static constexpr uint32_t kLimitOff = kHolderOff + 8;
+  // li + 1 of the last item with values put aside. The preparing warps may be
+  // ahead of an epilogue: it takes a later item's number for its own, and its search
+  // then finds what there is.
+  static constexpr uint32_t kBadOff = kLimitOff + 8;
+  static constexpr uint32_t kSmemUsed = kBadOff + 4;
+  static constexpr uint32_t kSmemBytes = kSmemUsed + 1024;  // + alignment
+  static_assert(kLimitOff % 8 == 0 && kSmemBytes <= 232448, "shared memory budget");
+  // split: O of tile A over Q (64 KB), of tile B over the first two slots, and
+  // (m, l) of the 256 rows where the other form stages its output
+  static constexpr uint32_t kPartOffB = kSlotOff;
 };
-constexpr uint32_t kHolderOff = kBarOff + 8 * kNumBars;
-constexpr uint32_t kAbortOff = kHolderOff + 4;
-constexpr uint32_t kLimitOff = (kHolderOff + 8 + 7) / 8 * 8;
-// li + 1 of the last item with values put aside, by li % 4: the preparing
-// warps run at most two items ahead of an epilogue
-constexpr uint32_t kBadOff = kLimitOff + 8;
-constexpr uint32_t kSmemUsed = kBadOff + 16;
-constexpr uint32_t kSmemBytes = 232448;  // all of it: what is over covers the alignment to 1024
-static_assert(kSmemUsed + 768 <= kSmemBytes, "shared memory budget");
+constexpr int kSoftmaxWarp0 = 4;
 
 template <bool kBf16>
 __host__ __device__ constexpr uint32_t idesc_16(uint32_t m, uint32_t n, bool b_mn_major) {
@@ -203,73 +226,50 @@ __device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
   return v;
 }
 
-// The raw codes of one prefix tile, held by 64 threads: thread (w, lane) has
-// the 16 codes of unit lane % 8 in the rows 8 i + 4 w + lane / 8.
-struct RawTile {
-  uint4 code[16];
-  uint32_t scale;  // bytes of rows i = lane / 4 (low) and i = 8 + lane / 4, sub-row lane % 4
-};
-__device__ __forceinline__ void load_raw(RawTile& raw, const uint8_t* codes, const uint8_t* scales,
-                                         int kv_heads, int head, int key, int rows, int w,
-                                         int lane) {
-  const int64_t stride = static_cast<int64_t>(kv_heads) * kHeadDim;
-  const uint8_t* src = codes + key * stride + head * kHeadDim + (lane & 7) * 16;
-  const int r0 = 4 * w + (lane >> 3);
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int r = r0 + 8 * i;
-    raw.code[i] = r < rows ? __ldg(reinterpret_cast<const uint4*>(src + r * stride))
-                           : make_uint4(0u, 0u, 0u, 0u);
-  }
-  raw.scale = 0x7f7fu;  // 2^0 for rows that do not exist
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int r = 8 * (8 * i + (lane >> 2)) + 4 * w + (lane & 3);
-    if (r < rows) {
-      const uint32_t s = __ldg(scales + static_cast<int64_t>(key + r) * kv_heads + head);
-      raw.scale = (raw.scale & ~(0xffu << (8 * i))) | (s << (8 * i));
-    }
-  }
-}
-// Converts it into the slot's swizzled layout. guard: values that are not
-// finite become 0; returns whether there were any.
+// Converts a landed raw tile (128 rows of 128 codes) into the slot's swizzled
+// layout. Lane (w, l) takes the 16 codes of unit l % 8 in the rows 16 i + 4 w +
+// l / 8, i < 8; `scale` is the byte of row 16 (l / 4) + 4 w + l % 4. guard: values
+// that are not finite become 0; returns whether there were any.
 template <bool kBf16, int kFormat>
-__device__ __forceinline__ bool store_raw(const RawTile& raw, uint32_t slot, bool guard, int w,
-                                          int lane) {
+__device__ __forceinline__ bool convert_tile(uint32_t stage, uint32_t slot, uint32_t scale,
+                                             bool guard, int w, int lane) {
   bool bad = false;
-  const int u = lane & 7;                       // dims 16 u .. 16 u + 15
-  const uint32_t half_base = slot + (u >> 2) * kHalfBytes;
-  const int first = u >> 2;  // lanes of the second half write their odd unit first (banks)
+  const int u = lane & 7;    // dims 16 u .. 16 u + 15
+  const int odd = u >> 2;    // lanes of the second half write their odd unit first (banks)
+  const int r0 = 4 * w + (lane >> 3);
+  const uint32_t from = stage + r0 * 128 + u * 16;
+  // r % 8 is the same for all of a lane's rows, 16 apart
+  const uint32_t base = slot + odd * kHalfBytes + r0 * 128;
+  const uint32_t at_a = base + (static_cast<uint32_t>((u & 3) * 2 + odd) ^ (r0 & 7)) * 16;
+  const uint32_t at_b = base + (static_cast<uint32_t>((u & 3) * 2 + 1 - odd) ^ (r0 & 7)) * 16;
+  const uint32_t mine = kBf16 ? scale : half2_pow2(static_cast<int>(scale) - 127);
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int r = 8 * i + 4 * w + (lane >> 3);
-    const uint32_t both = __shfl_sync(0xffffffffu, raw.scale, (i & 7) * 4 + (lane >> 3));
-    const int e = static_cast<int>((both >> (8 * (i >> 3))) & 0xffu) - 127;
-    const uint32_t h2 = half2_pow2(e);
+  for (int i = 0; i < 8; ++i) {
+    const uint4 raw = ld_shared_v4(from + i * 2048);
+    const uint32_t sc = __shfl_sync(0xffffffffu, mine, i * 4 + (lane >> 3));
+    const int e = static_cast<int>(sc) - 127;  // bf16
     const float sa = pow2f(e / 2), sb = pow2f(e - e / 2);
-    const uint32_t c[4] = {raw.code[i].x, raw.code[i].y, raw.code[i].z, raw.code[i].w};
+    const uint32_t c[4] = {raw.x, raw.y, raw.z, raw.w};
     uint32_t v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      v[j] = code_pair<kBf16, kFormat>((c[j >> 1] >> (16 * (j & 1))) & 0xffffu, h2, sa, sb);
-      if (guard) v[j] = finite_only<kBf16>(v[j], bad);
-    }
-    const uint32_t row = half_base + r * 128;
+    for (int j = 0; j < 8; ++j)
+      v[j] = code_pair<kBf16, kFormat>((c[j >> 1] >> (16 * (j & 1))) & 0xffffu, sc, sa, sb);
+    if (guard) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int which = j ^ first;
-      const uint32_t unit = static_cast<uint32_t>((u & 3) * 2 + which) ^ (r & 7);
-      if (which == 0) st_shared_v4(row + unit * 16, v[0], v[1], v[2], v[3]);
-      else st_shared_v4(row + unit * 16, v[4], v[5], v[6], v[7]);
+      for (int j = 0; j < 8; ++j) v[j] = finite_only<kBf16>(v[j], bad);
     }
+    st_shared_v4(at_a + i * 2048, odd ? v[4] : v[0], odd ? v[5] : v[1], odd ? v[6] : v[2],
+                 odd ? v[7] : v[3]);
+    st_shared_v4(at_b + i * 2048, odd ? v[0] : v[4], odd ? v[1] : v[5], odd ? v[2] : v[6],
+                 odd ? v[3] : v[7]);
   }
   return bad;
 }
 // Clears a landed V tile (rows [0, width)) of values that are not finite.
-template <bool kBf16>
+template <bool kBf16, int kWarps>
 __device__ __forceinline__ bool guard_tile(uint32_t slot, int width, int w, int lane) {
   bool bad = false;
-  for (int r = 4 * w + (lane >> 3); r < width; r += 8) {
+  for (int r = 4 * w + (lane >> 3); r < width; r += 4 * kWarps) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const uint32_t at = slot + h * kHalfBytes + r * 128 + (lane & 7) * 16;
@@ -379,61 +379,140 @@ __device__ __forceinline__ void share_tiles(const Share& s, const PrefixItem& it
   }
 }
 
+// The preparing warps (the file's head): w counts them from 0. They follow every
+// use of the ring, because a parity says nothing to a role that is more than a
+// phase away: each waits for its slot to be empty, then converts, or (8 bits) lets
+// the producer, which runs ahead on raw tiles, load an own tile.
 template <bool kBf16, int kFormat, bool kSplit>
-__global__ void __launch_bounds__(kThreads, 1)
+__device__ __forceinline__ void prepare_tiles(const PrefixArgs& args, const Share& share,
+                                              uint32_t sbase, int w, int lane,
+                                              volatile int* abort_flag,
+                                              const volatile unsigned long long* wait_limit,
+                                              volatile int* bad_item) {
+  using L = Layout<kFormat>;
+  auto bar = [&](int i) -> uint32_t { return sbase + L::kBarOff + 8u * i; };
+  // a warp-wide wait: every lane leaves it with the same answer
+  auto wait = [&](uint32_t b, uint32_t parity, int code) -> bool {
+    const bool got = mbar_wait(b, parity, abort_flag, args.status, code, wait_limit);
+    return __all_sync(0xffffffffu, got);
+  };
+  auto publish = [&](int s, bool bad, int li) {
+    if (__any_sync(0xffffffffu, bad) && lane == 0) *bad_item = li + 1;
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(L::kReady + s));
+  };
+  int s = 0;               // slot of the current use
+  uint32_t parity = 1;     // of the phase that says the slot is empty
+  int g = 0;               // raw stage of the next 8-bit tile, and its parity
+  uint32_t g_parity = 0;
+  uint32_t landed = 0;     // bit slot: parity of the slot's next copy
+  for (int it = share.beg, li = 0; it < share.end; ++it, ++li) {
+    const PrefixItem item = args.items[it];
+    int tb, te;
+    share_tiles<kSplit>(share, item, tb, te);
+    // this lane's scale byte of a tile, fetched one tile ahead
+    auto scale_of = [&](const PrefixTile& tile, int kv) -> uint32_t {
+      const int r = tile.key + 16 * (lane >> 2) + 4 * w + (lane & 3);
+      if ((tile.info & kTileOwn) || r >= args.prefix_len) return 127;
+      return __ldg((kv ? args.v_scale : args.k_scale) +
+                   static_cast<int64_t>(r) * args.kv_heads + item.head);
+    };
+    PrefixTile next = args.tiles[tb];
+    uint32_t scale = 0;
+    if (L::kConverts) scale = scale_of(next, 0);
+    for (int j = tb; j < te; ++j) {
+      const PrefixTile tile = next;
+      next = args.tiles[j + 1 < te ? j + 1 : j];
+      const bool own = tile.info & kTileOwn;
+      const bool guard = tile.info & kTileGuard;
+      for (int kv = 0; kv < 2; ++kv) {
+        const uint32_t slot = sbase + L::kSlotOff + s * kTileBytes;
+        if (!wait(bar(L::kSlotEmpty + s), parity, kDevTimeoutSlotEmpty)) return;
+        if (L::kConverts && !own) {
+          const uint32_t now = scale;
+          scale = kv == 0 ? scale_of(tile, 1) : scale_of(next, 0);
+          if (!wait(bar(L::kStageFull + g), g_parity, kDevTimeoutSlotFull)) return;
+          const bool bad = convert_tile<kBf16, kFormat>(
+              sbase + L::kStageOff + g * (kTileBytes / 2), slot, now, kv == 1 && guard, w, lane);
+          publish(s, bad, li);  // all lanes have read the raw tile
+          if (lane == 0) mbar_arrive(bar(L::kStageEmpty + g));
+          if (++g == L::kStages) {
+            g = 0;
+            g_parity ^= 1;
+          }
+        } else {
+          if (L::kConverts && w == 0 && lane == 0) mbar_arrive(bar(L::kOwnGo + s));
+          const uint32_t copy = (landed >> s) & 1u;
+          landed ^= 1u << s;
+          if (kv == 1 && guard) {
+            if (!wait(bar(L::kLanded + s), copy, kDevTimeoutSlotFull)) return;
+            publish(s, guard_tile<kBf16, L::kPrepWarps>(slot, tile.info & kTileWidthMask, w, lane),
+                    li);
+          }
+        }
+        if (++s == L::kSlots) {
+          s = 0;
+          parity ^= 1;
+        }
+      }
+    }
+  }
+}
+
+template <bool kBf16, int kFormat, bool kSplit>
+__global__ void __launch_bounds__(Layout<kFormat>::kThreads, 1)
     prefix_attention_kernel(const __grid_constant__ CUtensorMap tm_q,
                             const __grid_constant__ CUtensorMap tm_k,
                             const __grid_constant__ CUtensorMap tm_v,
                             const __grid_constant__ CUtensorMap tm_pk,
                             const __grid_constant__ CUtensorMap tm_pv,
                             const __grid_constant__ PrefixArgs args) {
+  using L = Layout<kFormat>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  if (smem - smem_raw + kSmemUsed > kSmemBytes) {  // the same in every CTA
-    if (threadIdx.x == 0) atomicCAS(args.status, 0, kDevSharedLayout);
-    return;
-  }
   const uint32_t sbase = smem_addr(smem);
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + kHolderOff);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kAbortOff);
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + L::kHolderOff);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kAbortOff);
   volatile unsigned long long* wait_limit =
-      reinterpret_cast<volatile unsigned long long*>(smem + kLimitOff);
-  volatile int* bad_item = reinterpret_cast<volatile int*>(smem + kBadOff);
-  auto bar = [&](int i) -> uint32_t { return sbase + kBarOff + 8u * i; };
+      reinterpret_cast<volatile unsigned long long*>(smem + L::kLimitOff);
+  volatile int* bad_item = reinterpret_cast<volatile int*>(smem + L::kBadOff);
+  auto bar = [&](int i) -> uint32_t { return sbase + L::kBarOff + 8u * i; };
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const Share share = my_share<kSplit>(args);
 
   if (threadIdx.x == 0) {
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(bar(kQFull + b), 1);
-      mbar_init(bar(kQEmpty + b), kQEmptyArrivals);
-      bad_item[2 * b] = bad_item[2 * b + 1] = 0;
+    mbar_init(bar(L::kQFull), 1);
+    mbar_init(bar(L::kQEmpty), 1);
+    *bad_item = 0;
+    for (int i = 0; i < L::kSlots; ++i) {
+      mbar_init(bar(L::kSlotEmpty + i), 1);
+      mbar_init(bar(L::kLanded + i), 1);
+      mbar_init(bar(L::kReady + i), L::kPrepWarps);
+      mbar_init(bar(L::kOwnGo + i), 1);
     }
-    for (int s = 0; s < kSlots; ++s) {
-      mbar_init(bar(kSlotFull + s), kSlotFullArrivals);
-      mbar_init(bar(kSlotEmpty + s), 1);
-      mbar_init(bar(kRawFull + s), 1);
+    for (int i = 0; i < L::kStages; ++i) {
+      mbar_init(bar(L::kStageFull + i), 1);
+      mbar_init(bar(L::kStageEmpty + i), L::kPrepWarps);
     }
     for (int x = 0; x < 2; ++x) {
-      mbar_init(bar(kSFull + x), 1);
-      mbar_init(bar(kPLo + x), 128);
-      mbar_init(bar(kPHi + x), 128);
-      mbar_init(bar(kOFinal + x), 1);
+      mbar_init(bar(L::kSFull + x), 1);
+      mbar_init(bar(L::kPLo + x), 128);
+      mbar_init(bar(L::kPHi + x), 128);
+      mbar_init(bar(L::kOFinal + x), 1);
     }
-    mbar_init(bar(kDrain), 1);
+    mbar_init(bar(L::kDrain), 1);
     *abort_flag = 0;
     *wait_limit = args.wait_ns;
     fence_mbar_init();
     tma_prefetch_desc(&tm_q);
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
-    if (kFormat == kKvPlain) {
-      tma_prefetch_desc(&tm_pk);
-      tma_prefetch_desc(&tm_pv);
-    }
+    tma_prefetch_desc(&tm_pk);
+    tma_prefetch_desc(&tm_pv);
   }
   if (warp == 1) {
     tmem_alloc(smem_addr(tmem_holder), kTmemCols);
@@ -447,72 +526,92 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int tile_rows = args.group * args.tile_tokens;
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsSupport));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::kRegsSupport));
     if (warp == 0) {
       // ---------------------------------------------------------- producer
       if (lane == 0) {
-        int c = 0;
         bool ok = true;
-        // phases whose copies may be in flight at the end: bit i + 8 valid, bit
-        // i parity; i = slot (full), 3 + slot (raw), 6 + Q buffer
-        uint32_t flying = 0;
-        uint32_t raw_uses = 0;  // bit s: parity of the next raw phase of slot s
-        auto fly = [&](int i, uint32_t parity) {
-          flying = (flying & ~(1u << i)) | (1u << (i + 16)) | (parity << i);
+        int s = 0;
+        uint32_t parity = 1;  // of the phase that says slot s is empty (16 bits)
+        int g = 0;
+        uint32_t g_parity = 1;   // raw stage g is empty
+        uint32_t go_parity = 0;  // bit slot: parity of the slot's next own tile (8 bits)
+        uint32_t landed = 0;     // bit slot: parity of the slot's next copy
+        // The last phase issued on each barrier that counts copies (Q, slots,
+        // stages), waited for before exit so that no copy lands after it. Only
+        // copies complete these phases, one in flight on each.
+        uint32_t fly_on = 0, fly_parity = 0;
+        auto fly = [&](int i, uint32_t p) {
+          fly_on |= 1u << i;
+          fly_parity = (fly_parity & ~(1u << i)) | (p << i);
         };
         for (int it = share.beg, li = 0; ok && it < share.end; ++it, ++li) {
           const PrefixItem item = args.items[it];
           int tb, te;
           share_tiles<kSplit>(share, item, tb, te);
-          const int qb = li & 1;
           const int nx = item.tokens > args.tile_tokens ? 2 : 1;
-          if (!(ok = mbar_wait(bar(kQEmpty + qb), ((li >> 1) & 1) ^ 1, abort_flag, args.status,
+          if (!(ok = mbar_wait(bar(L::kQEmpty), (li & 1) ^ 1, abort_flag, args.status,
                                kDevTimeoutQ, wait_limit)))
             break;
-          mbar_arrive_expect_tx(bar(kQFull + qb), nx * tile_rows * 256);
-          fly(2 * kSlots + qb, (li >> 1) & 1);
+          mbar_arrive_expect_tx(bar(L::kQFull), nx * tile_rows * 256);
+          fly(0, li & 1);
           for (int x = 0; x < nx; ++x) {
-            const uint32_t dst = sbase + qb * kQBufBytes + x * kTileBytes;
+            const uint32_t dst = sbase + x * kTileBytes;
             const int t0 = item.row0 + x * args.tile_tokens;
-            tma_load_3d(dst, &tm_q, bar(kQFull + qb), 0, item.head * args.group, t0);
-            tma_load_3d(dst + kHalfBytes, &tm_q, bar(kQFull + qb), 64, item.head * args.group, t0);
+            tma_load_3d(dst, &tm_q, bar(L::kQFull), 0, item.head * args.group, t0);
+            tma_load_3d(dst + kHalfBytes, &tm_q, bar(L::kQFull), 64, item.head * args.group, t0);
           }
+          PrefixTile next = args.tiles[tb];
           for (int j = tb; ok && j < te; ++j) {
-            const PrefixTile tile = args.tiles[j];
+            const PrefixTile tile = next;  // the next one is loaded a tile ahead
+            next = args.tiles[j + 1 < te ? j + 1 : j];
             const bool own = tile.info & kTileOwn;
-            for (int kv = 0; kv < 2; ++kv, ++c) {
-              const int s = c % kSlots;
-              if (!(ok = mbar_wait(bar(kSlotEmpty + s), ((c / kSlots) & 1) ^ 1, abort_flag,
-                                   args.status, kDevTimeoutSlotEmpty, wait_limit)))
-                break;
-              // what this slot held has been used, so it has landed
-              flying &= ~((1u << (s + 16)) | (1u << (s + kSlots + 16)));
-              if (kFormat != kKvPlain && !own) continue;  // the preparing warps fill it
-              const uint32_t dst = sbase + kSlotOff + s * kTileBytes;
-              const CUtensorMap* tm = own ? (kv ? &tm_v : &tm_k) : (kv ? &tm_pv : &tm_pk);
-              uint32_t full = bar(kSlotFull + s);
-              if (kv == 1 && (tile.info & kTileGuard)) {
-                full = bar(kRawFull + s);
-                fly(kSlots + s, (raw_uses >> s) & 1u);
-                raw_uses ^= 1u << s;
-                mbar_arrive_expect_tx(full, kTileBytes);
+            for (int kv = 0; kv < 2; ++kv) {
+              if (L::kConverts && !own) {  // a raw tile, converted by the preparing warps
+                if (!(ok = mbar_wait(bar(L::kStageEmpty + g), g_parity, abort_flag, args.status,
+                                     kDevTimeoutSlotEmpty, wait_limit)))
+                  break;
+                mbar_arrive_expect_tx(bar(L::kStageFull + g), kTileBytes / 2);
+                fly(1 + L::kSlots + g, g_parity ^ 1);
+                tma_load_3d(sbase + L::kStageOff + g * (kTileBytes / 2), kv ? &tm_pv : &tm_pk,
+                            bar(L::kStageFull + g), 0, item.head, tile.key);
+                if (++g == L::kStages) {
+                  g = 0;
+                  g_parity ^= 1;
+                }
               } else {
-                fly(s, (c / kSlots) & 1);
+                if (L::kConverts) {
+                  if (!(ok = mbar_wait(bar(L::kOwnGo + s), (go_parity >> s) & 1u, abort_flag,
+                                       args.status, kDevTimeoutSlotEmpty, wait_limit)))
+                    break;
+                  go_parity ^= 1u << s;
+                } else if (!(ok = mbar_wait(bar(L::kSlotEmpty + s), parity, abort_flag,
+                                            args.status, kDevTimeoutSlotEmpty, wait_limit))) {
+                  break;
+                }
+                const uint32_t dst = sbase + L::kSlotOff + s * kTileBytes;
+                const CUtensorMap* tm = own ? (kv ? &tm_v : &tm_k) : (kv ? &tm_pv : &tm_pk);
+                const uint32_t full = bar(L::kLanded + s);
+                fly(1 + s, (landed >> s) & 1u);
+                landed ^= 1u << s;
                 mbar_arrive_expect_tx(full, kTileBytes);
-                mbar_arrive(full);  // the second of kSlotFullArrivals
+                tma_load_3d(dst, tm, full, 0, item.head, tile.key);
+                tma_load_3d(dst + kHalfBytes, tm, full, 64, item.head, tile.key);
               }
-              tma_load_3d(dst, tm, full, 0, item.head, tile.key);
-              tma_load_3d(dst + kHalfBytes, tm, full, 64, item.head, tile.key);
+              if (++s == L::kSlots) {
+                s = 0;
+                parity ^= 1;
+              }
             }
           }
         }
         bool drained = true;
-        for (int i = 0; i < 2 * kSlots + 2; ++i)
-          if ((flying >> (i + 16)) & 1u) {
-            const int b = i < kSlots ? kSlotFull + i
-                                     : (i < 2 * kSlots ? kRawFull + i - kSlots
-                                                       : kQFull + i - 2 * kSlots);
-            drained &= mbar_drain(bar(b), (flying >> i) & 1u, *wait_limit);
+        for (int i = 0; i < 1 + L::kSlots + L::kStages; ++i)
+          if ((fly_on >> i) & 1u) {
+            const int b = i == 0 ? L::kQFull
+                                 : (i <= L::kSlots ? L::kLanded + i - 1
+                                                   : L::kStageFull + i - 1 - L::kSlots);
+            drained &= mbar_drain(bar(b), (fly_parity >> i) & 1u, *wait_limit);
           }
         if (!drained) atomicCAS(args.status, 0, kDevTimeoutDrain);
       }
@@ -521,30 +620,41 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) {
         const uint32_t t_s[2] = {tmem, tmem + 128};
         const uint32_t t_o[2] = {tmem + 256, tmem + 384};
-        const uint64_t q_desc0 = smem_desc_sw128(sbase, 16, 1024);
-        const uint64_t k_desc0 = smem_desc_sw128(sbase + kSlotOff, 16, 1024);
-        const uint64_t v_desc0 = smem_desc_sw128(sbase + kSlotOff, kHalfBytes, 1024);
+        const uint64_t qa = smem_desc_sw128(sbase, 16, 1024);
+        const uint64_t qbd = qa + (kTileBytes >> 4);
+        const uint64_t k_desc0 = smem_desc_sw128(sbase + L::kSlotOff, 16, 1024);
+        const uint64_t v_desc0 = smem_desc_sw128(sbase + L::kSlotOff, kHalfBytes, 1024);
         bool ok = true;
-        int t = 0;   // key tiles so far (tile A runs on all of them)
-        int tB = 0;  // those with a tile B
+        int s = 0;               // slot of the next use
+        uint32_t landed = 0;     // bit slot: parity of its next copy
+        uint32_t ready = 0;      // bit slot: parity of its next prepared tile
+        uint32_t tA = 0, tB = 0; // parity of tile A's and tile B's next key tile
         bool have_prev = false;  // PV_B of the previous tile still to issue
         int prev_v = 0, prev_nk = 8;
         bool prev_acc = false, prev_last = false;
-        // PV_B of the previous tile: its P has parity (tB - 1)
+        // waits for the tile in slot s, whoever completes it
+        auto wait_tile = [&](bool copied, bool prepared) -> bool {
+          const uint32_t l = (landed >> s) & 1u, r = (ready >> s) & 1u;
+          if (copied) landed ^= 1u << s;
+          if (prepared) ready ^= 1u << s;
+          return mbar_wait(prepared ? bar(L::kReady + s) : bar(L::kLanded + s), prepared ? r : l,
+                           abort_flag, args.status, kDevTimeoutSlotFull, wait_limit);
+        };
+        // PV_B of the previous tile, whose P has parity tB ^ 1
         auto issue_prev = [&]() -> bool {
           const uint64_t vd = v_desc0 + ((prev_v * kTileBytes) >> 4);
-          if (!mbar_wait(bar(kPLo + 1), (tB - 1) & 1, abort_flag, args.status, kDevTimeoutPFull,
+          if (!mbar_wait(bar(L::kPLo + 1), tB ^ 1u, abort_flag, args.status, kDevTimeoutPFull,
                          wait_limit))
             return false;
           tc_fence_after();
           issue_pv_part<kBf16>(t_o[1], t_s[1], vd, prev_acc, prev_nk, 0);
-          if (!mbar_wait(bar(kPHi + 1), (tB - 1) & 1, abort_flag, args.status, kDevTimeoutPFull,
+          if (!mbar_wait(bar(L::kPHi + 1), tB ^ 1u, abort_flag, args.status, kDevTimeoutPFull,
                          wait_limit))
             return false;
           tc_fence_after();
           issue_pv_part<kBf16>(t_o[1], t_s[1], vd, prev_acc, prev_nk, 1);
-          tc_commit(bar(kSlotEmpty + prev_v));
-          if (prev_last) tc_commit(bar(kOFinal + 1));
+          tc_commit(bar(L::kSlotEmpty + prev_v));
+          if (prev_last) tc_commit(bar(L::kOFinal + 1));
           have_prev = false;
           return true;
         };
@@ -553,120 +663,77 @@ __global__ void __launch_bounds__(kThreads, 1)
           int tb, te;
           share_tiles<kSplit>(share, item, tb, te);
           const int nx = item.tokens > args.tile_tokens ? 2 : 1;
-          const int qb = li & 1;
-          const uint64_t qa = q_desc0 + ((qb * kQBufBytes) >> 4);
-          const uint64_t qbd = qa + (kTileBytes >> 4);
-          if (!(ok = mbar_wait(bar(kQFull + qb), (li >> 1) & 1, abort_flag, args.status,
-                               kDevTimeoutQ, wait_limit)))
+          int next_info = args.tiles[tb].info;
+          // Q is loaded once the last S MMAs of the item before are done; if it
+          // is still on its way, the pending PV_B goes first
+          if (have_prev && !mbar_try_wait(bar(L::kQFull), li & 1) && !(ok = issue_prev())) break;
+          if (!(ok = mbar_wait(bar(L::kQFull), li & 1, abort_flag, args.status, kDevTimeoutQ,
+                               wait_limit)))
             break;
-          for (int j = tb; j < te; ++j, ++t) {
-            const int ck = 2 * t, sk = ck % kSlots;
-            const int cv = 2 * t + 1, sv = cv % kSlots;
-            const int width = args.tiles[j].info & kTileWidthMask;
-            const uint64_t k_desc = k_desc0 + ((sk * kTileBytes) >> 4);
-            if (!(ok = mbar_wait(bar(kSlotFull + sk), (ck / kSlots) & 1, abort_flag, args.status,
-                                 kDevTimeoutSlotFull, wait_limit)))
-              break;
+          for (int j = tb; j < te; ++j) {
+            const int info = next_info;
+            next_info = args.tiles[j + 1 < te ? j + 1 : j].info;
+            const int width = info & kTileWidthMask;
+            const bool converted = L::kConverts && !(info & kTileOwn);
+            const bool last = j == te - 1;
+            const int sk = s;
+            if (!(ok = wait_tile(!converted, converted))) break;
+            s = s + 1 == L::kSlots ? 0 : s + 1;
             tc_fence_after();
+            const uint64_t k_desc = k_desc0 + ((sk * kTileBytes) >> 4);
             const uint32_t idesc = idesc_16<kBf16>(128, width, false);
             issue_qk(t_s[0], qa, k_desc, idesc);
-            tc_commit(bar(kSFull + 0));
+            tc_commit(bar(L::kSFull + 0));
             if (have_prev && !(ok = issue_prev())) break;
             if (nx == 2) {
               issue_qk(t_s[1], qbd, k_desc, idesc);
-              tc_commit(bar(kSFull + 1));
+              tc_commit(bar(L::kSFull + 1));
             }
-            tc_commit(bar(kSlotEmpty + sk));
-            if (!(ok = mbar_wait(bar(kSlotFull + sv), (cv / kSlots) & 1, abort_flag, args.status,
-                                 kDevTimeoutSlotFull, wait_limit)))
-              break;
+            tc_commit(bar(L::kSlotEmpty + sk));
+            if (last) tc_commit(bar(L::kQEmpty));
+            const int sv = s;
+            if (!(ok = wait_tile(!converted, converted || (info & kTileGuard)))) break;
+            s = s + 1 == L::kSlots ? 0 : s + 1;
             const uint64_t vd = v_desc0 + ((sv * kTileBytes) >> 4);
-            if (!(ok = mbar_wait(bar(kPLo + 0), t & 1, abort_flag, args.status, kDevTimeoutPFull,
+            if (!(ok = mbar_wait(bar(L::kPLo + 0), tA, abort_flag, args.status, kDevTimeoutPFull,
                                  wait_limit)))
               break;
             tc_fence_after();
             issue_pv_part<kBf16>(t_o[0], t_s[0], vd, j > tb, width / 16, 0);
-            if (!(ok = mbar_wait(bar(kPHi + 0), t & 1, abort_flag, args.status, kDevTimeoutPFull,
+            if (!(ok = mbar_wait(bar(L::kPHi + 0), tA, abort_flag, args.status, kDevTimeoutPFull,
                                  wait_limit)))
               break;
             tc_fence_after();
+            tA ^= 1u;
             issue_pv_part<kBf16>(t_o[0], t_s[0], vd, j > tb, width / 16, 1);
-            if (j == te - 1) tc_commit(bar(kOFinal + 0));
+            if (last) tc_commit(bar(L::kOFinal + 0));
             if (nx == 2) {
               have_prev = true;
               prev_v = sv;
               prev_acc = j > tb;
               prev_nk = width / 16;
-              prev_last = j == te - 1;
-              ++tB;
+              prev_last = last;
+              tB ^= 1u;
             } else {
-              tc_commit(bar(kSlotEmpty + sv));
+              tc_commit(bar(L::kSlotEmpty + sv));
             }
           }
         }
         if (ok && have_prev) ok = issue_prev();
-        tc_commit(bar(kDrain));
-        if (!mbar_drain(bar(kDrain), 0, *wait_limit)) atomicCAS(args.status, 0, kDevTimeoutDrain);
+        tc_commit(bar(L::kDrain));
+        if (!mbar_drain(bar(L::kDrain), 0, *wait_limit))
+          atomicCAS(args.status, 0, kDevTimeoutDrain);
       }
-    } else {
-      // -------------------------------------------------- preparing warps
-      const int w = warp - 2;
-      int c = 0;
-      bool ok = true;
-      uint32_t raw_uses = 0;
-      RawTile raw;
-      // a warp-wide wait: every lane leaves it with the same answer
-      auto wait = [&](uint32_t b, uint32_t parity, int code) -> bool {
-        const bool got = mbar_wait(b, parity, abort_flag, args.status, code, wait_limit);
-        return __all_sync(0xffffffffu, got);
-      };
-      auto publish = [&](int s, bool bad, int li) {
-        if (__any_sync(0xffffffffu, bad) && lane == 0) bad_item[li & 3] = li + 1;
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(kSlotFull + s));
-      };
-      for (int it = share.beg, li = 0; ok && it < share.end; ++it, ++li) {
-        const PrefixItem item = args.items[it];
-        int tb, te;
-        share_tiles<kSplit>(share, item, tb, te);
-        // codes of the item's next 8-bit tile are fetched one tile ahead
-        auto fetch = [&](int j, int kv) {
-          const PrefixTile tile = args.tiles[j];
-          const int rows = min(tile.info & kTileWidthMask, args.prefix_len - tile.key);
-          load_raw(raw, static_cast<const uint8_t*>(kv ? args.v_prefix : args.k_prefix),
-                   kv ? args.v_scale : args.k_scale, args.kv_heads, item.head, tile.key, rows, w,
-                   lane);
-        };
-        if (kFormat != kKvPlain && tb < te && !(args.tiles[tb].info & kTileOwn)) fetch(tb, 0);
-        for (int j = tb; ok && j < te; ++j) {
-          const PrefixTile tile = args.tiles[j];
-          const bool own = tile.info & kTileOwn;
-          const bool guard = tile.info & kTileGuard;
-          for (int kv = 0; kv < 2; ++kv, ++c) {
-            const int s = c % kSlots;
-            const uint32_t slot = sbase + kSlotOff + s * kTileBytes;
-            if (kFormat != kKvPlain &&
-                !(ok = wait(bar(kSlotEmpty + s), ((c / kSlots) & 1) ^ 1, kDevTimeoutSlotEmpty)))
-              break;
-            if (kFormat != kKvPlain && !own) {
-              const bool bad =
-                  store_raw<kBf16, kFormat>(raw, slot, kv == 1 && guard, w, lane);
-              publish(s, bad, li);
-              if (kv == 0) fetch(j, 1);
-              else if (j + 1 < te && !(args.tiles[j + 1].info & kTileOwn)) fetch(j + 1, 0);
-            } else if (kv == 1 && guard) {
-              if (!(ok = wait(bar(kRawFull + s), (raw_uses >> s) & 1u, kDevTimeoutSlotFull)))
-                break;
-              raw_uses ^= 1u << s;
-              publish(s, guard_tile<kBf16>(slot, tile.info & kTileWidthMask, w, lane), li);
-            }
-          }
-        }
-      }
+    } else if (!L::kConverts) {
+      prepare_tiles<kBf16, kFormat, kSplit>(args, share, sbase, warp - L::kPrepWarp0, lane,
+                                            abort_flag, wait_limit, bad_item);
     }
+  } else if (L::kConverts && warp >= L::kPrepWarp0) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::kRegsPrep));
+    prepare_tiles<kBf16, kFormat, kSplit>(args, share, sbase, warp - L::kPrepWarp0, lane,
+                                          abort_flag, wait_limit, bad_item);
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(L::kRegsSoftmax));
     // ----------------------------------------------------------- softmax
     const int x = (warp - kSoftmaxWarp0) >> 2;
     const int sub = warp & 3;
@@ -682,23 +749,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       const PrefixItem item = args.items[it];
       int tb, te;
       share_tiles<kSplit>(share, item, tb, te);
-      const int qb = li & 1;
-      if (x == 1 && item.tokens <= args.tile_tokens) {
-        // no tile B: release the Q buffer once it is this item's
-        if (!(ok = mbar_wait(bar(kQFull + qb), (li >> 1) & 1, abort_flag, args.status,
-                             kDevTimeoutQ, wait_limit)))
-          break;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(kQEmpty + qb));
-        continue;
-      }
+      if (x == 1 && item.tokens <= args.tile_tokens) continue;  // no tile B
       const bool valid = row < tile_rows && x * args.tile_tokens + token < item.tokens;
       PrefixRow mine = {0, -1};
       if (valid) mine = args.rows[item.row0 + x * args.tile_tokens + token];
       float m_run = -INFINITY, l_run = 0.f;
+      PrefixTile next = args.tiles[tb];
       for (int j = tb; j < te; ++j, ++t) {
-        const PrefixTile tile = args.tiles[j];
-        if (!(ok = mbar_wait(bar(kSFull + x), t & 1, abort_flag, args.status, kDevTimeoutSFull,
+        const PrefixTile tile = next;
+        next = args.tiles[j + 1 < te ? j + 1 : j];
+        if (!(ok = mbar_wait(bar(L::kSFull + x), t & 1, abort_flag, args.status, kDevTimeoutSFull,
                              wait_limit)))
           break;
         tc_fence_after();
@@ -766,7 +826,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(bar(kPLo + x));
+        mbar_arrive(bar(L::kPLo + x));
         if (!narrow) {
           sum += exp_pack<kBf16>(a2, scale, m_use) + exp_pack<kBf16>(a3, scale, m_use);
           tmem_st16(t_s + 32, a2);
@@ -775,19 +835,20 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc_fence_before();
         }
         l_run += sum;
-        mbar_arrive(bar(kPHi + x));
+        mbar_arrive(bar(L::kPHi + x));
       }
-      // Epilogue: every MMA that reads this tile's Q rows has completed, so
-      // their buffer serves as staging.
-      if (!ok || !(ok = mbar_wait(bar(kOFinal + x), lx & 1, abort_flag, args.status,
+      // Epilogue.
+      if (!ok || !(ok = mbar_wait(bar(L::kOFinal + x), lx & 1, abort_flag, args.status,
                                   kDevTimeoutOFinal, wait_limit)))
         break;
       ++lx;
       tc_fence_after();
-      const bool aside = valid && bad_item[li & 3] == li + 1;
+      const bool aside = valid && *bad_item > li;
       if constexpr (kSplit) {
-        // f32 rows of 512 bytes, their 16-byte units swizzled by the row
-        const uint32_t dst = sbase + x * kQBufBytes + row * 512;
+        // f32 rows of 512 bytes, their 16-byte units swizzled by the row. Tile A's
+        // Q rows and tile B's are read no more, nor are, at the end of tile B,
+        // any slots.
+        const uint32_t dst = sbase + x * L::kPartOffB + row * 512;
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           uint32_t o[32];
@@ -805,11 +866,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             st_shared_v4(dst + (static_cast<uint32_t>(c * 8 + v) ^ lane) * 16, o[4 * v],
                          o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
         }
-        *reinterpret_cast<float2*>(smem + kStatOff + (x * 128 + row) * 8) =
+        *reinterpret_cast<float2*>(smem + L::kEpiOff + (x * 128 + row) * 8) =
             make_float2(m_run, l_run);
       } else {
+        // 32 dims at a time: the warp's 32 rows of 64 bytes through its 2 KB,
+        // out as 64-byte runs, eight rows an instruction
         const float inv_l = 1.f / l_run;
-        const uint32_t stage = sbase + qb * kQBufBytes + x * kTileBytes;
+        const uint32_t stage = sbase + L::kEpiOff + (warp - kSoftmaxWarp0) * 2048;
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           uint32_t o[32];
@@ -822,6 +885,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int i = 0; i < 32; ++i)
               o[i] = __float_as_uint(with_aside(__uint_as_float(o[i]), s, i));
           }
+          __syncwarp();  // the chunk before has been read
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
             const uint32_t* p = o + 8 * v;
@@ -830,28 +894,27 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int i = 0; i < 4; ++i)
               y[i] = pack2<kBf16>(__uint_as_float(p[2 * i]) * inv_l,
                                   __uint_as_float(p[2 * i + 1]) * inv_l);
-            st_shared_v4(stage + row * 256 + ((c * 4 + v) ^ (lane & 15)) * 16, y[0], y[1], y[2],
-                         y[3]);
+            // a row's unit v at v ^ (row / 2) % 4: two rows share 128 bytes of banks
+            st_shared_v4(stage + lane * 64 + (v ^ ((lane >> 1) & 3)) * 16, y[0], y[1], y[2], y[3]);
+          }
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int rw = 8 * i + (lane >> 2), r = sub * 32 + rw;
+            const int rt = r / args.group, rh = r - rt * args.group;
+            const int tok = x * args.tile_tokens + rt;
+            const uint4 v =
+                ld_shared_v4(stage + rw * 64 + ((lane & 3) ^ ((rw >> 1) & 3)) * 16);
+            if (r < tile_rows && tok < item.tokens)
+              *reinterpret_cast<uint4*>(args.out +
+                                        (static_cast<int64_t>(item.row0 + tok) * args.q_heads +
+                                         item.head * args.group + rh) *
+                                            kHeadDim +
+                                        c * 32 + (lane & 3) * 8) = v;
           }
         }
         tc_fence_before();
         __syncwarp();
-        // the warp's rows leave two at a time, 256 bytes each
-        for (int i = 0; i < 16; ++i) {
-          const int r = sub * 32 + 2 * i + (lane >> 4);
-          const int rt = r / args.group, rh = r - rt * args.group;
-          const int tok = x * args.tile_tokens + rt;
-          const uint4 v = ld_shared_v4(stage + r * 256 + ((lane & 15) ^ (r & 15)) * 16);
-          if (r < tile_rows && tok < item.tokens)
-            *reinterpret_cast<uint4*>(args.out +
-                                      (static_cast<int64_t>(item.row0 + tok) * args.q_heads +
-                                       item.head * args.group + rh) *
-                                          kHeadDim +
-                                      (lane & 15) * 8) = v;
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(kQEmpty + qb));
       }
     }
   }
@@ -862,7 +925,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // the cluster's O, m and l are in shared memory: each CTA merges its share
     // of the rows, a warp a row
     cluster_sync();
-    if (warp >= kSoftmaxWarp0) {
+    if (warp >= kSoftmaxWarp0 && warp < kSoftmaxWarp0 + 8) {
       const PrefixItem item = args.items[share.beg];
       const int rows = item.tokens > args.tile_tokens ? 256 : 128;
       const int per = (rows + share.ranks - 1) / share.ranks;
@@ -874,7 +937,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (r >= rows || rr >= tile_rows || tok >= item.tokens) continue;
         float2 ml = make_float2(-INFINITY, 0.f);
         if (lane < share.ranks)
-          ml = ld_cluster_v2(mapa_shared(sbase + kStatOff + r * 8, lane));
+          ml = ld_cluster_v2(mapa_shared(sbase + L::kEpiOff + r * 8, lane));
         float m = ml.x;
 #pragma unroll
         for (int o = 4; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -886,7 +949,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         l = __shfl_sync(0xffffffffu, l, 0);
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
         const uint32_t at =
-            sbase + x * kQBufBytes + rr * 512 + (static_cast<uint32_t>(lane) ^ (rr & 31)) * 16;
+            sbase + x * L::kPartOffB + rr * 512 + (static_cast<uint32_t>(lane) ^ (rr & 31)) * 16;
         for (int k = 0; k < share.ranks; ++k) {
           const float wk = __shfl_sync(0xffffffffu, w, k);
           const float4 v = ld_cluster_v4(mapa_shared(at, k));
@@ -928,14 +991,15 @@ cudaError_t launch(const PrefixMaps& m, const PrefixArgs& args, int grid, int sp
   if (e != cudaSuccess) return e;
   if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
   if (!configured[dev]) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             Layout<kFormat>::kSmemBytes);
     if (e != cudaSuccess) return e;
     configured[dev] = true;
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = kSmemBytes;
+  cfg.blockDim = dim3(Layout<kFormat>::kThreads);
+  cfg.dynamicSmemBytes = Layout<kFormat>::kSmemBytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;

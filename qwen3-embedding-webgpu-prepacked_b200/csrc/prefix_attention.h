@@ -10,7 +10,7 @@
 namespace qwa {
 
 struct PrefixMaps {
-  CUtensorMap q, k, v, pk, pv;  // pk / pv: of a 16-bit prefix only
+  CUtensorMap q, k, v, pk, pv;  // pk / pv: the prefix, 16-bit values or 8-bit codes
 };
 
 struct PrefixArgs {

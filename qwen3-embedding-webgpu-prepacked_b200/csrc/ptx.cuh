@@ -29,7 +29,6 @@ enum DeviceError : int {
   kDevTimeoutAccFull = 0x204,
   kDevTimeoutPairSync = 0x205,
   kDevTimeoutSmallGemm = 0x301,
-  kDevSharedLayout = 0x401,  // shared memory less aligned than the kernel allows for
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) {
