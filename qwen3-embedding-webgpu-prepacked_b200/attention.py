@@ -54,6 +54,9 @@ class Context:
         if device is None:
             device = torch.cuda.current_device()
         device = torch.device("cuda", device).index if not isinstance(device, int) else device
+        ctx = cls._by_device.get(device)  # made once, never replaced
+        if ctx is not None:
+            return ctx
         with cls._lock:
             ctx = cls._by_device.get(device)
             if ctx is None:
@@ -82,6 +85,12 @@ def _stream(stream, device=None) -> int:
     return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
 
 
+def _raw_stream(device: int) -> int:
+    """cudaStream_t of the device's current stream (without a Stream object: this
+    is on the path of calls of a few microseconds)."""
+    return torch._C._cuda_getCurrentRawStream(device)
+
+
 def _need(cond: bool, msg: str) -> None:
     if not cond:
         raise ValueError(msg)
@@ -96,6 +105,15 @@ def _f16_cuda(t: torch.Tensor, name: str) -> None:
 def _f32_weight(t: torch.Tensor, name: str) -> None:
     _need(t.is_cuda and t.dtype == torch.float32 and t.numel() == HEAD_DIM and t.is_contiguous(),
           f"{name} must be a contiguous CUDA float32 tensor of 128 elements")
+
+
+def _launch(ctx: "Context", stream, fn, *args) -> None:
+    """Issue a C ABI call on ``stream`` (None: the current stream of the context's
+    device), without a bound run in between."""
+    status = fn(ctx.handle, *args, _raw_stream(ctx.device) if stream is None
+                else _stream(stream))
+    if status:
+        _lib.check(status, ctx.handle)
 
 
 @dataclass

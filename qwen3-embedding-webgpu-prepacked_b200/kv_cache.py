@@ -21,11 +21,12 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .attention import HEAD_DIM, KV_HEADS, Context, EncodableRun, _need, _ptr, encode_run
+from .attention import HEAD_DIM, KV_HEADS, Context, EncodableRun, _launch, _need
 
 _DTYPES = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
 FORMATS = {"none": _lib.KV_PLAIN, "e4m3": _lib.KV_E4M3, "int8": _lib.KV_INT8}
 _CODES = {"e4m3": torch.float8_e4m3fn, "int8": torch.int8}
+_FORMAT_OF = {code: name for name, code in _CODES.items()}
 
 
 class KVCache:
@@ -61,45 +62,71 @@ class KVCache:
 
     def _set(self, k, v, k_scale, v_scale, dtype) -> None:
         _need(dtype in _DTYPES, "dtype must be float16 or bfloat16")
-        fmt = {torch.float8_e4m3fn: "e4m3", torch.int8: "int8", dtype: "none"}.get(k.dtype)
+        fmt = _FORMAT_OF.get(k.dtype)
+        if fmt is None and k.dtype == dtype:
+            fmt = "none"
         _need(fmt is not None, "k must hold float8_e4m3fn, int8 or values of dtype")
-        _need(k.is_cuda and k.dim() == 3 and k.is_contiguous() and v.is_contiguous()
-              and v.shape == k.shape and v.dtype == k.dtype and v.device == k.device,
+        index, shape = k.get_device(), k.shape
+        _need(index >= 0 and len(shape) == 3 and k.is_contiguous() and v.is_contiguous()
+              and v.shape == shape and v.dtype == k.dtype and v.get_device() == index,
               "k and v must be contiguous CUDA tensors [slots, heads, head_dim] of one kind")
+        ks = vs = None
         if fmt == "none":
             _need(k_scale is None and v_scale is None, "16-bit values have no scales")
         else:
+            held = (shape[0], shape[1])
             for s in (k_scale, v_scale):
-                _need(s is not None and s.dtype == torch.uint8 and s.is_contiguous()
-                      and s.device == k.device and s.shape == k.shape[:2],
+                _need(s is not None and s.dtype == torch.uint8 and s.shape == held
+                      and s.get_device() == index and s.is_contiguous(),
                       "scales must be contiguous uint8 tensors [slots, heads]")
+            ks, vs = k_scale.data_ptr(), v_scale.data_ptr()
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.format, self.dtype = fmt, dtype
-        self.slots, self.heads, self.head_dim = k.shape
-        self.device = k.device
+        self.format, self.dtype, self.device = fmt, dtype, k.device
+        self.slots, self.heads, self.head_dim = shape
         self.struct = _lib.KvCacheStruct(_DTYPES[dtype], FORMATS[fmt], self.heads, self.head_dim,
-                                         self.slots, k.data_ptr(), v.data_ptr(),
-                                         k_scale.data_ptr() if k_scale is not None else None,
-                                         v_scale.data_ptr() if v_scale is not None else None)
+                                         self.slots, k.data_ptr(), v.data_ptr(), ks, vs)
 
     def nbytes(self) -> int:
         held = (self.k, self.v, self.k_scale, self.v_scale)
         return sum(t.numel() * t.element_size() for t in held if t is not None)
 
 
-def _slots(slots: torch.Tensor, device) -> int:
-    _need(isinstance(slots, torch.Tensor) and slots.device == device
-          and slots.dtype == torch.int32 and slots.is_contiguous(),
+def _slots(slots: torch.Tensor, index: int) -> int:
+    _need(slots.get_device() == index and slots.dtype == torch.int32 and slots.is_contiguous(),
           "slots must be a contiguous int32 tensor on the cache's device")
     return slots.numel()
 
 
-def _rows(t: torch.Tensor, name: str, cache: KVCache, tokens: int) -> None:
-    _need(isinstance(t, torch.Tensor) and t.dtype == cache.dtype and t.device == cache.device
-          and tuple(t.shape) == (tokens, cache.heads, cache.head_dim)
-          and t.stride(2) == 1 and (t.stride(1) == cache.head_dim or cache.heads == 1),
-          f"{name} must be [tokens, heads, head_dim] of the cache's dtype and device, "
-          "a token's heads contiguous")
+def _rows(t: torch.Tensor, name: str, cache: KVCache, tokens: int, index: int) -> int:
+    """Checks rows [tokens, heads, head_dim] of the cache; their token stride."""
+    heads, dim = cache.heads, cache.head_dim
+    if t.shape != (tokens, heads, dim) or t.dtype != cache.dtype or t.get_device() != index:
+        raise ValueError(f"{name} must be [tokens, heads, head_dim] of the cache's dtype and "
+                         "device")
+    s0, s1, s2 = t.stride()
+    if s2 != 1 or (s1 != dim and heads != 1):
+        raise ValueError(f"{name}: a token's heads must be contiguous")
+    return s0 if tokens > 1 else heads * dim  # a single row has no stride of its own
+
+
+def _write_args(ctx: Context, cache: KVCache, k, v, slots) -> tuple:
+    index = ctx.device
+    _need(cache.device.index == index, "the cache must be on the kernel's device")
+    n = _slots(slots, index)
+    return (ctypes.byref(cache.struct), k.data_ptr(), _rows(k, "k", cache, n, index),
+            v.data_ptr(), _rows(v, "v", cache, n, index), slots.data_ptr(), n)
+
+
+def _read_args(ctx: Context, cache: KVCache, slots, k_output, v_output) -> tuple:
+    index = ctx.device
+    _need(cache.device.index == index, "the cache must be on the kernel's device")
+    n = _slots(slots, index)
+    width = cache.heads * cache.head_dim
+    _need(_rows(k_output, "k_output", cache, n, index) == width
+          and _rows(v_output, "v_output", cache, n, index) == width,
+          "k_output and v_output must be contiguous")
+    return (ctypes.byref(cache.struct), slots.data_ptr(), n, k_output.data_ptr(),
+            v_output.data_ptr())
 
 
 class KVCacheKernel:
@@ -112,15 +139,8 @@ class KVCacheKernel:
                          slots: torch.Tensor) -> EncodableRun:
         """Row t of k and v goes into slot ``slots[t]``, which must differ within
         a call; a slot outside the cache skips its row."""
-        n = _slots(slots, cache.device)
-        _rows(k, "k", cache, n)
-        _rows(v, "v", cache, n)
-        _need(cache.device.index == self.ctx.device, "the cache must be on the kernel's device")
+        args = _write_args(self.ctx, cache, k, v, slots)
         lib, h = self.ctx.lib, self.ctx.handle
-        width = cache.heads * cache.head_dim
-        # a single row has no stride of its own
-        args = (ctypes.byref(cache.struct), _ptr(k), k.stride(0) if n > 1 else width, _ptr(v),
-                v.stride(0) if n > 1 else width, _ptr(slots), n)
         return EncodableRun(lambda s: lib.qwa_kv_cache_write(h, *args, s), self.ctx,
                             "KV cache write")
 
@@ -128,13 +148,8 @@ class KVCacheKernel:
                         v_output: torch.Tensor) -> EncodableRun:
         """k_output, v_output [tokens, heads, head_dim]; a slot outside the cache
         gives zeros."""
-        n = _slots(slots, cache.device)
-        for t, name in ((k_output, "k_output"), (v_output, "v_output")):
-            _rows(t, name, cache, n)
-            _need(t.is_contiguous(), f"{name} must be contiguous")
-        _need(cache.device.index == self.ctx.device, "the cache must be on the kernel's device")
+        args = _read_args(self.ctx, cache, slots, k_output, v_output)
         lib, h = self.ctx.lib, self.ctx.handle
-        args = (ctypes.byref(cache.struct), _ptr(slots), n, _ptr(k_output), _ptr(v_output))
         return EncodableRun(lambda s: lib.qwa_kv_cache_read(h, *args, s), self.ctx,
                             "KV cache read")
 
@@ -142,19 +157,21 @@ class KVCacheKernel:
 def kv_cache_write(cache: KVCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor,
                    stream=None) -> None:
     """Quantise rows k, v [tokens, heads, head_dim] into the cache's ``slots``
-    (int32 [tokens])."""
-    encode_run(stream, KVCacheKernel(cache.device.index).create_write_run(cache, k, v, slots))
+    (int32 [tokens], all different)."""
+    ctx = Context.for_device(cache.device.index)
+    _launch(ctx, stream, ctx.lib.qwa_kv_cache_write, *_write_args(ctx, cache, k, v, slots))
 
 
 def kv_cache_read(cache: KVCache, slots: torch.Tensor, k_out: Optional[torch.Tensor] = None,
                   v_out: Optional[torch.Tensor] = None, stream=None
                   ) -> Tuple[torch.Tensor, torch.Tensor]:
     """(k, v) [tokens, heads, head_dim] of ``slots`` in the cache's dtype."""
-    shape = (slots.numel(), cache.heads, cache.head_dim)
-    if k_out is None:
-        k_out = torch.empty(shape, dtype=cache.dtype, device=cache.device)
-    if v_out is None:
-        v_out = torch.empty(shape, dtype=cache.dtype, device=cache.device)
-    encode_run(stream, KVCacheKernel(cache.device.index).create_read_run(cache, slots, k_out,
-                                                                        v_out))
+    if k_out is None or v_out is None:
+        shape = (slots.numel(), cache.heads, cache.head_dim)
+        if k_out is None:
+            k_out = cache.k.new_empty(shape, dtype=cache.dtype)
+        if v_out is None:
+            v_out = torch.empty_like(k_out)
+    ctx = Context.for_device(cache.device.index)
+    _launch(ctx, stream, ctx.lib.qwa_kv_cache_read, *_read_args(ctx, cache, slots, k_out, v_out))
     return k_out, v_out

@@ -24,7 +24,7 @@ import torch
 
 from . import _lib
 from .attention import (HEAD_DIM, MODE_AUTO, PREFIX, WINDOW, AttentionRun, Context, EncodableRun,
-                        _need, _ptr, encode_run)
+                        _launch, _need, encode_run)
 from .kv_cache import _DTYPES, KVCache
 
 
@@ -48,9 +48,8 @@ class PrefixPlan:
         _need(len(cu_q) >= 2, "cu_seqlens needs at least one request")
         _need(cu_k is None or len(cu_k) == len(cu_q),
               "cu_seqlens and cu_seqlens_k must be of the same requests")
-        with torch.cuda.device(self.ctx.device):
-            _need(not torch.cuda.is_current_stream_capturing(),
-                  "a plan allocates memory: make it before the capture")
+        _need(not _capturing(self.ctx.device),
+              "a plan allocates memory: make it before the capture")
         while _retired:
             lib, old = _retired.pop()
             lib.qwa_prefix_plan_destroy(old)
@@ -80,16 +79,34 @@ class PrefixPlan:
             pass
 
 
-def _packed(t: torch.Tensor, name: str, tokens: int, heads: int, like: torch.Tensor) -> int:
+def _packed(t: torch.Tensor, name: str, tokens: int, heads: int, dtype, index: int) -> int:
     """Checks a packed [tokens, heads, 128] operand; its token stride."""
-    _need(isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in _DTYPES and t.dim() == 3
-          and t.dtype == like.dtype and t.device == like.device,
-          f"{name} must be a CUDA float16 or bfloat16 tensor of q's dtype and device")
-    _need(tuple(t.shape) == (tokens, heads, HEAD_DIM),
-          f"{name} must be [{tokens}, {heads}, {HEAD_DIM}], got {tuple(t.shape)}")
-    _need(t.stride(2) == 1 and (heads == 1 or t.stride(1) == HEAD_DIM),
-          f"{name}: a token's heads must be contiguous")
-    return t.stride(0) if tokens > 1 else heads * HEAD_DIM
+    if t.shape != (tokens, heads, HEAD_DIM) or t.dtype != dtype or t.get_device() != index:
+        raise ValueError(f"{name} must be [{tokens}, {heads}, {HEAD_DIM}] of q's dtype and device")
+    s0, s1, s2 = t.stride()
+    if s2 != 1 or (s1 != HEAD_DIM and heads != 1):
+        raise ValueError(f"{name}: a token's heads must be contiguous")
+    return s0 if tokens > 1 else heads * HEAD_DIM  # a single row has no stride of its own
+
+
+def _attention_args(ctx: Context, plan: PrefixPlan, q, k, v, output, cache, first_slot) -> tuple:
+    dtype, index = q.dtype, ctx.device
+    code = _DTYPES.get(dtype)
+    _need(code is not None, "q must be float16 or bfloat16")
+    _need(plan.ctx.device == index, "the plan must be on the kernel's device")
+    _need(plan.handle is not None, "the plan is closed")
+    n, hq, m, hk = plan.queries, plan.q_heads, plan.keys, plan.kv_heads
+    _need(_packed(output, "output", n, hq, dtype, index) == hq * HEAD_DIM,
+          "output must be contiguous")
+    struct = None
+    if cache is not None:
+        _need(cache.device.index == index, "the cache must be on q's device")
+        struct = ctypes.byref(cache.struct)
+    else:
+        _need(plan.prefix_len == 0, "a prefix needs its cache")
+    return (code, q.data_ptr(), _packed(q, "q", n, hq, dtype, index), k.data_ptr(),
+            _packed(k, "k", m, hk, dtype, index), v.data_ptr(),
+            _packed(v, "v", m, hk, dtype, index), output.data_ptr(), struct, first_slot)
 
 
 class PrefixAttentionKernel:
@@ -104,22 +121,8 @@ class PrefixAttentionKernel:
         """q [queries, q_heads, 128], k, v [own keys, kv_heads, 128] packed
         request after request, output as q, contiguous; the prefix is in the
         cache's slots ``first_slot`` .. ``first_slot + plan.prefix_len - 1``."""
-        q_stride = _packed(q, "q", plan.queries, plan.q_heads, q)
-        k_stride = _packed(k, "k", plan.keys, plan.kv_heads, q)
-        v_stride = _packed(v, "v", plan.keys, plan.kv_heads, q)
-        _packed(output, "output", plan.queries, plan.q_heads, q)
-        _need(output.is_contiguous(), "output must be contiguous")
-        _need(q.device.index == self.ctx.device and plan.ctx.device == self.ctx.device,
-              "q and the plan must be on the kernel's device")
-        _need(plan.handle is not None, "the plan is closed")
-        _need(cache is not None or plan.prefix_len == 0, "a prefix needs its cache")
-        struct = None
-        if cache is not None:
-            _need(cache.device == q.device, "the cache must be on q's device")
-            struct = ctypes.byref(cache.struct)
+        args = _attention_args(self.ctx, plan, q, k, v, output, cache, first_slot)
         lib, h = self.ctx.lib, self.ctx.handle
-        args = (_DTYPES[q.dtype], _ptr(q), q_stride, _ptr(k), k_stride, _ptr(v), v_stride,
-                _ptr(output), struct, first_slot)
 
         def launch(stream):
             _need(plan.handle is not None, "the plan is closed")
@@ -138,25 +141,32 @@ _captured: dict = {}  # plans that a graph was captured with are kept
 _plans_lock = threading.Lock()
 
 
-def _plan_for(ctx: Context, key: tuple) -> PrefixPlan:
-    with torch.cuda.device(ctx.device):
-        capturing = torch.cuda.is_current_stream_capturing()
+def _capturing(device: int) -> bool:
+    """Whether the device's current stream is being captured."""
+    if torch.cuda.current_device() == device:
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(device):
+        return torch.cuda.is_current_stream_capturing()
+
+
+def _plan_for(ctx: Context, *key) -> PrefixPlan:
     full = (ctx.device,) + key
     with _plans_lock:
-        plan = _captured.get(full) or _plans.get(full)
-        if plan is not None:
-            if capturing:
-                _captured[full] = plan
-            elif full in _plans:
+        plan = _captured.get(full)
+        if plan is None:
+            plan = _plans.get(full)
+            if plan is not None:
                 _plans.move_to_end(full)
-            return plan
-    cu_q, cu_k, prefix_len, q_heads, kv_heads, mode, sparse_prefix, window = key
-    plan = PrefixPlan(cu_q, prefix_len, q_heads, kv_heads, cu_k, mode, sparse_prefix, window,
-                      ctx=ctx)
-    with _plans_lock:
-        _plans[full] = plan
-        while len(_plans) > MAX_PLANS:
-            _plans.popitem(last=False)
+                if _capturing(ctx.device):
+                    _captured[full] = plan
+    if plan is None:
+        cu_q, cu_k, prefix_len, q_heads, kv_heads, mode, sparse_prefix, window = key
+        plan = PrefixPlan(cu_q, prefix_len, q_heads, kv_heads, cu_k, mode, sparse_prefix, window,
+                          ctx=ctx)
+        with _plans_lock:
+            _plans[full] = plan
+            while len(_plans) > MAX_PLANS:
+                _plans.popitem(last=False)
     return plan
 
 
@@ -172,16 +182,17 @@ def prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     k and v (None: the same); a request's queries are the last of its keys.
     Lengths met before reuse their plan; inside a capture they must have been
     met before it."""
-    _need(isinstance(q, torch.Tensor) and q.is_cuda and q.dim() == 3
-          and isinstance(k, torch.Tensor) and k.dim() == 3,
+    q_shape, k_shape = q.shape, k.shape
+    _need(q.is_cuda and len(q_shape) == 3 and len(k_shape) == 3,
           "q and k must be CUDA tensors [tokens, heads, 128]")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    kern = PrefixAttentionKernel(q.device.index)
-    plan = _plan_for(kern.ctx, (tuple(cu_seqlens),
-                                tuple(cu_seqlens_k) if cu_seqlens_k is not None else None,
-                                prefix_len, q.shape[1], k.shape[1], mode, sparse_prefix, window))
-    kern.encode(stream, kern.create_run(q, k, v, out, plan, cache, first_slot))
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    ctx = Context.for_device(q.get_device())
+    plan = _plan_for(ctx, tuple(cu_seqlens),
+                     tuple(cu_seqlens_k) if cu_seqlens_k is not None else None, prefix_len,
+                     q_shape[1], k_shape[1], mode, sparse_prefix, window)
+    args = _attention_args(ctx, plan, q, k, v, out, cache, first_slot)
+    _launch(ctx, stream, ctx.lib.qwa_prefix_attention, plan.handle, *args)
     return out
 
 

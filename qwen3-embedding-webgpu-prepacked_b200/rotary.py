@@ -19,7 +19,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .attention import ROPE_THETA, Context, EncodableRun, _need, _ptr, encode_run
+from .attention import ROPE_THETA, Context, EncodableRun, _launch, _need
 
 _DTYPES = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
 _LAYOUTS = {"half": _lib.ROPE_HALF, "interleaved": _lib.ROPE_INTERLEAVED}
@@ -66,25 +66,51 @@ def rope_table(positions: int, rotary_dim: int = 128, theta: float = ROPE_THETA,
         out = torch.empty(positions, rotary_dim // 2, 2, dtype=torch.float32,
                           device=torch.device("cuda", ctx.device))
     s = scaling.struct() if scaling is not None else None
-    lib, h = ctx.lib, ctx.handle
-    encode_run(stream, EncodableRun(
-        lambda st: lib.qwa_rope_table(h, _ptr(out), first, positions, rotary_dim, theta,
-                                      ctypes.byref(s) if s is not None else None, st),
-        ctx, "rotary table"))
+    _launch(ctx, stream, ctx.lib.qwa_rope_table, out.data_ptr(), first, positions, rotary_dim,
+            theta, ctypes.byref(s) if s is not None else None)
     return out
 
 
-def _heads(t: torch.Tensor, name: str, tokens: int, dim: int, dtype, device) -> None:
-    _need(isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in _DTYPES and t.dim() == 3,
-          f"{name} must be a CUDA float16 or bfloat16 tensor [tokens, heads, head_dim]")
-    _need(t.shape[0] == tokens and t.shape[2] == dim and t.dtype == dtype and t.device == device,
-          f"{name} must agree with the others in tokens, head_dim, dtype and device")
-    _need(t.stride(2) == 1 or dim == 1, f"{name}: a head's values must be contiguous")
+def _side(x: Optional[torch.Tensor], y: Optional[torch.Tensor], name: str, tokens: int, dim: int,
+          dtype, index: int):
+    """Checks one of q and k with its output; its qwa_rope_tensor."""
+    if x is None:
+        return None
+    if y is None:
+        raise ValueError(f"{name} needs an output")
+    shape = x.shape
+    if len(shape) != 3 or shape[0] != tokens or shape[2] != dim or y.shape != shape:
+        raise ValueError(f"{name} and its output must be [tokens, heads, head_dim] of one shape")
+    if x.dtype != dtype or y.dtype != dtype or x.get_device() != index or y.get_device() != index:
+        raise ValueError(f"{name} and its output must agree with the others in dtype and device")
+    x0, x1, x2 = x.stride()
+    y0, y1, y2 = y.stride()
+    if x2 != 1 or y2 != 1:
+        raise ValueError(f"{name}: a head's values must be contiguous")
+    return _lib.RopeTensor(x.data_ptr(), x0, x1, y.data_ptr(), y0, y1, shape[1])
 
 
-def _side(x: torch.Tensor, y: torch.Tensor) -> "_lib.RopeTensor":
-    return _lib.RopeTensor(x.data_ptr(), x.stride(0), x.stride(1), y.data_ptr(), y.stride(0),
-                           y.stride(1), x.shape[1])
+def _rope_args(ctx: Context, q, k, table, positions, q_output, k_output, layout, inverse) -> tuple:
+    some = q if q is not None else k
+    dtype, index, shape = some.dtype, ctx.device, some.shape
+    code = _DTYPES.get(dtype)
+    _need(code is not None and len(shape) == 3,
+          "q or k must be a CUDA float16 or bfloat16 tensor [tokens, heads, head_dim]")
+    _need(layout in _LAYOUTS, "layout must be 'half' or 'interleaved'")
+    tokens, _, dim = shape
+    qs = _side(q, q_output, "q", tokens, dim, dtype, index)
+    ks = _side(k, k_output, "k", tokens, dim, dtype, index)
+    rows = table.shape
+    _need(table.dtype == torch.float32 and table.get_device() == index and len(rows) == 3
+          and rows[2] == 2 and table.is_contiguous(),
+          "table must be a contiguous float32 [rows, rotary_dim / 2, 2] on q's device")
+    _need(positions.dtype == torch.int32 and positions.get_device() == index
+          and positions.is_contiguous() and positions.numel() >= tokens,
+          "positions must be a contiguous int32 tensor of one position a token")
+    return (code, ctypes.byref(qs) if qs is not None else None,
+            ctypes.byref(ks) if ks is not None else None, tokens, dim, 2 * rows[1],
+            _LAYOUTS[layout], 1 if inverse else 0, positions.data_ptr(), table.data_ptr(),
+            rows[0])
 
 
 class RopeKernel:
@@ -100,33 +126,9 @@ class RopeKernel:
         """q, k: [tokens, heads, head_dim], any strides with contiguous heads;
         either may be None. An output may be its input (in place). A token
         whose position is not a row of the table is left unwritten."""
-        some = q if q is not None else k
-        _need(some is not None, "one of q and k is required")
-        _need(layout in _LAYOUTS, "layout must be 'half' or 'interleaved'")
-        _need(isinstance(some, torch.Tensor) and some.dim() == 3,
-              "q and k must be tensors [tokens, heads, head_dim]")
-        tokens, _, dim = some.shape
-        for x, y, name in ((q, q_output, "q"), (k, k_output, "k")):
-            if x is None:
-                continue
-            _heads(x, name, tokens, dim, some.dtype, some.device)
-            _need(y is not None, f"{name} needs an output")
-            _heads(y, name + "_output", tokens, dim, some.dtype, some.device)
-            _need(y.shape[1] == x.shape[1], f"{name}_output must have {name}'s heads")
-        _need(some.device.index == self.ctx.device, "q and k must be on the kernel's device")
-        _need(table.device == some.device and table.dtype == torch.float32 and table.dim() == 3
-              and table.shape[2] == 2 and table.is_contiguous(),
-              "table must be a contiguous float32 [rows, rotary_dim / 2, 2] on q's device")
-        _need(positions.device == some.device and positions.dtype == torch.int32
-              and positions.is_contiguous() and positions.numel() >= tokens,
-              "positions must be a contiguous int32 tensor of one position a token")
+        _need(q is not None or k is not None, "one of q and k is required")
+        args = _rope_args(self.ctx, q, k, table, positions, q_output, k_output, layout, inverse)
         lib, h = self.ctx.lib, self.ctx.handle
-        qs = _side(q, q_output) if q is not None else None
-        ks = _side(k, k_output) if k is not None else None
-        args = (_DTYPES[some.dtype], ctypes.byref(qs) if qs is not None else None,
-                ctypes.byref(ks) if ks is not None else None, tokens, dim, 2 * table.shape[1],
-                _LAYOUTS[layout], 1 if inverse else 0, _ptr(positions), _ptr(table),
-                table.shape[0])
         return EncodableRun(lambda s: lib.qwa_rope(h, *args, s), self.ctx, "rotary positions")
 
 
@@ -135,13 +137,13 @@ def rope(q: Optional[torch.Tensor], k: Optional[torch.Tensor], table: torch.Tens
          q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None, stream=None
          ) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
     """(q, k) rotated at each token's position (the way back with ``inverse``)."""
-    if q is not None and q_out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    if k is not None and k_out is None:
-        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
     some = q if q is not None else k
     _need(some is not None and some.is_cuda, "q or k must be a CUDA tensor")
-    run = RopeKernel(some.device.index).create_run(q, k, table, positions, q_out, k_out, layout,
-                                                   inverse)
-    encode_run(stream, run)
+    if q is not None and q_out is None:
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if k is not None and k_out is None:
+        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+    ctx = Context.for_device(some.get_device())
+    _launch(ctx, stream, ctx.lib.qwa_rope,
+            *_rope_args(ctx, q, k, table, positions, q_out, k_out, layout, inverse))
     return q_out, k_out
