@@ -1199,8 +1199,8 @@ qwa_status cache_args(qwa_ctx* ctx, const qwa_kv_cache* c, const int32_t* slots_
   if (tokens < 0) return fail(ctx, QWA_ERR_INVALID_ARG, "tokens must be >= 0");
   if (tokens > 0 && (!slots_device || (reinterpret_cast<uintptr_t>(slots_device) & 3u)))
     return fail(ctx, QWA_ERR_INVALID_ARG, "slots must be a 4-byte aligned pointer");
-  if (static_cast<int64_t>(tokens) * c->heads > (1ll << 31))
-    return fail(ctx, QWA_ERR_INVALID_ARG, "tokens * heads must be at most 2^31");
+  if (static_cast<int64_t>(tokens) * c->heads > (1ll << 30))
+    return fail(ctx, QWA_ERR_INVALID_ARG, "tokens * heads must be at most 2^30");
   *a = KvCacheArgs{};
   a->k = c->k;
   a->v = c->v;
@@ -1210,6 +1210,7 @@ qwa_status cache_args(qwa_ctx* ctx, const qwa_kv_cache* c, const int32_t* slots_
   a->heads = c->heads;
   a->head_dim = c->head_dim;
   a->tokens = tokens;
+  a->vectors = 2u * static_cast<uint32_t>(tokens) * static_cast<uint32_t>(c->heads);
   a->slot_of = slots_device;
   return QWA_OK;
 }

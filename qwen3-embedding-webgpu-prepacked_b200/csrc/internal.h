@@ -251,7 +251,10 @@ struct RopeArgs {
   const int32_t* positions;
   const float2* table;  // [table_rows, rotary / 2]
   int table_rows, tokens, head_dim, rotary, layout, inverse;
-  int smem_heads;  // heads a block stages at a time
+  int smem_heads;  // any rows: heads that a block stages at a time
+  // rows of whole 16-byte units: units of a head, heads between those of one
+  // thread, threads of a token, tokens of a block
+  int units, head_step, token_threads, block_tokens;
   __device__ __forceinline__ const uint16_t* in_row(int64_t t, int h) const {
     return h < q.heads ? q.in + t * q.in_stride + h * q.in_head_stride
                        : k.in + t * k.in_stride + (h - q.heads) * k.in_head_stride;
@@ -270,6 +273,7 @@ struct KvCacheArgs {
   uint8_t *k_scale, *v_scale;  // [slots, heads] exponent + 127
   int64_t slots;
   int heads, head_dim, tokens;
+  uint32_t vectors;        // 2 * tokens * heads
   const int32_t* slot_of;  // [tokens]
   const void *k_in, *v_in;
   int64_t k_stride, v_stride;  // elements a token

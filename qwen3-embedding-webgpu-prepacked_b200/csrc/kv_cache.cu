@@ -34,159 +34,240 @@ struct Code {
   static constexpr int kShift = kFormat == kKvE4M3 ? 8 : 6;
   static constexpr uint32_t kMantissa = kFormat == kKvE4M3 ? 0x600000u : 0x7e0000u;
 
-  // e of a vector whose largest magnitude is amax (an f32 that is a value of
-  // the 16-bit type).
-  static __device__ __forceinline__ int exponent(float amax) {
-    if (amax == 0.f) return 0;
-    int x;
-    uint32_t m;
-    const uint32_t u = __float_as_uint(amax);
-    if (u < 0x00800000u) {  // a subnormal bf16
-      x = -126;
-      m = 0;
-    } else {
-      x = static_cast<int>(u >> 23) - 127;
-      m = u & 0x7fffffu;
-    }
-    const int e = x - kShift + (m > kMantissa ? 1 : 0);
+  // e of a vector whose largest magnitude is `bits` (of the 16-bit type,
+  // finite).
+  static __device__ __forceinline__ int exponent(uint32_t bits) {
+    const uint32_t u = kBf16 ? bits << 16
+                             : __float_as_uint(__half2float(__ushort_as_half(
+                                   static_cast<unsigned short>(bits))));
+    if (u == 0) return 0;
+    if (u < 0x00800000u) return kLow;  // a subnormal bf16
+    const int e = static_cast<int>(u >> 23) - 127 - kShift + ((u & 0x7fffffu) > kMantissa ? 1 : 0);
     return e < kLow ? kLow : e;
   }
 };
 
-// Eight values of one lane, and their largest magnitude: infinities count as
-// the largest finite value and NaN as nothing.
-template <bool kBf16>
-__device__ __forceinline__ float largest_of(const uint4& raw, float (&x)[8]) {
-  constexpr float kFinite = kBf16 ? 3.3895313892515355e38f : 65504.f;
-  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-  float top = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = unpack2<kBf16>(w[i]);
-    x[2 * i] = f.x;
-    x[2 * i + 1] = f.y;
-    top = fmaxf(top, fabsf(f.x));  // max(a, NaN) = a
-    top = fmaxf(top, fabsf(f.y));
-  }
-  return fminf(top, kFinite);
+__host__ __device__ constexpr uint32_t kExpBits(bool bf16) { return bf16 ? 0x7f80u : 0x7c00u; }
+
+// Largest magnitude of eight values, as the bits of |x| in both halves: they
+// order as the values do, NaN above infinity.
+__device__ __forceinline__ uint32_t largest8(const uint4& v) {
+  constexpr uint32_t kAbs = 0x7fff7fffu;
+  return __vmaxu2(__vmaxu2(v.x & kAbs, v.y & kAbs), __vmaxu2(v.z & kAbs, v.w & kAbs));
 }
 
-// Codes of eight values, low byte first.
+// The same with NaN left out (one value at a time; NaN is rare).
+template <bool kBf16>
+__device__ __noinline__ uint32_t largest8_but_nan(uint4 v) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  uint32_t top = 0;
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t x = (w[i >> 1] >> (16 * (i & 1))) & 0x7fffu;
+    if (x <= kExpBits(kBf16) && x > top) top = x;
+  }
+  return top | (top << 16);
+}
+
+// Codes of eight values by the rule, one value at a time: for vectors with NaN,
+// at the top of the range, or too small for the short way below.
 template <bool kBf16, int kFormat>
-__device__ __forceinline__ uint2 encode8(const float (&x)[8], int e) {
+__device__ __noinline__ uint2 encode8_any(uint4 v, int e) {
   using C = Code<kBf16, kFormat>;
-  const float inv_a = pow2f(-(e / 2)), inv_b = pow2f(-(e - e / 2));  // 2^-e may leave f32's range
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
   const float most = e == C::kTop ? C::kMaxAtTop : C::kMax;
   uint32_t out[2] = {0u, 0u};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float r[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const float v = x[2 * i + j] * inv_a * inv_b;
-      // a comparison, not fminf: NaN has to stay NaN
-      r[j] = v > most ? most : (v < -most ? -most : v);
-    }
-    uint32_t pair;
-    if constexpr (kFormat == kKvE4M3) {
-      pair = float2_to_e4m3x2(r[0], r[1]);
-    } else {
-      const int a = r[0] == r[0] ? __float2int_rn(r[0]) : 0;  // NaN: 0
-      const int b = r[1] == r[1] ? __float2int_rn(r[1]) : 0;
-      pair = (static_cast<uint32_t>(a) & 0xffu) | ((static_cast<uint32_t>(b) & 0xffu) << 8);
-    }
-    out[i >> 1] |= pair << (16 * (i & 1));
+  for (int i = 0; i < 8; ++i) {
+    const float2 pair = unpack2<kBf16>(w[i >> 1]);
+    float x = ((i & 1) ? pair.y : pair.x) * pow2f(-e);
+    // comparisons, not fminf: NaN has to stay NaN
+    x = x > most ? most : (x < -most ? -most : x);
+    uint32_t code;
+    if constexpr (kFormat == kKvE4M3) code = float2_to_e4m3x2(x, 0.f) & 0xffu;
+    else code = static_cast<uint32_t>(x == x ? __float2int_rn(x) : 0) & 0xffu;
+    out[i >> 2] |= code << (8 * (i & 3));
   }
   return make_uint2(out[0], out[1]);
 }
 
+// Four codes of two pairs. The products with 2^-e are exact; E4M3 rounds in the
+// conversion, INT8 in the sum with 1.5 * 2^m (m: mantissa bits), whose low byte is
+// then the code.
 template <bool kBf16, int kFormat>
-__device__ __forceinline__ uint4 decode8(uint2 codes, int e) {
-  const float sa = pow2f(e / 2), sb = pow2f(e - e / 2);
-  const uint32_t w[2] = {codes.x, codes.y};
-  uint32_t out[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t pair = w[i >> 1] >> (16 * (i & 1));
-    float2 f;
+__device__ __forceinline__ uint32_t encode4(uint32_t lo, uint32_t hi, int e) {
+  if constexpr (kBf16) {
+    const float s = pow2f(-e);
+    const float2 a = unpack2<true>(lo), b = unpack2<true>(hi);
     if constexpr (kFormat == kKvE4M3) {
-      f = unpack2<false>(e4m3x2_to_half2(pair));
+      return float2_to_e4m3x2(a.x * s, a.y * s) | (float2_to_e4m3x2(b.x * s, b.y * s) << 16);
     } else {
-      f = make_float2(static_cast<float>(static_cast<int8_t>(pair & 0xffu)),
-                      static_cast<float>(static_cast<int8_t>((pair >> 8) & 0xffu)));
+      constexpr float kRound = 12582912.f;  // 1.5 * 2^23
+      const uint32_t x = __float_as_uint(fmaf(a.x, s, kRound)),
+                     y = __float_as_uint(fmaf(a.y, s, kRound)),
+                     z = __float_as_uint(fmaf(b.x, s, kRound)),
+                     t = __float_as_uint(fmaf(b.y, s, kRound));
+      return __byte_perm(__byte_perm(x, y, 0x0040), __byte_perm(z, t, 0x0040), 0x5410);
     }
-    out[i] = pack2<kBf16>(f.x * sa * sb, f.y * sa * sb);
+  } else {
+    const uint32_t s2 = pair_pow2<false>(-e);
+    const __half2 s = *reinterpret_cast<const __half2*>(&s2);
+    const __half2 a = *reinterpret_cast<const __half2*>(&lo);
+    const __half2 b = *reinterpret_cast<const __half2*>(&hi);
+    if constexpr (kFormat == kKvE4M3) {
+      const __half2 x = __hmul2(a, s), y = __hmul2(b, s);
+      return half2_to_e4m3x2(*reinterpret_cast<const uint32_t*>(&x)) |
+             (half2_to_e4m3x2(*reinterpret_cast<const uint32_t*>(&y)) << 16);
+    } else {
+      const __half2 round = __floats2half2_rn(1536.f, 1536.f);  // 1.5 * 2^10
+      const __half2 x = __hfma2(a, s, round), y = __hfma2(b, s, round);
+      return __byte_perm(*reinterpret_cast<const uint32_t*>(&x),
+                         *reinterpret_cast<const uint32_t*>(&y), 0x6420);
+    }
   }
-  return make_uint4(out[0], out[1], out[2], out[3]);
 }
 
 constexpr int kThreads = 256;
+constexpr int kVectors = 4;  // vectors of one thread group, loaded before any is used
 
-// d / 8 lanes a vector, one vector of k or v per lane group.
+// Where vector `vec` of the call is: vectors go head by head through k and then
+// v of a token.
+struct Where {
+  int64_t token;
+  int kv, head;
+};
+__device__ __forceinline__ Where where(const KvCacheArgs& a, uint32_t vec) {
+  const uint32_t th = vec / a.heads;
+  return {th >> 1, static_cast<int>(th & 1), static_cast<int>(vec - th * a.heads)};
+}
+
+// head_dim / 16 lanes hold a vector, 16 values each (two loads, one 16-byte
+// store of codes). HBM-bound: a thread's kVectors loads are in flight together.
 template <bool kBf16, int kFormat>
 __global__ void __launch_bounds__(kThreads) kv_write_kernel(const KvCacheArgs a) {
-  const int lanes = a.head_dim / 8;
-  const int64_t vec = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / lanes;
+  using C = Code<kBf16, kFormat == kKvPlain ? kKvE4M3 : kFormat>;
+  const int lanes = a.head_dim / 16, per_pass = kThreads / lanes;
   const int l = threadIdx.x % lanes;
-  const int64_t vectors = static_cast<int64_t>(a.tokens) * a.heads * 2;
-  const bool live = vec < vectors;
-  const int kv = static_cast<int>(vec & 1);
-  const int64_t th = vec >> 1;
-  const int64_t t = live ? th / a.heads : 0;
-  const int h = live ? static_cast<int>(th % a.heads) : 0;
-  const int64_t slot = a.slot_of[t];
-  const bool in = live && slot >= 0 && slot < a.slots;
-  uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-  const uint16_t* src = static_cast<const uint16_t*>(kv ? a.v_in : a.k_in);
-  if (in)
-    raw = *reinterpret_cast<const uint4*>(src + t * (kv ? a.v_stride : a.k_stride) +
-                                          static_cast<int64_t>(h) * a.head_dim + l * 8);
-  const int64_t at = (slot * a.heads + h) * a.head_dim + l * 8;
-  if constexpr (kFormat == kKvPlain) {
-    if (in) *reinterpret_cast<uint4*>(static_cast<uint16_t*>(kv ? a.v : a.k) + at) = raw;
-  } else {
-    float x[8];
-    float top = largest_of<kBf16>(raw, x);
-    for (int o = lanes >> 1; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const int e = Code<kBf16, kFormat>::exponent(top);
-    if (in) {
-      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(kv ? a.v : a.k) + at) =
-          encode8<kBf16, kFormat>(x, e);
-      if (l == 0) (kv ? a.v_scale : a.k_scale)[slot * a.heads + h] = static_cast<uint8_t>(e + 127);
+  const uint32_t v0 = blockIdx.x * (per_pass * kVectors) + threadIdx.x / lanes;
+  uint4 x[kVectors][2];
+  int64_t row[kVectors];  // (slot, head), -1: nothing to write
+#pragma unroll
+  for (int i = 0; i < kVectors; ++i) {
+    const uint32_t vec = v0 + i * per_pass;
+    row[i] = -1;
+    x[i][0] = x[i][1] = make_uint4(0u, 0u, 0u, 0u);
+    if (vec >= a.vectors) continue;
+    const Where w = where(a, vec);
+    const int64_t slot = __ldg(a.slot_of + w.token);
+    if (slot < 0 || slot >= a.slots) continue;
+    row[i] = slot * a.heads + w.head;
+    const uint4* src = reinterpret_cast<const uint4*>(
+        static_cast<const uint16_t*>(w.kv ? a.v_in : a.k_in) +
+        w.token * (w.kv ? a.v_stride : a.k_stride) +
+        static_cast<int64_t>(w.head) * a.head_dim + l * 16);
+    x[i][0] = __ldcs(src);
+    x[i][1] = __ldcs(src + 1);
+  }
+#pragma unroll
+  for (int i = 0; i < kVectors; ++i) {
+    const uint32_t vec = v0 + i * per_pass;
+    const bool v = (vec / a.heads) & 1;
+    const int64_t at = row[i] * a.head_dim + l * 16;
+    if constexpr (kFormat == kKvPlain) {
+      if (row[i] >= 0) {
+        uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(v ? a.v : a.k) + at);
+        dst[0] = x[i][0];
+        dst[1] = x[i][1];
+      }
+    } else {
+      uint32_t top = __vmaxu2(largest8(x[i][0]), largest8(x[i][1]));
+      for (int o = lanes >> 1; o > 0; o >>= 1)
+        top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o));
+      uint32_t bits = max(top & 0xffffu, top >> 16);
+      constexpr uint32_t kInf = kExpBits(kBf16);
+      const bool nan = bits > kInf;
+      if (__any_sync(0xffffffffu, nan)) {
+        uint32_t t = __vmaxu2(largest8_but_nan<kBf16>(x[i][0]), largest8_but_nan<kBf16>(x[i][1]));
+        for (int o = lanes >> 1; o > 0; o >>= 1)
+          t = __vmaxu2(t, __shfl_xor_sync(0xffffffffu, t, o));
+        bits = t & 0xffffu;
+      }
+      if (bits == kInf) bits = kInf - 1;  // infinities count as the largest finite value
+      const int e = C::exponent(bits);
+      // f16's short way multiplies by 2^-e in f16
+      const bool any = nan || e == C::kTop || (!kBf16 && e < -15);
+      uint4 code;
+      if (any) {
+        const uint2 p = encode8_any<kBf16, kFormat>(x[i][0], e);
+        const uint2 q = encode8_any<kBf16, kFormat>(x[i][1], e);
+        code = make_uint4(p.x, p.y, q.x, q.y);
+      } else {
+        code.x = encode4<kBf16, kFormat>(x[i][0].x, x[i][0].y, e);
+        code.y = encode4<kBf16, kFormat>(x[i][0].z, x[i][0].w, e);
+        code.z = encode4<kBf16, kFormat>(x[i][1].x, x[i][1].y, e);
+        code.w = encode4<kBf16, kFormat>(x[i][1].z, x[i][1].w, e);
+      }
+      if (row[i] >= 0) {
+        *reinterpret_cast<uint4*>(static_cast<uint8_t*>(v ? a.v : a.k) + at) = code;
+        if (l == 0) (v ? a.v_scale : a.k_scale)[row[i]] = static_cast<uint8_t>(e + 127);
+      }
     }
   }
 }
 
+// The way back: 16 codes a lane (one load, two stores).
 template <bool kBf16, int kFormat>
 __global__ void __launch_bounds__(kThreads) kv_read_kernel(const KvCacheArgs a) {
-  const int lanes = a.head_dim / 8;
-  const int64_t vec = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / lanes;
+  const int lanes = a.head_dim / 16, per_pass = kThreads / lanes;
   const int l = threadIdx.x % lanes;
-  if (vec >= static_cast<int64_t>(a.tokens) * a.heads * 2) return;
-  const int kv = static_cast<int>(vec & 1);
-  const int64_t t = (vec >> 1) / a.heads;
-  const int h = static_cast<int>((vec >> 1) % a.heads);
-  const int64_t slot = a.slot_of[t];
-  uint4 out = make_uint4(0u, 0u, 0u, 0u);
-  if (slot >= 0 && slot < a.slots) {
-    const int64_t at = (slot * a.heads + h) * a.head_dim + l * 8;
+  const uint32_t v0 = blockIdx.x * (per_pass * kVectors) + threadIdx.x / lanes;
+  uint4 x[kVectors][2];
+  int e[kVectors];
+#pragma unroll
+  for (int i = 0; i < kVectors; ++i) {
+    const uint32_t vec = v0 + i * per_pass;
+    x[i][0] = x[i][1] = make_uint4(0u, 0u, 0u, 0u);
+    e[i] = 0;
+    if (vec >= a.vectors) continue;
+    const Where w = where(a, vec);
+    const int64_t slot = __ldg(a.slot_of + w.token);
+    if (slot < 0 || slot >= a.slots) continue;  // zeros
+    const int64_t row = slot * a.heads + w.head, at = row * a.head_dim + l * 16;
     if constexpr (kFormat == kKvPlain) {
-      out = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(kv ? a.v : a.k) + at);
+      const uint4* src =
+          reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(w.kv ? a.v : a.k) + at);
+      x[i][0] = src[0];
+      x[i][1] = src[1];
     } else {
-      const uint2 codes =
-          *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(kv ? a.v : a.k) + at);
-      const int e = static_cast<int>((kv ? a.v_scale : a.k_scale)[slot * a.heads + h]) - 127;
-      out = decode8<kBf16, kFormat>(codes, e);
+      x[i][0] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(w.kv ? a.v : a.k) + at);
+      e[i] = static_cast<int>((w.kv ? a.v_scale : a.k_scale)[row]) - 127;
     }
   }
-  uint16_t* dst = static_cast<uint16_t*>(kv ? a.v_out : a.k_out);
-  *reinterpret_cast<uint4*>(dst + (t * a.heads + h) * a.head_dim + l * 8) = out;
+#pragma unroll
+  for (int i = 0; i < kVectors; ++i) {
+    const uint32_t vec = v0 + i * per_pass;
+    if (vec >= a.vectors) break;
+    const Where w = where(a, vec);
+    if constexpr (kFormat != kKvPlain) {
+      const uint32_t c[4] = {x[i][0].x, x[i][0].y, x[i][0].z, x[i][0].w};
+      const uint32_t s2 = pair_pow2<kBf16>(e[i]);
+      uint32_t y[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        y[j] = code_pair<kBf16, kFormat == kKvE4M3>((c[j >> 1] >> (16 * (j & 1))) & 0xffffu, s2);
+      x[i][0] = make_uint4(y[0], y[1], y[2], y[3]);
+      x[i][1] = make_uint4(y[4], y[5], y[6], y[7]);
+    }
+    uint4* dst = reinterpret_cast<uint4*>(
+        static_cast<uint16_t*>(w.kv ? a.v_out : a.k_out) +
+        (w.token * a.heads + w.head) * a.head_dim + l * 16);
+    dst[0] = x[i][0];
+    dst[1] = x[i][1];
+  }
 }
 
 template <bool kWrite, bool kBf16>
 cudaError_t launch_format(const KvCacheArgs& a, int format, cudaStream_t stream) {
-  const int64_t threads = static_cast<int64_t>(a.tokens) * a.heads * 2 * (a.head_dim / 8);
-  const unsigned blocks = static_cast<unsigned>((threads + kThreads - 1) / kThreads);
+  const int64_t per_block = kThreads / (a.head_dim / 16) * kVectors;
+  const unsigned blocks = static_cast<unsigned>((a.vectors + per_block - 1) / per_block);
   auto go = [&](auto kernel) { kernel<<<blocks, kThreads, 0, stream>>>(a); };
   if constexpr (kWrite) {
     if (format == kKvPlain) go(kv_write_kernel<kBf16, kKvPlain>);

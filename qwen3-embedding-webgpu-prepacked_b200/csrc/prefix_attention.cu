@@ -168,40 +168,6 @@ __device__ __forceinline__ void mask_keys(uint32_t (&a)[32], const Kept& k, int 
 }
 
 // ------------------------------------------------------------- 8-bit tiles
-// 2^e as two equal 16-bit (f16) values; out of f16's range it is 0 or inf.
-__device__ __forceinline__ uint32_t half2_pow2(int e) {
-  uint32_t h;
-  if (e > 15) h = 0x7c00u;
-  else if (e >= -14) h = static_cast<uint32_t>(e + 15) << 10;
-  else if (e >= -24) h = 1u << (e + 24);
-  else h = 0u;
-  return h | (h << 16);
-}
-
-// Two codes (the low 16 bits) -> the 16-bit pair of values that they stand for.
-template <bool kBf16, int kFormat>
-__device__ __forceinline__ uint32_t code_pair(uint32_t codes, uint32_t scale_h2, float scale_a,
-                                              float scale_b) {
-  uint32_t h;
-  if constexpr (kFormat == kKvE4M3) {
-    h = e4m3x2_to_half2(codes);
-  } else {
-    // 1024 + (code + 128) has the code's bits in an f16's low byte
-    const uint32_t u = __byte_perm(codes ^ 0x8080u, 0x64646464u, 0x4140);
-    const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&u),
-                              __floats2half2_rn(1152.f, 1152.f));
-    h = *reinterpret_cast<const uint32_t*>(&v);
-  }
-  if constexpr (kBf16) {
-    const float2 f = unpack2<false>(h);
-    return pack2<true>(f.x * scale_a * scale_b, f.y * scale_a * scale_b);
-  } else {
-    const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&h),
-                              *reinterpret_cast<const __half2*>(&scale_h2));
-    return *reinterpret_cast<const uint32_t*>(&v);
-  }
-}
-
 // Clears the halves of w whose exponent is all ones (inf, NaN).
 template <bool kBf16>
 __device__ __forceinline__ uint32_t finite_only(uint32_t w, bool& bad) {
@@ -242,18 +208,16 @@ __device__ __forceinline__ bool convert_tile(uint32_t stage, uint32_t slot, uint
   const uint32_t base = slot + odd * kHalfBytes + r0 * 128;
   const uint32_t at_a = base + (static_cast<uint32_t>((u & 3) * 2 + odd) ^ (r0 & 7)) * 16;
   const uint32_t at_b = base + (static_cast<uint32_t>((u & 3) * 2 + 1 - odd) ^ (r0 & 7)) * 16;
-  const uint32_t mine = kBf16 ? scale : half2_pow2(static_cast<int>(scale) - 127);
+  const uint32_t mine = pair_pow2<kBf16>(static_cast<int>(scale) - 127);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const uint4 raw = ld_shared_v4(from + i * 2048);
     const uint32_t sc = __shfl_sync(0xffffffffu, mine, i * 4 + (lane >> 3));
-    const int e = static_cast<int>(sc) - 127;  // bf16
-    const float sa = pow2f(e / 2), sb = pow2f(e - e / 2);
     const uint32_t c[4] = {raw.x, raw.y, raw.z, raw.w};
     uint32_t v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      v[j] = code_pair<kBf16, kFormat>((c[j >> 1] >> (16 * (j & 1))) & 0xffffu, sc, sa, sb);
+      v[j] = code_pair<kBf16, kFormat == kKvE4M3>((c[j >> 1] >> (16 * (j & 1))) & 0xffffu, sc);
     if (guard) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = finite_only<kBf16>(v[j], bad);
@@ -318,8 +282,7 @@ __device__ __noinline__ Aside find_aside(const PrefixArgs& a, int tile_beg, int 
             const int64_t at = key * a.kv_heads + head;
             const int e = static_cast<int>(a.v_scale[at]) - 127;
             const uint32_t code = static_cast<const uint8_t*>(a.v_prefix)[at * kHeadDim + dim];
-            v = code_pair<kBf16, kFormat>(code, half2_pow2(e), pow2f(e / 2), pow2f(e - e / 2)) &
-                0xffffu;
+            v = code_pair<kBf16, kFormat == kKvE4M3>(code, pair_pow2<kBf16>(e)) & 0xffffu;
           }
           constexpr uint32_t kExp = kBf16 ? 0x7f80u : 0x7c00u;
           if ((v & kExp) != kExp) continue;

@@ -19,8 +19,12 @@ namespace qwa {
 namespace {
 
 // ------------------------------------------------------------------- table
-constexpr int kTableRun = 16;       // consecutive positions of one thread
-constexpr int kTableThreads = 256;
+// A thread takes one frequency over kTableRun positions: sin and cos of the
+// first, then turns by f in 64 bits (16 turns add less than 2^-47, far below the
+// rounding to f32). With sincos for every entry the kernel was bound by its 64-bit
+// arithmetic (27 us for 131072 x 64 entries, against 10 us to write them).
+constexpr int kTableRun = 16;
+constexpr int kTableThreads = 128;
 
 __global__ void __launch_bounds__(kTableThreads)
     rope_table_kernel(const __grid_constant__ RopeFrequencies fr, float2* __restrict__ table,
@@ -32,11 +36,17 @@ __global__ void __launch_bounds__(kTableThreads)
   const double f = fr.f[i];
   const int n = static_cast<int>(positions - p0 < kTableRun ? positions - p0 : kTableRun);
   float2* dst = table + p0 * fr.half + i;
+  double s, c, sf, cf;
+  sincos(static_cast<double>(first + p0) * f, &s, &c);
+  sincos(f, &sf, &cf);
+  s *= fr.m;
+  c *= fr.m;
   for (int j = 0; j < n; ++j) {
-    double s, c;
-    sincos(static_cast<double>(first + p0 + j) * f, &s, &c);
-    dst[static_cast<int64_t>(j) * fr.half] =
-        make_float2(static_cast<float>(c * fr.m), static_cast<float>(s * fr.m));
+    *dst = make_float2(static_cast<float>(c), static_cast<float>(s));
+    dst += fr.half;
+    const double next = c * cf - s * sf;
+    s = s * cf + c * sf;
+    c = next;
   }
 }
 
@@ -82,6 +92,97 @@ __global__ void __launch_bounds__(kRopeThreads) rope_any_kernel(const RopeArgs a
   }
 }
 
+// Rows of whole 16-byte units. A thread owns one unit u of the heads hs, hs +
+// step, ... of a token, so its cosines and sines are read once. Units of a head:
+//   half:        u < rotary / 16: the 8 pairs from 8 u on (two 16-byte loads);
+//                then the units behind the rotated part, copied
+//   interleaved: 4 pairs, of which those past the rotated part are copied
+// HBM-bound: up to kRopeHeads heads' loads of a thread are issued before any
+// arithmetic.
+constexpr int kRopeHeads = 4;
+
+template <bool kBf16>
+__device__ __forceinline__ uint32_t turn_pair(uint32_t x, float c, float s) {
+  const float2 v = unpack2<kBf16>(x);
+  return pack2<kBf16>(v.x * c - v.y * s, v.y * c + v.x * s);
+}
+
+template <bool kBf16, bool kInterleaved>
+__global__ void __launch_bounds__(kRopeThreads) rope_rows_kernel(const RopeArgs a) {
+  const int group = threadIdx.x / a.token_threads;  // token of the block
+  const int r = threadIdx.x - group * a.token_threads;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * a.block_tokens + group;
+  if (group >= a.block_tokens || t >= a.tokens) return;
+  const int u = r % a.units, hs = r / a.units;
+  const int pos = __ldg(a.positions + t);
+  if (pos < 0 || pos >= a.table_rows) return;
+  const int half = a.rotary / 2, heads = a.q.heads + a.k.heads;
+  const float2* row = a.table + static_cast<int64_t>(pos) * half;
+  const bool turns = kInterleaved ? u * 4 < half : u * 8 < half;
+  constexpr int kPairs = kInterleaved ? 4 : 8;
+  float c[kPairs], s[kPairs];
+  int at = u * 8;  // first value of the unit
+  if (turns) {
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+      const bool in = !kInterleaved || u * 4 + i < half;
+      const float2 cs = in ? __ldg(row + u * kPairs + i) : make_float2(1.f, 0.f);
+      c[i] = cs.x;
+      s[i] = a.inverse ? -cs.y : cs.y;
+    }
+  } else if (!kInterleaved) {
+    at = a.rotary + (u - half / 8) * 8;
+  }
+  for (int h0 = hs; h0 < heads; h0 += kRopeHeads * a.head_step) {
+    uint4 x[kRopeHeads], y[kRopeHeads];
+#pragma unroll
+    for (int i = 0; i < kRopeHeads; ++i) {
+      const int h = h0 + i * a.head_step;
+      if (h < heads) {
+        const uint16_t* src = a.in_row(t, h) + at;
+        x[i] = __ldcs(reinterpret_cast<const uint4*>(src));
+        if (!kInterleaved && turns) y[i] = __ldcs(reinterpret_cast<const uint4*>(src + half));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kRopeHeads; ++i) {
+      const int h = h0 + i * a.head_step;
+      if (h >= heads) break;
+      uint16_t* dst = a.out_row(t, h) + at;
+      if (turns) {
+        uint32_t xs[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+        if constexpr (kInterleaved) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t turned = turn_pair<kBf16>(xs[j], c[j], s[j]);
+            if (u * 4 + j < half) xs[j] = turned;
+          }
+        } else {
+          uint32_t ys[4] = {y[i].x, y[i].y, y[i].z, y[i].w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 p = unpack2<kBf16>(xs[j]), q = unpack2<kBf16>(ys[j]);
+            const float c0 = c[2 * j], c1 = c[2 * j + 1], s0 = s[2 * j], s1 = s[2 * j + 1];
+            xs[j] = pack2<kBf16>(p.x * c0 - q.x * s0, p.y * c1 - q.y * s1);
+            ys[j] = pack2<kBf16>(q.x * c0 + p.x * s0, q.y * c1 + p.y * s1);
+          }
+          *reinterpret_cast<uint4*>(dst + half) = make_uint4(ys[0], ys[1], ys[2], ys[3]);
+        }
+        x[i] = make_uint4(xs[0], xs[1], xs[2], xs[3]);
+      }
+      *reinterpret_cast<uint4*>(dst) = x[i];
+    }
+  }
+}
+
+bool whole_units(const RopeSide& s) {
+  auto multiple = [](const void* p, int64_t a, int64_t b) {
+    return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && a % 8 == 0 && b % 8 == 0;
+  };
+  return s.heads == 0 || (multiple(s.in, s.in_stride, s.in_head_stride) &&
+                          multiple(s.out, s.out_stride, s.out_head_stride));
+}
+
 }  // namespace
 
 cudaError_t launch_rope_table(const RopeFrequencies& fr, float2* table, int64_t first,
@@ -95,9 +196,27 @@ cudaError_t launch_rope_table(const RopeFrequencies& fr, float2* table, int64_t 
 }
 
 cudaError_t launch_rope(RopeArgs a, int bf16, cudaStream_t stream) {
-  if (a.tokens <= 0 || a.q.heads + a.k.heads <= 0) return cudaSuccess;
-  a.smem_heads = 32768 / (a.head_dim * 2);
   const int heads = a.q.heads + a.k.heads;
+  if (a.tokens <= 0 || heads <= 0) return cudaSuccess;
+  // 16-byte units need whole units on both sides of a pair of halves; pairs of
+  // neighbours never straddle one
+  const bool rows = a.head_dim % 8 == 0 && a.head_dim <= 8 * kRopeThreads && whole_units(a.q) &&
+                    whole_units(a.k) && (a.layout == 1 || a.rotary % 16 == 0);
+  if (rows) {
+    a.units = a.layout == 1 ? a.head_dim / 8 : a.rotary / 16 + (a.head_dim - a.rotary) / 8;
+    // Heads of one thread: kRopeHeads, so that a token's cosines are read by few
+    // threads; one where there are few tokens, for latency.
+    const int step = a.tokens >= 1024 ? (heads + kRopeHeads - 1) / kRopeHeads : heads;
+    a.head_step = step * a.units <= kRopeThreads ? step : kRopeThreads / a.units;
+    a.token_threads = a.units * a.head_step;
+    a.block_tokens = kRopeThreads / a.token_threads;
+    const unsigned blocks = static_cast<unsigned>((a.tokens + a.block_tokens - 1) / a.block_tokens);
+    auto go = [&](auto kernel) { kernel<<<blocks, kRopeThreads, 0, stream>>>(a); };
+    if (bf16) a.layout == 1 ? go(rope_rows_kernel<true, true>) : go(rope_rows_kernel<true, false>);
+    else a.layout == 1 ? go(rope_rows_kernel<false, true>) : go(rope_rows_kernel<false, false>);
+    return cudaGetLastError();
+  }
+  a.smem_heads = 32768 / (a.head_dim * 2);
   if (a.smem_heads > heads) a.smem_heads = heads;
   const size_t smem = static_cast<size_t>(a.smem_heads) * a.head_dim * 2;
   if (bf16)
