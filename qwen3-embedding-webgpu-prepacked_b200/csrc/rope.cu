@@ -97,9 +97,9 @@ __global__ void __launch_bounds__(kRopeThreads) rope_any_kernel(const RopeArgs a
 //   half:        u < rotary / 16: the 8 pairs from 8 u on (two 16-byte loads);
 //                then the units behind the rotated part, copied
 //   interleaved: 4 pairs, of which those past the rotated part are copied
-// HBM-bound: up to kRopeHeads heads' loads of a thread are issued before any
-// arithmetic.
-constexpr int kRopeHeads = 4;
+// HBM-bound: a thread issues the loads of kHeads heads before any arithmetic,
+// six in both layouts.
+constexpr int kRowThreads = 128;
 
 template <bool kBf16>
 __device__ __forceinline__ uint32_t turn_pair(uint32_t x, float c, float s) {
@@ -108,7 +108,8 @@ __device__ __forceinline__ uint32_t turn_pair(uint32_t x, float c, float s) {
 }
 
 template <bool kBf16, bool kInterleaved>
-__global__ void __launch_bounds__(kRopeThreads) rope_rows_kernel(const RopeArgs a) {
+__global__ void __launch_bounds__(kRowThreads) rope_rows_kernel(const RopeArgs a) {
+  constexpr int kHeads = kInterleaved ? 6 : 3;
   const int group = threadIdx.x / a.token_threads;  // token of the block
   const int r = threadIdx.x - group * a.token_threads;
   const int64_t t = static_cast<int64_t>(blockIdx.x) * a.block_tokens + group;
@@ -119,9 +120,10 @@ __global__ void __launch_bounds__(kRopeThreads) rope_rows_kernel(const RopeArgs 
   const int half = a.rotary / 2, heads = a.q.heads + a.k.heads;
   const float2* row = a.table + static_cast<int64_t>(pos) * half;
   const bool turns = kInterleaved ? u * 4 < half : u * 8 < half;
+  // first value of the unit
+  const int at = kInterleaved || turns ? u * 8 : a.rotary + (u - half / 8) * 8;
   constexpr int kPairs = kInterleaved ? 4 : 8;
   float c[kPairs], s[kPairs];
-  int at = u * 8;  // first value of the unit
   if (turns) {
 #pragma unroll
     for (int i = 0; i < kPairs; ++i) {
@@ -130,13 +132,11 @@ __global__ void __launch_bounds__(kRopeThreads) rope_rows_kernel(const RopeArgs 
       c[i] = cs.x;
       s[i] = a.inverse ? -cs.y : cs.y;
     }
-  } else if (!kInterleaved) {
-    at = a.rotary + (u - half / 8) * 8;
   }
-  for (int h0 = hs; h0 < heads; h0 += kRopeHeads * a.head_step) {
-    uint4 x[kRopeHeads], y[kRopeHeads];
+  for (int h0 = hs; h0 < heads; h0 += kHeads * a.head_step) {
+    uint4 x[kHeads], y[kHeads];
 #pragma unroll
-    for (int i = 0; i < kRopeHeads; ++i) {
+    for (int i = 0; i < kHeads; ++i) {
       const int h = h0 + i * a.head_step;
       if (h < heads) {
         const uint16_t* src = a.in_row(t, h) + at;
@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_rows_kernel(const RopeArgs 
       }
     }
 #pragma unroll
-    for (int i = 0; i < kRopeHeads; ++i) {
+    for (int i = 0; i < kHeads; ++i) {
       const int h = h0 + i * a.head_step;
       if (h >= heads) break;
       uint16_t* dst = a.out_row(t, h) + at;
@@ -200,18 +200,19 @@ cudaError_t launch_rope(RopeArgs a, int bf16, cudaStream_t stream) {
   if (a.tokens <= 0 || heads <= 0) return cudaSuccess;
   // 16-byte units need whole units on both sides of a pair of halves; pairs of
   // neighbours never straddle one
-  const bool rows = a.head_dim % 8 == 0 && a.head_dim <= 8 * kRopeThreads && whole_units(a.q) &&
+  const bool rows = a.head_dim % 8 == 0 && a.head_dim <= 8 * kRowThreads && whole_units(a.q) &&
                     whole_units(a.k) && (a.layout == 1 || a.rotary % 16 == 0);
   if (rows) {
     a.units = a.layout == 1 ? a.head_dim / 8 : a.rotary / 16 + (a.head_dim - a.rotary) / 8;
-    // Heads of one thread: kRopeHeads, so that a token's cosines are read by few
-    // threads; one where there are few tokens, for latency.
-    const int step = a.tokens >= 1024 ? (heads + kRopeHeads - 1) / kRopeHeads : heads;
-    a.head_step = step * a.units <= kRopeThreads ? step : kRopeThreads / a.units;
+    // Heads of one thread: as many as it has loads in flight for, so that few
+    // threads read a token's cosines; one where there are few tokens, for latency.
+    const int most = a.layout == 1 ? 6 : 3;
+    const int step = a.tokens >= 1024 ? (heads + most - 1) / most : heads;
+    a.head_step = step * a.units <= kRowThreads ? step : kRowThreads / a.units;
     a.token_threads = a.units * a.head_step;
-    a.block_tokens = kRopeThreads / a.token_threads;
+    a.block_tokens = kRowThreads / a.token_threads;
     const unsigned blocks = static_cast<unsigned>((a.tokens + a.block_tokens - 1) / a.block_tokens);
-    auto go = [&](auto kernel) { kernel<<<blocks, kRopeThreads, 0, stream>>>(a); };
+    auto go = [&](auto kernel) { kernel<<<blocks, kRowThreads, 0, stream>>>(a); };
     if (bf16) a.layout == 1 ? go(rope_rows_kernel<true, true>) : go(rope_rows_kernel<true, false>);
     else a.layout == 1 ? go(rope_rows_kernel<false, true>) : go(rope_rows_kernel<false, false>);
     return cudaGetLastError();
