@@ -435,6 +435,11 @@ QWA_API qwa_status qwa_prefix_plan_create(qwa_ctx *ctx, const int32_t *cu_seqlen
                                           int sparse_prefix, int window, qwa_prefix_plan **out);
 QWA_API qwa_status qwa_prefix_plan_destroy(qwa_prefix_plan *plan);
 
+/* Bytes of device memory with which qwa_prefix_attention converts an 8-bit
+ * prefix once instead of once for every block of rows; 0 where that does not
+ * pay. format: a qwa_kv_format. */
+QWA_API size_t qwa_prefix_attention_workspace(const qwa_prefix_plan *plan, int format);
+
 /* Attention of the plan's requests behind the prefix held in the cache's slots
  * first_slot .. first_slot + prefix_len - 1 (cache may be NULL if prefix_len is 0):
  * every query sees the prefix and its request's own keys up to itself,
@@ -443,12 +448,14 @@ QWA_API qwa_status qwa_prefix_plan_destroy(qwa_prefix_plan *plan);
  * elements a token (multiples of 8), out [queries, q_heads, 128] contiguous; all
  * 16-byte aligned, head_dim 128. The prefix is read and multiplied once for
  * the rows of all requests together. A value of v that is not finite reaches only the
- * queries that see it. */
+ * queries that see it. workspace: NULL, or workspace_bytes of device memory,
+ * 16-byte aligned, that no other call uses at the same time; with fewer bytes than
+ * qwa_prefix_attention_workspace says it is not used. */
 QWA_API qwa_status qwa_prefix_attention(qwa_ctx *ctx, const qwa_prefix_plan *plan, int dtype,
                                         const void *q, int64_t q_stride, const void *k,
                                         int64_t k_stride, const void *v, int64_t v_stride,
                                         void *out, const qwa_kv_cache *cache, int64_t first_slot,
-                                        void *stream);
+                                        void *workspace, size_t workspace_bytes, void *stream);
 
 /* Work of such a call: kept (query, key) pairs of one query head (FLOPs = 512 *
  * q_heads * pairs), and key tiles visited over all kv heads. */

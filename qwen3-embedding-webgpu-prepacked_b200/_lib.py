@@ -87,7 +87,9 @@ SIGNATURES = {
     "qwa_prefix_plan_create": (I32, [P, I32P, I32P, I32, I32, I32, I32, I32, I32, I32,
                                      ctypes.POINTER(P)]),
     "qwa_prefix_plan_destroy": (I32, [P]),
-    "qwa_prefix_attention": (I32, [P, P, I32, P, I64, P, I64, P, I64, P, KvCacheP, I64, P]),
+    "qwa_prefix_attention_workspace": (ctypes.c_size_t, [P, I32]),
+    "qwa_prefix_attention": (I32, [P, P, I32, P, I64, P, I64, P, I64, P, KvCacheP, I64, P,
+                                   ctypes.c_size_t, P]),
     "qwa_prefix_attention_work": (I32, [I32P, I32P, I32, I32, I32, I32, I32, I32, I32, I64P,
                                         I64P]),
 }

@@ -72,6 +72,7 @@ struct qwa_ctx {
   int skip_load = -1;                             // test hook, see qwa_set_debug
   float* small_ws = nullptr;                      // partial sums of the small-M Q4_0 path
   size_t small_ws_bytes = 0;
+  int clusters[9] = {};           // [n]: clusters of n CTAs that run at one time
   cudaStream_t upload = nullptr;  // copies of prefix plans, waited for before they are used
 };
 
@@ -86,6 +87,8 @@ struct qwa_prefix_plan {
   const PrefixRow* rows = nullptr;
   const int* offsets = nullptr;
   int grid = 0, splits = 1;
+  int blocks = 0;                // blocks of rows, each with all kv heads
+  int gap_beg = 0, gap_end = 0;  // prefix keys that no tile reaches
 };
 
 namespace {
@@ -1310,25 +1313,97 @@ qwa_status make_code_map(qwa_ctx* ctx, CUtensorMap* map, const void* base, int h
   return QWA_OK;
 }
 
-// CTAs of a cluster that share a block's tiles: as many as keep the SMs busy,
-// each with a tile at least.
-int prefix_splits(const PrefixWork& w, int items, int sms) {
-  int least = 1 << 30;
-  for (const PrefixItem& i : w.items) least = std::min(least, i.tile_end - i.tile_beg);
-  const int s = std::min(std::min(8, sms / std::max(items, 1)), least);
-  return std::max(s, 1);
+// An 8-bit prefix is converted once into a workspace, or tile by tile on the way of
+// each block. Once pays from two blocks on unless the prefix is short: E4M3, 3
+// blocks behind 1000 keys 39 us against 41, 2 behind 4000 50 against 53, 10 behind 200
+// 19 against 24; but 5 behind 200 23.3 against 22.0, 1 behind 8000 32 against 30.
+bool convert_once(int blocks, int prefix_len) {
+  return blocks >= 2 && static_cast<int64_t>(blocks) * prefix_len >= 2000;
+}
+
+constexpr int kMaxSplits = 8;  // the portable cluster size
+
+// How a call's blocks go over the SMs: the CTAs of a cluster that share a block's
+// tiles (1: none, whole blocks dealt to the SMs), and an estimate of its time. Its unit is the
+// period of one key tile for two row tiles (2.3 us). A cluster costs a start and
+// a merge more, which moves 512 bytes a row between SMs, and as many rounds as the
+// clusters do not fit at once (of 8 CTAs 15 fit, not 18: the GPCs are not even).
+struct PrefixDeal {
+  int splits = 1;
+  double cost = 0;
+};
+PrefixDeal prefix_deal(qwa_ctx* ctx, const PrefixWork& w, const PrefixShape& s) {
+  const int64_t items = static_cast<int64_t>(w.items.size()) * s.kv_heads;
+  int least = 1 << 30, most = 0, tokens = 0;
+  double longest = 0, total = 0;
+  for (size_t i = 0; i < w.items.size(); ++i) {
+    const int n = w.items[i].tile_end - w.items[i].tile_beg;
+    least = std::min(least, n);
+    most = std::max(most, n);
+    tokens = std::max(tokens, w.items[i].tokens);
+    longest = std::max(longest, w.cost[i]);
+    total += w.cost[i] * s.kv_heads;
+  }
+  PrefixDeal best;
+  best.cost = std::max(longest, total / ctx->sms);
+  if (items > ctx->sms) {
+    // rounds of whole blocks: the last is rarely full
+    const int64_t rounds = (items + ctx->sms - 1) / ctx->sms;
+    best.cost = std::max(best.cost, rounds * total / static_cast<double>(items));
+  }
+  if (items >= ctx->sms) return best;
+  if (ctx->clusters[1] == 0) {
+    ctx->clusters[1] = ctx->sms;
+    for (int i = 2; i <= kMaxSplits; ++i) ctx->clusters[i] = prefix_active_clusters(i);
+  }
+  const int rows = tokens * (s.q_heads / s.kv_heads);
+  const double merge = 0.8 + rows / 128.0;
+  for (int n = 2; n <= std::min(kMaxSplits, least); ++n) {
+    if (ctx->clusters[n] < 1) continue;
+    const int64_t rounds = (items + ctx->clusters[n] - 1) / ctx->clusters[n];
+    const int share = (most + n - 1) / n;
+    const double cost = rounds * ((tokens <= s.tile_tokens ? (share + 1) / 2 : share) + 0.6 + merge) +
+                        (rounds - 1) * 2.0;
+    if (cost < best.cost) {
+      best.splits = n;
+      best.cost = cost;
+    }
+  }
+  return best;
 }
 
 qwa_status create_prefix_plan(qwa_ctx* ctx, const int32_t* cu_q, const int32_t* cu_k,
-                              const PrefixShape& shape, qwa_prefix_plan** out) {
+                              PrefixShape shape, qwa_prefix_plan** out) {
   auto plan = std::make_unique<qwa_prefix_plan>();
   plan->device = ctx->device;
-  plan->shape = shape;
   plan->total_q = cu_q[shape.batch];
   plan->total_k = cu_k[shape.batch];
+  PrefixWork w;
   if (plan->total_q > 0) {
-    const PrefixWork w = build_prefix_work(shape, cu_q, cu_k);
+    // Blocks of two row tiles read and convert less; blocks of one give more SMs
+    // work where there are few.
+    w = build_prefix_work(shape, cu_q, cu_k);
+    PrefixDeal deal = prefix_deal(ctx, w, shape);
+    if (static_cast<int64_t>(w.items.size()) * shape.kv_heads < 2 * ctx->sms &&
+        plan->total_q > shape.tile_tokens) {
+      PrefixShape low = shape;
+      low.block_tokens = shape.tile_tokens;
+      PrefixWork w_low = build_prefix_work(low, cu_q, cu_k);
+      const PrefixDeal deal_low = prefix_deal(ctx, w_low, low);
+      if (deal_low.cost < 0.95 * deal.cost) {
+        shape = low;
+        deal = deal_low;
+        w = std::move(w_low);
+      }
+    }
+    plan->splits = deal.splits;
+  }
+  plan->shape = shape;
+  if (plan->total_q > 0) {
     const int blocks = static_cast<int>(w.items.size());
+    plan->blocks = blocks;
+    plan->gap_beg = w.gap_beg;
+    plan->gap_end = w.gap_end;
     const int64_t n = static_cast<int64_t>(blocks) * shape.kv_heads;
     if (n > 0x7fffffff / 8)
       return fail(ctx, QWA_ERR_UNSUPPORTED, "too many blocks of rows (%lld)",
@@ -1336,7 +1411,6 @@ qwa_status create_prefix_plan(qwa_ctx* ctx, const int32_t* cu_q, const int32_t* 
     std::vector<PrefixItem> items;
     items.reserve(n);
     std::vector<int> offsets(1, 0);
-    plan->splits = prefix_splits(w, static_cast<int>(n), ctx->sms);
     if (plan->splits > 1) {
       for (int i = 0; i < blocks; ++i)
         for (int g = 0; g < shape.kv_heads; ++g) {
@@ -1432,10 +1506,17 @@ qwa_status qwa_prefix_plan_destroy(qwa_prefix_plan* plan) {
   return QWA_OK;
 }
 
+size_t qwa_prefix_attention_workspace(const qwa_prefix_plan* plan, int format) {
+  if (!plan || format == QWA_KV_PLAIN || !convert_once(plan->blocks, plan->shape.prefix_len))
+    return 0;
+  return static_cast<size_t>(plan->shape.prefix_len) * plan->shape.kv_heads * kHeadDim * 4;
+}
+
 qwa_status qwa_prefix_attention(qwa_ctx* ctx, const qwa_prefix_plan* plan, int dtype,
                                 const void* q, int64_t q_stride, const void* k, int64_t k_stride,
                                 const void* v, int64_t v_stride, void* out,
-                                const qwa_kv_cache* cache, int64_t first_slot, void* stream) {
+                                const qwa_kv_cache* cache, int64_t first_slot, void* workspace,
+                                size_t workspace_bytes, void* stream) {
   if (!ctx) return QWA_ERR_INVALID_ARG;
   if (!plan) return fail(ctx, QWA_ERR_INVALID_ARG, "plan is NULL");
   if (plan->device != ctx->device)
@@ -1487,6 +1568,33 @@ qwa_status qwa_prefix_attention(qwa_ctx* ctx, const qwa_prefix_plan* plan, int d
     const int64_t at = first_slot * kv_width * (format == QWA_KV_PLAIN ? 2 : 1);
     a.k_prefix = static_cast<const uint8_t*>(cache->k) + at;
     a.v_prefix = static_cast<const uint8_t*>(cache->v) + at;
+    const size_t need = qwa_prefix_attention_workspace(plan, format);
+    if (workspace && need > 0 && workspace_bytes >= need) {
+      if (!aligned16(workspace))
+        return fail(ctx, QWA_ERR_INVALID_ARG, "workspace must be 16-byte aligned");
+      // the prefix as 16-bit values, made once for all blocks
+      KvCacheArgs c{};
+      c.k = const_cast<void*>(cache->k);
+      c.v = const_cast<void*>(cache->v);
+      c.k_scale = cache->k_scale;
+      c.v_scale = cache->v_scale;
+      c.slots = cache->slots;
+      c.heads = s.kv_heads;
+      c.head_dim = kHeadDim;
+      c.first_slot = first_slot;
+      c.head = plan->gap_beg;
+      c.gap = plan->gap_end - plan->gap_beg;
+      c.tokens = s.prefix_len - c.gap;
+      c.vectors = 2u * static_cast<uint32_t>(c.tokens) * static_cast<uint32_t>(c.heads);
+      c.k_out = workspace;
+      c.v_out = static_cast<uint8_t*>(workspace) + need / 2;
+      if (static_cast<int64_t>(c.tokens) * c.heads > (1ll << 30))
+        return fail(ctx, QWA_ERR_INVALID_ARG, "prefix_len * kv_heads must be at most 2^30");
+      QWA_CUDA(ctx, launch_kv_read(c, bf16, format, static_cast<cudaStream_t>(stream)));
+      a.k_prefix = c.k_out;
+      a.v_prefix = c.v_out;
+      format = QWA_KV_PLAIN;
+    }
     if (format != QWA_KV_PLAIN) {
       if ((st = make_code_map(ctx, &m.pk, a.k_prefix, s.kv_heads, s.prefix_len)) != QWA_OK)
         return st;

@@ -274,7 +274,9 @@ struct KvCacheArgs {
   int64_t slots;
   int heads, head_dim, tokens;
   uint32_t vectors;        // 2 * tokens * heads
-  const int32_t* slot_of;  // [tokens]
+  const int32_t* slot_of;  // [tokens]; reading, nullptr: slots in order (below)
+  int64_t first_slot;      // of the first row; rows from `head` on lie `gap` rows
+  int head, gap;           // further, in the cache and in the output
   const void *k_in, *v_in;
   int64_t k_stride, v_stride;  // elements a token
   void *k_out, *v_out;

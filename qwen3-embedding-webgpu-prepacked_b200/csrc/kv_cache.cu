@@ -227,7 +227,9 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const KvCacheArgs a) 
     e[i] = 0;
     if (vec >= a.vectors) continue;
     const Where w = where(a, vec);
-    const int64_t slot = __ldg(a.slot_of + w.token);
+    // without a list: the slots from first_slot on, a gap left out after `head`
+    const int64_t slot = a.slot_of ? __ldg(a.slot_of + w.token)
+                                   : a.first_slot + w.token + (w.token >= a.head ? a.gap : 0);
     if (slot < 0 || slot >= a.slots) continue;  // zeros
     const int64_t row = slot * a.heads + w.head, at = row * a.head_dim + l * 16;
     if constexpr (kFormat == kKvPlain) {
@@ -255,9 +257,9 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const KvCacheArgs a) 
       x[i][0] = make_uint4(y[0], y[1], y[2], y[3]);
       x[i][1] = make_uint4(y[4], y[5], y[6], y[7]);
     }
-    uint4* dst = reinterpret_cast<uint4*>(
-        static_cast<uint16_t*>(w.kv ? a.v_out : a.k_out) +
-        (w.token * a.heads + w.head) * a.head_dim + l * 16);
+    const int64_t to = a.slot_of || w.token < a.head ? w.token : w.token + a.gap;
+    uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(w.kv ? a.v_out : a.k_out) +
+                                          (to * a.heads + w.head) * a.head_dim + l * 16);
     dst[0] = x[i][0];
     dst[1] = x[i][1];
   }

@@ -22,6 +22,9 @@
 // TMEM: S_A, S_B (P over them, as 16-bit pairs), O_A, O_B; 512 columns.
 // MMA order per key tile: S_A(j), PV_B(j-1), S_B(j), PV_A(j), so the softmax of
 // one tile runs under the MMAs of the other.
+// A block of at most tile_tokens tokens has no row tile B: its key tiles then
+// alternate between A and B, both over the same Q ("dual"), and the two O are
+// merged in tensor memory at the end.
 //
 // Guard. A masked key has p = 0, but the MMA still multiplies: 0 * inf = NaN
 // would reach rows of other requests. So V tiles in which some row drops a key
@@ -69,7 +72,8 @@ struct Layout {
   static constexpr uint32_t kSlotOff = 2 * kTileBytes;  // after Q_A, Q_B
   static constexpr uint32_t kStageOff = kSlotOff + kSlots * kTileBytes;
   static constexpr uint32_t kEpiOff = kStageOff + kStages * (kTileBytes / 2);
-  static constexpr uint32_t kBarOff = kEpiOff + 8 * 2048;  // 2 KB for each softmax warp
+  static constexpr uint32_t kStatOff = kEpiOff + 8 * 2048;  // 2 KB for each softmax warp
+  static constexpr uint32_t kBarOff = kStatOff + 2048;      // dual: (m, l) of 256 threads
   enum Bar : int {
     kQFull = 0,
     kQEmpty,
@@ -83,7 +87,9 @@ struct Layout {
     kPLo = kSFull + 2,
     kPHi = kPLo + 2,
     kOFinal = kPHi + 2,
-    kDrain = kOFinal + 2,
+    kStat = kOFinal + 2,   // dual: (m, l) of the warpgroup are in shared memory
+    kTaken = kStat + 2,    // dual: the warpgroup has read both O
+    kDrain = kTaken + 2,
     kNumBars
   };
   static constexpr uint32_t kHolderOff = kBarOff + 8 * kNumBars;
@@ -94,13 +100,14 @@ struct Layout {
   // then finds what there is.
   static constexpr uint32_t kBadOff = kLimitOff + 8;
   static constexpr uint32_t kSmemUsed = kBadOff + 4;
-  static constexpr uint32_t kSmemBytes = kSmemUsed + 1024;  // + alignment
+  static constexpr uint32_t kSmemBytes = kSmemUsed;
   static_assert(kLimitOff % 8 == 0 && kSmemBytes <= 232448, "shared memory budget");
-  // split: O of tile A over Q (64 KB), of tile B over the first two slots, and
-  // (m, l) of the 256 rows where the other form stages its output
+  // split: O of row tile A over Q (64 KB), of B over the first two slots, and
+  // (m, l) of the rows where the other form stages its output
   static constexpr uint32_t kPartOffB = kSlotOff;
 };
 constexpr int kSoftmaxWarp0 = 4;
+constexpr int kMaxSplit = 8;  // CTAs of a cluster (the portable size)
 
 template <bool kBf16>
 __host__ __device__ constexpr uint32_t idesc_16(uint32_t m, uint32_t n, bool b_mn_major) {
@@ -194,11 +201,11 @@ __device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
 
 // Converts a landed raw tile (128 rows of 128 codes) into the slot's swizzled
 // layout. Lane (w, l) takes the 16 codes of unit l % 8 in the rows 16 i + 4 w +
-// l / 8, i < 8; `scale` is the byte of row 16 (l / 4) + 4 w + l % 4. guard: values
+// l / 8, i < 8; `scale` is the byte of row 16 (l / 4) + 4 w + l % 4. kGuard: values
 // that are not finite become 0; returns whether there were any.
-template <bool kBf16, int kFormat>
-__device__ __forceinline__ bool convert_tile(uint32_t stage, uint32_t slot, uint32_t scale,
-                                             bool guard, int w, int lane) {
+template <bool kBf16, int kFormat, bool kGuard>
+__device__ __forceinline__ bool convert_tile(uint32_t stage, uint32_t slot, uint32_t scale, int w,
+                                             int lane) {
   bool bad = false;
   const int u = lane & 7;    // dims 16 u .. 16 u + 15
   const int odd = u >> 2;    // lanes of the second half write their odd unit first (banks)
@@ -209,16 +216,20 @@ __device__ __forceinline__ bool convert_tile(uint32_t stage, uint32_t slot, uint
   const uint32_t at_a = base + (static_cast<uint32_t>((u & 3) * 2 + odd) ^ (r0 & 7)) * 16;
   const uint32_t at_b = base + (static_cast<uint32_t>((u & 3) * 2 + 1 - odd) ^ (r0 & 7)) * 16;
   const uint32_t mine = pair_pow2<kBf16>(static_cast<int>(scale) - 127);
+  // all loads first: they and the stores are kept in order, and a load behind
+  // a store would wait for the conversion before it
+  uint4 raw[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) raw[i] = ld_shared_v4(from + i * 2048);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const uint4 raw = ld_shared_v4(from + i * 2048);
     const uint32_t sc = __shfl_sync(0xffffffffu, mine, i * 4 + (lane >> 3));
-    const uint32_t c[4] = {raw.x, raw.y, raw.z, raw.w};
+    const uint32_t c[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
     uint32_t v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j)
       v[j] = code_pair<kBf16, kFormat == kKvE4M3>((c[j >> 1] >> (16 * (j & 1))) & 0xffffu, sc);
-    if (guard) {
+    if constexpr (kGuard) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = finite_only<kBf16>(v[j], bad);
     }
@@ -396,8 +407,12 @@ __device__ __forceinline__ void prepare_tiles(const PrefixArgs& args, const Shar
           const uint32_t now = scale;
           scale = kv == 0 ? scale_of(tile, 1) : scale_of(next, 0);
           if (!wait(bar(L::kStageFull + g), g_parity, kDevTimeoutSlotFull)) return;
-          const bool bad = convert_tile<kBf16, kFormat>(
-              sbase + L::kStageOff + g * (kTileBytes / 2), slot, now, kv == 1 && guard, w, lane);
+          const uint32_t stage = sbase + L::kStageOff + g * (kTileBytes / 2);
+          bool bad = false;
+          if (kv == 1 && guard)
+            bad = convert_tile<kBf16, kFormat, true>(stage, slot, now, w, lane);
+          else
+            convert_tile<kBf16, kFormat, false>(stage, slot, now, w, lane);
           publish(s, bad, li);  // all lanes have read the raw tile
           if (lane == 0) mbar_arrive(bar(L::kStageEmpty + g));
           if (++g == L::kStages) {
@@ -433,9 +448,12 @@ __global__ void __launch_bounds__(Layout<kFormat>::kThreads, 1)
                             const __grid_constant__ PrefixArgs args) {
   using L = Layout<kFormat>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
-                                             ~static_cast<uintptr_t>(1023));
+  uint8_t* smem = smem_raw;
   const uint32_t sbase = smem_addr(smem);
+  if (sbase & 1023u) {  // the swizzled tiles need it; the same in every CTA
+    if (threadIdx.x == 0) atomicCAS(args.status, 0, kDevSharedLayout);
+    return;
+  }
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + L::kHolderOff);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kAbortOff);
   volatile unsigned long long* wait_limit =
@@ -466,6 +484,8 @@ __global__ void __launch_bounds__(Layout<kFormat>::kThreads, 1)
       mbar_init(bar(L::kPLo + x), 128);
       mbar_init(bar(L::kPHi + x), 128);
       mbar_init(bar(L::kOFinal + x), 1);
+      mbar_init(bar(L::kStat + x), 128);
+      mbar_init(bar(L::kTaken + x), 128);
     }
     mbar_init(bar(L::kDrain), 1);
     *abort_flag = 0;
@@ -581,19 +601,16 @@ __global__ void __launch_bounds__(Layout<kFormat>::kThreads, 1)
     } else if (warp == 1) {
       // -------------------------------------------------------- MMA issuer
       if (lane == 0) {
-        const uint32_t t_s[2] = {tmem, tmem + 128};
-        const uint32_t t_o[2] = {tmem + 256, tmem + 384};
         const uint64_t qa = smem_desc_sw128(sbase, 16, 1024);
-        const uint64_t qbd = qa + (kTileBytes >> 4);
         const uint64_t k_desc0 = smem_desc_sw128(sbase + L::kSlotOff, 16, 1024);
         const uint64_t v_desc0 = smem_desc_sw128(sbase + L::kSlotOff, kHalfBytes, 1024);
         bool ok = true;
         int s = 0;               // slot of the next use
         uint32_t landed = 0;     // bit slot: parity of its next copy
         uint32_t ready = 0;      // bit slot: parity of its next prepared tile
-        uint32_t tA = 0, tB = 0; // parity of tile A's and tile B's next key tile
-        bool have_prev = false;  // PV_B of the previous tile still to issue
-        int prev_v = 0, prev_nk = 8;
+        uint32_t t_par = 0;      // bit x: parity of row tile x's next key tile
+        bool have_prev = false;  // a PV still to issue, of row tile prev_x
+        int prev_x = 1, prev_v = 0, prev_nk = 8;
         bool prev_acc = false, prev_last = false;
         // waits for the tile in slot s, whoever completes it
         auto wait_tile = [&](bool copied, bool prepared) -> bool {
@@ -603,21 +620,28 @@ __global__ void __launch_bounds__(Layout<kFormat>::kThreads, 1)
           return mbar_wait(prepared ? bar(L::kReady + s) : bar(L::kLanded + s), prepared ? r : l,
                            abort_flag, args.status, kDevTimeoutSlotFull, wait_limit);
         };
-        // PV_B of the previous tile, whose P has parity tB ^ 1
+        // PV of row tile x with the V tile in slot v, as P arrives in halves
+        auto run_pv = [&](int x, int v, bool acc, int nk) -> bool {
+          const uint64_t vd = v_desc0 + ((v * kTileBytes) >> 4);
+          const uint32_t o = tmem + 256 + x * 128, p = tmem + x * 128;
+          const uint32_t par = (t_par >> x) & 1u;
+          t_par ^= 1u << x;
+          if (!mbar_wait(bar(L::kPLo + x), par, abort_flag, args.status, kDevTimeoutPFull,
+                         wait_limit))
+            return false;
+          tc_fence_after();
+          issue_pv_part<kBf16>(o, p, vd, acc, nk, 0);
+          if (!mbar_wait(bar(L::kPHi + x), par, abort_flag, args.status, kDevTimeoutPFull,
+                         wait_limit))
+            return false;
+          tc_fence_after();
+          issue_pv_part<kBf16>(o, p, vd, acc, nk, 1);
+          return true;
+        };
         auto issue_prev = [&]() -> bool {
-          const uint64_t vd = v_desc0 + ((prev_v * kTileBytes) >> 4);
-          if (!mbar_wait(bar(L::kPLo + 1), tB ^ 1u, abort_flag, args.status, kDevTimeoutPFull,
-                         wait_limit))
-            return false;
-          tc_fence_after();
-          issue_pv_part<kBf16>(t_o[1], t_s[1], vd, prev_acc, prev_nk, 0);
-          if (!mbar_wait(bar(L::kPHi + 1), tB ^ 1u, abort_flag, args.status, kDevTimeoutPFull,
-                         wait_limit))
-            return false;
-          tc_fence_after();
-          issue_pv_part<kBf16>(t_o[1], t_s[1], vd, prev_acc, prev_nk, 1);
+          if (!run_pv(prev_x, prev_v, prev_acc, prev_nk)) return false;
           tc_commit(bar(L::kSlotEmpty + prev_v));
-          if (prev_last) tc_commit(bar(L::kOFinal + 1));
+          if (prev_last) tc_commit(bar(L::kOFinal + prev_x));
           have_prev = false;
           return true;
         };
@@ -626,6 +650,7 @@ __global__ void __launch_bounds__(Layout<kFormat>::kThreads, 1)
           int tb, te;
           share_tiles<kSplit>(share, item, tb, te);
           const int nx = item.tokens > args.tile_tokens ? 2 : 1;
+          const bool dual = nx == 1;
           int next_info = args.tiles[tb].info;
           // Q is loaded once the last S MMAs of the item before are done; if it
           // is still on its way, the pending PV_B goes first
@@ -639,17 +664,26 @@ __global__ void __launch_bounds__(Layout<kFormat>::kThreads, 1)
             const int width = info & kTileWidthMask;
             const bool converted = L::kConverts && !(info & kTileOwn);
             const bool last = j == te - 1;
+            const int x = dual ? (j - tb) & 1 : 0;
             const int sk = s;
             if (!(ok = wait_tile(!converted, converted))) break;
             s = s + 1 == L::kSlots ? 0 : s + 1;
             tc_fence_after();
             const uint64_t k_desc = k_desc0 + ((sk * kTileBytes) >> 4);
             const uint32_t idesc = idesc_16<kBf16>(128, width, false);
-            issue_qk(t_s[0], qa, k_desc, idesc);
-            tc_commit(bar(L::kSFull + 0));
+            // (the empty asm keeps the compiler from holding sixteen descriptors
+            // of Q in registers through the loop)
+            uint64_t q_now = qa;
+            asm volatile("" : "+l"(q_now));
+            // S of a row tile goes over its P
+            if (have_prev && prev_x == x && !(ok = issue_prev())) break;
+            issue_qk(tmem + x * 128, q_now, k_desc, idesc);
+            tc_commit(bar(L::kSFull + x));
             if (have_prev && !(ok = issue_prev())) break;
             if (nx == 2) {
-              issue_qk(t_s[1], qbd, k_desc, idesc);
+              q_now = qa + (kTileBytes >> 4);
+              asm volatile("" : "+l"(q_now));
+              issue_qk(tmem + 128, q_now, k_desc, idesc);
               tc_commit(bar(L::kSFull + 1));
             }
             tc_commit(bar(L::kSlotEmpty + sk));
@@ -657,29 +691,20 @@ __global__ void __launch_bounds__(Layout<kFormat>::kThreads, 1)
             const int sv = s;
             if (!(ok = wait_tile(!converted, converted || (info & kTileGuard)))) break;
             s = s + 1 == L::kSlots ? 0 : s + 1;
-            const uint64_t vd = v_desc0 + ((sv * kTileBytes) >> 4);
-            if (!(ok = mbar_wait(bar(L::kPLo + 0), tA, abort_flag, args.status, kDevTimeoutPFull,
-                                 wait_limit)))
-              break;
-            tc_fence_after();
-            issue_pv_part<kBf16>(t_o[0], t_s[0], vd, j > tb, width / 16, 0);
-            if (!(ok = mbar_wait(bar(L::kPHi + 0), tA, abort_flag, args.status, kDevTimeoutPFull,
-                                 wait_limit)))
-              break;
-            tc_fence_after();
-            tA ^= 1u;
-            issue_pv_part<kBf16>(t_o[0], t_s[0], vd, j > tb, width / 16, 1);
-            if (last) tc_commit(bar(L::kOFinal + 0));
-            if (nx == 2) {
-              have_prev = true;
-              prev_v = sv;
-              prev_acc = j > tb;
-              prev_nk = width / 16;
-              prev_last = last;
-              tB ^= 1u;
+            if (dual) {
+              prev_x = x;
+              prev_acc = j - tb >= 2;
+              prev_last = j + 2 >= te;
             } else {
-              tc_commit(bar(L::kSlotEmpty + sv));
+              if (!(ok = run_pv(0, sv, j > tb, width / 16))) break;
+              if (last) tc_commit(bar(L::kOFinal + 0));
+              prev_x = 1;
+              prev_acc = j > tb;
+              prev_last = last;
             }
+            have_prev = true;
+            prev_v = sv;
+            prev_nk = width / 16;
           }
         }
         if (ok && have_prev) ok = issue_prev();
@@ -707,21 +732,30 @@ __global__ void __launch_bounds__(Layout<kFormat>::kThreads, 1)
     const float scale = args.scale_log2;
     const int token = row / args.group;  // of this row in its tile
     bool ok = true;
-    int t = 0, lx = 0;  // key tiles and items of this row tile so far
+    // parities of this warpgroup's next key tile (bit 0), item with any (1) and
+    // dual item (2)
+    uint32_t ph = 0;
     for (int it = share.beg, li = 0; ok && it < share.end; ++it, ++li) {
-      const PrefixItem item = args.items[it];
-      int tb, te;
-      share_tiles<kSplit>(share, item, tb, te);
-      if (x == 1 && item.tokens <= args.tile_tokens) continue;  // no tile B
-      const bool valid = row < tile_rows && x * args.tile_tokens + token < item.tokens;
+      // (what only the epilogue needs is read again there: registers)
+      int tb, te, first_token, tokens;
       PrefixRow mine = {0, -1};
-      if (valid) mine = args.rows[item.row0 + x * args.tile_tokens + token];
+      {
+        const PrefixItem item = args.items[it];
+        share_tiles<kSplit>(share, item, tb, te);
+        tokens = item.tokens;
+        first_token = tokens <= args.tile_tokens ? 0 : x * args.tile_tokens;
+        if (row < tile_rows && first_token + token < tokens)
+          mine = args.rows[item.row0 + first_token + token];
+      }
+      // dual: one row tile only, A takes its even key tiles and B its odd ones
+      const bool dual = tokens <= args.tile_tokens;
+      const int j0 = dual ? tb + x : tb, step = dual ? 2 : 1;
       float m_run = -INFINITY, l_run = 0.f;
-      PrefixTile next = args.tiles[tb];
-      for (int j = tb; j < te; ++j, ++t) {
+      PrefixTile next = args.tiles[j0 < te ? j0 : tb];
+      for (int j = j0; j < te; j += step, ph ^= 1u) {
         const PrefixTile tile = next;
-        next = args.tiles[j + 1 < te ? j + 1 : j];
-        if (!(ok = mbar_wait(bar(L::kSFull + x), t & 1, abort_flag, args.status, kDevTimeoutSFull,
+        next = args.tiles[j + step < te ? j + step : j];
+        if (!(ok = mbar_wait(bar(L::kSFull + x), ph & 1u, abort_flag, args.status, kDevTimeoutSFull,
                              wait_limit)))
           break;
         tc_fence_after();
@@ -755,7 +789,7 @@ __global__ void __launch_bounds__(Layout<kFormat>::kThreads, 1)
         const float m_new = fmaxf(m_run, tmax);
         bool need = false;
         float f = 1.f;
-        if (j == tb) {
+        if (j == j0) {
           m_run = m_new;
         } else if (m_new > m_run + 8.f) {
           // lazy rescale: P stays <= 2^8 against a maximum that is out of date
@@ -800,54 +834,88 @@ __global__ void __launch_bounds__(Layout<kFormat>::kThreads, 1)
         l_run += sum;
         mbar_arrive(bar(L::kPHi + x));
       }
-      // Epilogue.
-      if (!ok || !(ok = mbar_wait(bar(L::kOFinal + x), lx & 1, abort_flag, args.status,
-                                  kDevTimeoutOFinal, wait_limit)))
-        break;
-      ++lx;
-      tc_fence_after();
-      const bool aside = valid && *bad_item > li;
-      if constexpr (kSplit) {
-        // f32 rows of 512 bytes, their 16-byte units swizzled by the row. Tile A's
-        // Q rows and tile B's are read no more, nor are, at the end of tile B,
-        // any slots.
-        const uint32_t dst = sbase + x * L::kPartOffB + row * 512;
+      // Epilogue. (m, l) of a warpgroup without tiles stay (-inf, 0).
+      if (!ok) break;
+      const PrefixItem item = args.items[it];
+      if (j0 < te) {
+        if (!(ok = mbar_wait(bar(L::kOFinal + x), (ph >> 1) & 1u, abort_flag, args.status,
+                             kDevTimeoutOFinal, wait_limit)))
+          break;
+        ph ^= 2u;
+        tc_fence_after();
+      }
+      // o = w * (own O) + w2 * (the other's); dual: both warpgroups have the same
+      // lanes of tensor memory, so each merges half of the dims
+      float w = 1.f, w2 = 0.f;
+      bool both = false;
+      if (dual) {
+        float2* stat = reinterpret_cast<float2*>(smem + L::kStatOff);
+        stat[x * 128 + row] = make_float2(m_run, l_run);
+        tc_fence_before();
+        mbar_arrive(bar(L::kStat + x));
+        if (!(ok = mbar_wait(bar(L::kStat + (x ^ 1)), (ph >> 2) & 1u, abort_flag, args.status,
+                             kDevTimeoutOFinal, wait_limit)))
+          break;
+        tc_fence_after();
+        const float2 ml = stat[(x ^ 1) * 128 + row];
+        const float m = fmaxf(m_run, ml.x);
+        w = m_run == -INFINITY ? 0.f : ex2(m_run - m);
+        w2 = ml.x == -INFINITY ? 0.f : ex2(ml.x - m);
+        l_run = w * l_run + w2 * ml.y;
+        m_run = m;
+        both = te - tb > 1;
+      }
+      const bool aside = mine.hi >= 0 && *bad_item > li;  // (a row that exists keeps itself)
+      const float inv_l = 1.f / l_run;
+      const int chunks = dual ? 2 : 4, c0 = dual ? 2 * x : 0;
+      const uint32_t stage = sbase + L::kEpiOff + (warp - kSoftmaxWarp0) * 2048;
+      // split: f32 rows of 512 bytes, their 16-byte units swizzled by the row: of
+      // tile A over Q, of B over the first slots (at A's end Q is read no more,
+      // at B's no slot is)
+      const uint32_t part = sbase + (dual ? 0 : x) * L::kPartOffB + row * 512;
 #pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          uint32_t o[32];
+      for (int c = c0; c < c0 + chunks; ++c) {
+        uint32_t o[32];
+        if (dual) {
+          // (a warpgroup without tiles has no O of its own: n == 1, and x == 1)
+          uint32_t o2[32];
+          tmem_ld32((j0 < te ? t_o : t_lane + 256) + 32 * c, o);
+          if (both) tmem_ld32(t_lane + 256 + (x ^ 1) * 128 + 32 * c, o2);
+          tmem_wait_ld();
+          reg_fence32(o);
+          const float a = j0 < te ? w : w2;
+          if (both) {
+            reg_fence32(o2);
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              o[i] = __float_as_uint(fmaf(__uint_as_float(o2[i]), w2, __uint_as_float(o[i]) * a));
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a);
+          }
+          if (c == c0 + 1) {
+            tc_fence_before();
+            mbar_arrive(bar(L::kTaken + x));
+          }
+        } else {
           tmem_ld32(t_o + 32 * c, o);
           tmem_wait_ld();
           reg_fence32(o);
-          if (aside) {
-            const Aside s = find_aside<kBf16, kFormat>(args, tb, te, mine, item.head, c);
+        }
+        if (aside) {
+          const Aside s = find_aside<kBf16, kFormat>(args, tb, te, mine, item.head, c);
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              o[i] = __float_as_uint(with_aside(__uint_as_float(o[i]), s, i));
-          }
+          for (int i = 0; i < 32; ++i)
+            o[i] = __float_as_uint(with_aside(__uint_as_float(o[i]), s, i));
+        }
+        if constexpr (kSplit) {
 #pragma unroll
           for (int v = 0; v < 8; ++v)
-            st_shared_v4(dst + (static_cast<uint32_t>(c * 8 + v) ^ lane) * 16, o[4 * v],
+            st_shared_v4(part + (static_cast<uint32_t>(c * 8 + v) ^ lane) * 16, o[4 * v],
                          o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
-        }
-        *reinterpret_cast<float2*>(smem + L::kEpiOff + (x * 128 + row) * 8) =
-            make_float2(m_run, l_run);
-      } else {
-        // 32 dims at a time: the warp's 32 rows of 64 bytes through its 2 KB,
-        // out as 64-byte runs, eight rows an instruction
-        const float inv_l = 1.f / l_run;
-        const uint32_t stage = sbase + L::kEpiOff + (warp - kSoftmaxWarp0) * 2048;
-#pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          uint32_t o[32];
-          tmem_ld32(t_o + 32 * c, o);
-          tmem_wait_ld();
-          reg_fence32(o);
-          if (aside) {
-            const Aside s = find_aside<kBf16, kFormat>(args, tb, te, mine, item.head, c);
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              o[i] = __float_as_uint(with_aside(__uint_as_float(o[i]), s, i));
-          }
+        } else {
+          // 32 dims at a time: the warp's 32 rows of 64 bytes through its 2 KB,
+          // out as 64-byte runs, eight rows an instruction
           __syncwarp();  // the chunk before has been read
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
@@ -865,7 +933,7 @@ __global__ void __launch_bounds__(Layout<kFormat>::kThreads, 1)
           for (int i = 0; i < 4; ++i) {
             const int rw = 8 * i + (lane >> 2), r = sub * 32 + rw;
             const int rt = r / args.group, rh = r - rt * args.group;
-            const int tok = x * args.tile_tokens + rt;
+            const int tok = first_token + rt;
             const uint4 v =
                 ld_shared_v4(stage + rw * 64 + ((lane & 3) ^ ((rw >> 1) & 3)) * 16);
             if (r < tile_rows && tok < item.tokens)
@@ -876,8 +944,18 @@ __global__ void __launch_bounds__(Layout<kFormat>::kThreads, 1)
                                         c * 32 + (lane & 3) * 8) = v;
           }
         }
-        tc_fence_before();
-        __syncwarp();
+      }
+      if (kSplit && !(dual && x == 1))
+        *reinterpret_cast<float2*>(smem + L::kEpiOff + ((dual ? 0 : x) * 128 + row) * 8) =
+            make_float2(m_run, l_run);
+      tc_fence_before();
+      __syncwarp();
+      if (dual) {
+        // the next item's P, and with it PV over O, only once both have read O
+        if (!(ok = mbar_wait(bar(L::kTaken + (x ^ 1)), (ph >> 2) & 1u, abort_flag, args.status,
+                             kDevTimeoutOFinal, wait_limit)))
+          break;
+        ph ^= 4u;
       }
     }
   }
@@ -890,48 +968,61 @@ __global__ void __launch_bounds__(Layout<kFormat>::kThreads, 1)
     cluster_sync();
     if (warp >= kSoftmaxWarp0 && warp < kSoftmaxWarp0 + 8) {
       const PrefixItem item = args.items[share.beg];
-      const int rows = item.tokens > args.tile_tokens ? 256 : 128;
+      const int rows = item.tokens * args.group;  // of the block, those of B after A's
       const int per = (rows + share.ranks - 1) / share.ranks;
-      for (int i = warp - kSoftmaxWarp0; i < per; i += 8) {
-        const int r = share.rank * per + i;  // of the block's 128 or 256
-        const int x = r >> 7, rr = r & 127;
-        const int rt = rr / args.group, rh = rr - rt * args.group;
-        const int tok = x * args.tile_tokens + rt;
-        if (r >= rows || rr >= tile_rows || tok >= item.tokens) continue;
-        float2 ml = make_float2(-INFINITY, 0.f);
-        if (lane < share.ranks)
-          ml = ld_cluster_v2(mapa_shared(sbase + L::kEpiOff + r * 8, lane));
-        float m = ml.x;
+      const int end = min(rows, share.rank * per + per);
+      // two rows at a time, all their loads in flight together
+      for (int i = share.rank * per + (warp - kSoftmaxWarp0) * 2; i < end; i += 16) {
+        float2 ml[2];
+        float4 v[2][kMaxSplit];
+        int rr[2], x[2];
 #pragma unroll
-        for (int o = 4; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        m = __shfl_sync(0xffffffffu, m, 0);
-        const float w = ml.x == -INFINITY ? 0.f : ex2(ml.x - m);
-        float l = w * ml.y;
+        for (int h = 0; h < 2; ++h) {
+          const int r = min(i + h, end - 1);
+          x[h] = r >= tile_rows ? 1 : 0;
+          rr[h] = r - x[h] * tile_rows;
+          ml[h] = make_float2(-INFINITY, 0.f);
+          if (lane < share.ranks)
+            ml[h] = ld_cluster_v2(
+                mapa_shared(sbase + L::kEpiOff + (x[h] * 128 + rr[h]) * 8, lane));
+          const uint32_t at = sbase + x[h] * L::kPartOffB + rr[h] * 512 +
+                              (static_cast<uint32_t>(lane) ^ (rr[h] & 31)) * 16;
 #pragma unroll
-        for (int o = 4; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-        l = __shfl_sync(0xffffffffu, l, 0);
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        const uint32_t at =
-            sbase + x * L::kPartOffB + rr * 512 + (static_cast<uint32_t>(lane) ^ (rr & 31)) * 16;
-        for (int k = 0; k < share.ranks; ++k) {
-          const float wk = __shfl_sync(0xffffffffu, w, k);
-          const float4 v = ld_cluster_v4(mapa_shared(at, k));
-          if (wk != 0.f) {  // a rank in which the row keeps nothing adds nothing
-            acc.x = fmaf(wk, v.x, acc.x);
-            acc.y = fmaf(wk, v.y, acc.y);
-            acc.z = fmaf(wk, v.z, acc.z);
-            acc.w = fmaf(wk, v.w, acc.w);
-          }
+          for (int k = 0; k < kMaxSplit; ++k)
+            if (k < share.ranks) v[h][k] = ld_cluster_v4(mapa_shared(at, k));
         }
-        const float inv_l = 1.f / l;
-        uint2 y;
-        y.x = pack2<kBf16>(acc.x * inv_l, acc.y * inv_l);
-        y.y = pack2<kBf16>(acc.z * inv_l, acc.w * inv_l);
-        *reinterpret_cast<uint2*>(args.out +
-                                  (static_cast<int64_t>(item.row0 + tok) * args.q_heads +
-                                   item.head * args.group + rh) *
-                                      kHeadDim +
-                                  lane * 4) = y;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (i + h >= end) break;
+          float m = ml[h].x;
+#pragma unroll
+          for (int o = 4; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+          m = __shfl_sync(0xffffffffu, m, 0);
+          const float w = ml[h].x == -INFINITY ? 0.f : ex2(ml[h].x - m);
+          float l = w * ml[h].y;
+#pragma unroll
+          for (int o = 4; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+          l = __shfl_sync(0xffffffffu, l, 0);
+          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int k = 0; k < kMaxSplit; ++k) {
+            if (k >= share.ranks) break;
+            const float wk = __shfl_sync(0xffffffffu, w, k);
+            acc.x = fmaf(wk, v[h][k].x, acc.x);
+            acc.y = fmaf(wk, v[h][k].y, acc.y);
+            acc.z = fmaf(wk, v[h][k].z, acc.z);
+            acc.w = fmaf(wk, v[h][k].w, acc.w);
+          }
+          const float inv_l = 1.f / l;
+          uint2 y;
+          y.x = pack2<kBf16>(acc.x * inv_l, acc.y * inv_l);
+          y.y = pack2<kBf16>(acc.z * inv_l, acc.w * inv_l);
+          const int rt = rr[h] / args.group, rh = rr[h] - rt * args.group;
+          const int64_t tok = item.row0 + x[h] * args.tile_tokens + rt;
+          *reinterpret_cast<uint2*>(
+              args.out + (tok * args.q_heads + item.head * args.group + rh) * kHeadDim +
+              lane * 4) = y;
+        }
       }
     }
     __syncwarp();
@@ -994,6 +1085,27 @@ cudaError_t launch_typed(const PrefixMaps& m, const PrefixArgs& a, int format, i
 }
 
 }  // namespace
+
+int prefix_active_clusters(int splits) {
+  using L = Layout<kKvInt8>;
+  auto kernel = prefix_attention_kernel<false, kKvInt8, true>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmemBytes) !=
+      cudaSuccess)
+    return 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(splits);
+  cfg.blockDim = dim3(L::kThreads);
+  cfg.dynamicSmemBytes = L::kSmemBytes;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = static_cast<unsigned>(splits);
+  attr.val.clusterDim.y = 1;
+  attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  return cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) == cudaSuccess ? n : 0;
+}
 
 cudaError_t launch_prefix_attention(const PrefixMaps& maps, const PrefixArgs& args, int bf16,
                                     int format, int grid, cudaStream_t stream) {

@@ -31,6 +31,9 @@ struct PrefixArgs {
   unsigned long long wait_ns;
 };
 
+// Clusters of `splits` CTAs that run at one time on the current device.
+int prefix_active_clusters(int splits);
+
 cudaError_t launch_prefix_attention(const PrefixMaps& maps, const PrefixArgs& args, int bf16,
                                     int format, int grid, cudaStream_t stream);
 

@@ -52,14 +52,16 @@ struct PrefixRow {
 struct PrefixShape {
   int batch, q_heads, kv_heads, prefix_len, sparse, sparse_prefix, window;
   int tile_tokens;   // tokens of one 128-row tile: 128 / (q_heads / kv_heads)
-  int block_tokens;  // 2 * tile_tokens
+  int block_tokens;  // of a block: tile_tokens or 2 * tile_tokens
 };
 
 struct PrefixWork {
   std::vector<PrefixItem> items;  // without the head; one per block
   std::vector<PrefixTile> tiles;
   std::vector<PrefixRow> rows;
-  std::vector<double> cost;       // of an item, in 128-key tiles
+  std::vector<double> cost;       // of an item: periods of one key tile for two row tiles
+  // prefix keys that no tile reaches: [gap_beg, gap_end)
+  int gap_beg = 0, gap_end = 0;
 };
 
 inline int prefix_tile_width(int keys) { return std::min(128, (keys + 15) / 16 * 16); }
@@ -97,6 +99,9 @@ inline PrefixWork build_prefix_work(const PrefixShape& s, const int32_t* cu_q,
       request_of[cu_q[b] + i] = b;
     }
   }
+  // tiles begin at the first key of a span, and reach at most 128 keys on
+  w.gap_beg = s.sparse ? std::min(P, (s.sparse_prefix + 127) / 128 * 128) : P;
+  w.gap_end = P;
   struct Segment {  // the rows of one request inside a block
     int lo, first_hi, last_hi;
   };
@@ -126,7 +131,7 @@ inline PrefixWork build_prefix_work(const PrefixShape& s, const int32_t* cu_q,
     item.row0 = row0;
     item.tokens = tokens;
     item.tile_beg = static_cast<int>(w.tiles.size());
-    double cost = 0.6;  // what an item costs besides its tiles, in tiles
+    double cost = 0;
     auto emit = [&](int own) {
       int64_t next = 0;
       for (size_t i = 0; i < spans.size();) {
@@ -176,6 +181,8 @@ inline PrefixWork build_prefix_work(const PrefixShape& s, const int32_t* cu_q,
         p_min = std::min<int64_t>(p_min, static_cast<int64_t>(P) + g.first_hi - g.lo);
       add_span(0, std::min<int64_t>(P, s.sparse_prefix));
       add_span(std::max<int64_t>(0, p_min - s.window + 1), P);
+      w.gap_end = static_cast<int>(
+          std::min<int64_t>(w.gap_end, std::max<int64_t>(0, p_min - s.window + 1)));
     }
     emit(0);
     // own keys, request by request (their packed rows ascend)
@@ -192,8 +199,10 @@ inline PrefixWork build_prefix_work(const PrefixShape& s, const int32_t* cu_q,
     emit(1);
     item.tile_end = static_cast<int>(w.tiles.size());
     w.items.push_back(item);
-    w.cost.push_back(cost);
+    // one row tile takes two key tiles a period; 0.6 goes to the item's ends
+    w.cost.push_back(0.6 + (tokens <= s.tile_tokens ? std::max(1.0, cost / 2) : cost));
   }
+  w.gap_end = std::max(w.gap_end, w.gap_beg);
   return w;
 }
 

@@ -29,6 +29,7 @@ enum DeviceError : int {
   kDevTimeoutAccFull = 0x204,
   kDevTimeoutPairSync = 0x205,
   kDevTimeoutSmallGemm = 0x301,
+  kDevSharedLayout = 0x401,  // dynamic shared memory is not 1024-byte aligned
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) {

@@ -25,7 +25,7 @@ import torch
 from . import _lib
 from .attention import (HEAD_DIM, MODE_AUTO, PREFIX, WINDOW, AttentionRun, Context, EncodableRun,
                         _launch, _need, encode_run)
-from .kv_cache import _DTYPES, KVCache
+from .kv_cache import _DTYPES, FORMATS, KVCache
 
 
 _retired: list = []  # lists of plans that ended during a capture
@@ -61,6 +61,8 @@ class PrefixPlan:
         self.queries = cu_q[len(cu_q) - 1]
         self.keys = cu_k[len(cu_k) - 1] if cu_k is not None else self.queries
         self.prefix_len, self.q_heads, self.kv_heads = prefix_len, q_heads, kv_heads
+        fn = self.ctx.lib.qwa_prefix_attention_workspace
+        self.workspace = {name: fn(h, code) for name, code in FORMATS.items()}  # bytes
 
     def close(self) -> None:
         """Release the lists; waits for the device. During a stream capture
@@ -89,7 +91,8 @@ def _packed(t: torch.Tensor, name: str, tokens: int, heads: int, dtype, index: i
     return s0 if tokens > 1 else heads * HEAD_DIM  # a single row has no stride of its own
 
 
-def _attention_args(ctx: Context, plan: PrefixPlan, q, k, v, output, cache, first_slot) -> tuple:
+def _attention_args(ctx: Context, plan: PrefixPlan, q, k, v, output, cache, first_slot):
+    """(workspace or None, the C call's arguments between plan and stream)"""
     dtype, index = q.dtype, ctx.device
     code = _DTYPES.get(dtype)
     _need(code is not None, "q must be float16 or bfloat16")
@@ -98,15 +101,21 @@ def _attention_args(ctx: Context, plan: PrefixPlan, q, k, v, output, cache, firs
     n, hq, m, hk = plan.queries, plan.q_heads, plan.keys, plan.kv_heads
     _need(_packed(output, "output", n, hq, dtype, index) == hq * HEAD_DIM,
           "output must be contiguous")
-    struct = None
+    struct = workspace = None
+    need = 0
     if cache is not None:
         _need(cache.device.index == index, "the cache must be on q's device")
         struct = ctypes.byref(cache.struct)
+        need = plan.workspace[cache.format]
+        if need:
+            workspace = q.new_empty(need, dtype=torch.uint8)
     else:
         _need(plan.prefix_len == 0, "a prefix needs its cache")
-    return (code, q.data_ptr(), _packed(q, "q", n, hq, dtype, index), k.data_ptr(),
-            _packed(k, "k", m, hk, dtype, index), v.data_ptr(),
-            _packed(v, "v", m, hk, dtype, index), output.data_ptr(), struct, first_slot)
+    return workspace, (
+        code, q.data_ptr(), _packed(q, "q", n, hq, dtype, index), k.data_ptr(),
+        _packed(k, "k", m, hk, dtype, index), v.data_ptr(), _packed(v, "v", m, hk, dtype, index),
+        output.data_ptr(), struct, first_slot,
+        workspace.data_ptr() if workspace is not None else None, need)
 
 
 class PrefixAttentionKernel:
@@ -120,15 +129,17 @@ class PrefixAttentionKernel:
                    first_slot: int = 0) -> AttentionRun:
         """q [queries, q_heads, 128], k, v [own keys, kv_heads, 128] packed
         request after request, output as q, contiguous; the prefix is in the
-        cache's slots ``first_slot`` .. ``first_slot + plan.prefix_len - 1``."""
-        args = _attention_args(self.ctx, plan, q, k, v, output, cache, first_slot)
+        cache's slots ``first_slot`` .. ``first_slot + plan.prefix_len - 1``. A run
+        with ``owned_buffers`` is issued on one stream at a time."""
+        workspace, args = _attention_args(self.ctx, plan, q, k, v, output, cache, first_slot)
         lib, h = self.ctx.lib, self.ctx.handle
 
         def launch(stream):
             _need(plan.handle is not None, "the plan is closed")
             return lib.qwa_prefix_attention(h, plan.handle, *args, stream)
 
-        return AttentionRun([EncodableRun(launch, self.ctx, "shared-prefix attention")])
+        return AttentionRun([EncodableRun(launch, self.ctx, "shared-prefix attention")],
+                            [workspace] if workspace is not None else [])
 
     def encode(self, stream, run: AttentionRun) -> None:
         for command in run.commands:
@@ -191,8 +202,12 @@ def prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     plan = _plan_for(ctx, tuple(cu_seqlens),
                      tuple(cu_seqlens_k) if cu_seqlens_k is not None else None, prefix_len,
                      q_shape[1], k_shape[1], mode, sparse_prefix, window)
-    args = _attention_args(ctx, plan, q, k, v, out, cache, first_slot)
+    workspace, args = _attention_args(ctx, plan, q, k, v, out, cache, first_slot)
     _launch(ctx, stream, ctx.lib.qwa_prefix_attention, plan.handle, *args)
+    if workspace is not None and stream is not None:
+        # its memory must not be handed out again before that stream is done with it
+        workspace.record_stream(stream if isinstance(stream, torch.cuda.Stream) else
+                                torch.cuda.ExternalStream(int(stream), device=q.device))
     return out
 
 

@@ -1,6 +1,6 @@
 // Checks the work lists of csrc/prefix_plan.h against the keep rule, pair by
-// pair. Arguments: P sparse sparse_prefix window group, then n m of each
-// request. Prints what is wrong and exits 1, or the numbers of kept pairs and
+// pair. Arguments: P sparse sparse_prefix window group row_tiles (1 or 2), then
+// n m of each request. Prints what is wrong and exits 1, or the numbers of kept pairs and
 // of tiles.
 #include <cstdio>
 #include <cstdlib>
@@ -26,15 +26,17 @@ int main(int argc, char** argv) {
   s.kv_heads = 1;
   s.q_heads = group;
   s.tile_tokens = 128 / group;
-  s.block_tokens = 2 * s.tile_tokens;
+  s.block_tokens = std::atoi(argv[6]) * s.tile_tokens;
   std::vector<int> cu_q(1, 0), cu_k(1, 0);
-  for (int i = 6; i + 1 < argc; i += 2) {
+  for (int i = 7; i + 1 < argc; i += 2) {
     cu_q.push_back(cu_q.back() + std::atoi(argv[i]));
     cu_k.push_back(cu_k.back() + std::atoi(argv[i + 1]));
   }
   s.batch = static_cast<int>(cu_q.size()) - 1;
   const int P = s.prefix_len, total_k = cu_k.back(), total_q = cu_q.back();
   const PrefixWork w = build_prefix_work(s, cu_q.data(), cu_k.data());
+  if (total_q && (w.gap_beg < 0 || w.gap_end < w.gap_beg || w.gap_end > P))
+    return wrong("gap", w.gap_beg, w.gap_end);
   std::vector<int> seen_rows(total_q, 0);
   long pairs = 0;
   for (const PrefixItem& it : w.items) {
@@ -67,6 +69,8 @@ int main(int argc, char** argv) {
         const int limit = own ? total_k : P;
         if (width < 16 || width > 128 || width % 16) return wrong("width", r, width);
         if (t.key < 0 || t.key >= limit) return wrong("tile outside", r, t.key);
+        if (!own && t.key < w.gap_end && std::min(t.key + width, P) > w.gap_beg)
+          return wrong("tile in the gap", r, t.key);
         for (int c = 0; c < 128; ++c) {
           const long key = t.key + c;
           const bool keep = keeps(own, key);

@@ -23,11 +23,13 @@ def checker(tmp_path_factory):
 
 
 def check(exe, prefix, sparse, sparse_prefix, window, group, requests):
-    args = [prefix, sparse, sparse_prefix, window, group]
-    for n, m in requests:
-        args += [n, m]
-    out = subprocess.run([exe] + [str(a) for a in args], capture_output=True, text=True)
-    assert out.returncode == 0, (args, out.stdout)
+    """[kept pairs, tiles] of blocks of two row tiles; blocks of one are checked too."""
+    for row_tiles in (1, 2):
+        args = [prefix, sparse, sparse_prefix, window, group, row_tiles]
+        for n, m in requests:
+            args += [n, m]
+        out = subprocess.run([exe] + [str(a) for a in args], capture_output=True, text=True)
+        assert out.returncode == 0, (args, out.stdout)
     return [int(x) for x in out.stdout.split()]
 
 
