@@ -1356,13 +1356,14 @@ PrefixDeal prefix_deal(qwa_ctx* ctx, const PrefixWork& w, const PrefixShape& s) 
     ctx->clusters[1] = ctx->sms;
     for (int i = 2; i <= kMaxSplits; ++i) ctx->clusters[i] = prefix_active_clusters(i);
   }
+  const bool one_tile = s.block_tokens == s.tile_tokens;
   const int rows = tokens * (s.q_heads / s.kv_heads);
   const double merge = 0.8 + rows / 128.0;
   for (int n = 2; n <= std::min(kMaxSplits, least); ++n) {
     if (ctx->clusters[n] < 1) continue;
     const int64_t rounds = (items + ctx->clusters[n] - 1) / ctx->clusters[n];
     const int share = (most + n - 1) / n;
-    const double cost = rounds * ((tokens <= s.tile_tokens ? (share + 1) / 2 : share) + 0.6 + merge) +
+    const double cost = rounds * ((one_tile ? (share + 1) / 2 : share) + 0.6 + merge) +
                         (rounds - 1) * 2.0;
     if (cost < best.cost) {
       best.splits = n;
@@ -1384,8 +1385,7 @@ qwa_status create_prefix_plan(qwa_ctx* ctx, const int32_t* cu_q, const int32_t* 
     // work where there are few.
     w = build_prefix_work(shape, cu_q, cu_k);
     PrefixDeal deal = prefix_deal(ctx, w, shape);
-    if (static_cast<int64_t>(w.items.size()) * shape.kv_heads < 2 * ctx->sms &&
-        plan->total_q > shape.tile_tokens) {
+    if (static_cast<int64_t>(w.items.size()) * shape.kv_heads < 2 * ctx->sms) {
       PrefixShape low = shape;
       low.block_tokens = shape.tile_tokens;
       PrefixWork w_low = build_prefix_work(low, cu_q, cu_k);
@@ -1616,6 +1616,7 @@ qwa_status qwa_prefix_attention(qwa_ctx* ctx, const qwa_prefix_plan* plan, int d
   a.rows = plan->rows;
   a.cta_offsets = plan->offsets;
   a.splits = plan->splits;
+  a.one_tile = s.block_tokens == s.tile_tokens;
   a.v_own = static_cast<const uint16_t*>(v);
   a.v_stride = v_stride;
   a.out = static_cast<uint16_t*>(out);

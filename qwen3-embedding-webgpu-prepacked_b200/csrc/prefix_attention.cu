@@ -22,9 +22,10 @@
 // TMEM: S_A, S_B (P over them, as 16-bit pairs), O_A, O_B; 512 columns.
 // MMA order per key tile: S_A(j), PV_B(j-1), S_B(j), PV_A(j), so the softmax of
 // one tile runs under the MMAs of the other.
-// A block of at most tile_tokens tokens has no row tile B: its key tiles then
-// alternate between A and B, both over the same Q ("dual"), and the two O are
-// merged in tensor memory at the end.
+// In the dual form (few blocks: each has one row tile) the key tiles of a block
+// alternate between A and B, both over the same Q, and the two O are merged in
+// tensor memory at the end. It has kernels of its own: with both forms in one, the
+// softmax warps spilled registers (4 x 5000 tokens 3% slower).
 //
 // Guard. A masked key has p = 0, but the MMA still multiplies: 0 * inf = NaN
 // would reach rows of other requests. So V tiles in which some row drops a key
@@ -267,7 +268,7 @@ struct Aside {
   uint32_t pos, neg, nan;
 };
 template <bool kBf16, int kFormat>
-__device__ __noinline__ Aside find_aside(const PrefixArgs& a, int tile_beg, int tile_end,
+__device__ __forceinline__ Aside find_aside(const PrefixArgs& a, int tile_beg, int tile_end,
                                          PrefixRow row, int head, int chunk) {
   Aside s{0u, 0u, 0u};
   for (int j = tile_beg; j < tile_end; ++j) {
@@ -311,6 +312,31 @@ __device__ __forceinline__ float with_aside(float o, const Aside& s, int d) {
   if ((s.pos >> d) & 1u) o += INFINITY;
   if ((s.neg >> d) & 1u) o -= INFINITY;
   return o;
+}
+
+// Puts them back into O in tensor memory (chunks [c_beg, c_end) at t_o) for the
+// lanes with `mine`. Out of line: it is rare, and its registers are not the
+// epilogue's.
+template <bool kBf16, int kFormat>
+__device__ __noinline__ void put_back(const PrefixArgs& a, int tile_beg, int tile_end,
+                                      PrefixRow row, int head, int c_beg, int c_end, uint32_t t_o,
+                                      bool mine) {
+#pragma unroll 1
+  for (int c = c_beg; c < c_end; ++c) {
+    uint32_t o[32];
+    tmem_ld32(t_o + 32 * c, o);
+    tmem_wait_ld();
+    reg_fence32(o);
+    if (mine) {
+      const Aside s = find_aside<kBf16, kFormat>(a, tile_beg, tile_end, row, head, c);
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        o[i] = __float_as_uint(with_aside(__uint_as_float(o[i]), s, i));
+    }
+    __syncwarp();
+    tmem_st32(t_o + 32 * c, o);
+    tmem_wait_st();
+  }
 }
 
 __device__ __forceinline__ float4 ld_cluster_v4(uint32_t addr) {
@@ -438,7 +464,8 @@ __device__ __forceinline__ void prepare_tiles(const PrefixArgs& args, const Shar
   }
 }
 
-template <bool kBf16, int kFormat, bool kSplit>
+// kDual: every block has one row tile (block_tokens == tile_tokens).
+template <bool kBf16, int kFormat, bool kSplit, bool kDual>
 __global__ void __launch_bounds__(Layout<kFormat>::kThreads, 1)
     prefix_attention_kernel(const __grid_constant__ CUtensorMap tm_q,
                             const __grid_constant__ CUtensorMap tm_k,
@@ -639,9 +666,9 @@ __global__ void __launch_bounds__(Layout<kFormat>::kThreads, 1)
           return true;
         };
         auto issue_prev = [&]() -> bool {
-          if (!run_pv(prev_x, prev_v, prev_acc, prev_nk)) return false;
+          if (!run_pv(kDual ? prev_x : 1, prev_v, prev_acc, prev_nk)) return false;
           tc_commit(bar(L::kSlotEmpty + prev_v));
-          if (prev_last) tc_commit(bar(L::kOFinal + prev_x));
+          if (prev_last) tc_commit(bar(L::kOFinal + (kDual ? prev_x : 1)));
           have_prev = false;
           return true;
         };
@@ -650,7 +677,6 @@ __global__ void __launch_bounds__(Layout<kFormat>::kThreads, 1)
           int tb, te;
           share_tiles<kSplit>(share, item, tb, te);
           const int nx = item.tokens > args.tile_tokens ? 2 : 1;
-          const bool dual = nx == 1;
           int next_info = args.tiles[tb].info;
           // Q is loaded once the last S MMAs of the item before are done; if it
           // is still on its way, the pending PV_B goes first
@@ -664,7 +690,7 @@ __global__ void __launch_bounds__(Layout<kFormat>::kThreads, 1)
             const int width = info & kTileWidthMask;
             const bool converted = L::kConverts && !(info & kTileOwn);
             const bool last = j == te - 1;
-            const int x = dual ? (j - tb) & 1 : 0;
+            const int x = kDual ? (j - tb) & 1 : 0;
             const int sk = s;
             if (!(ok = wait_tile(!converted, converted))) break;
             s = s + 1 == L::kSlots ? 0 : s + 1;
@@ -676,11 +702,11 @@ __global__ void __launch_bounds__(Layout<kFormat>::kThreads, 1)
             uint64_t q_now = qa;
             asm volatile("" : "+l"(q_now));
             // S of a row tile goes over its P
-            if (have_prev && prev_x == x && !(ok = issue_prev())) break;
+            if (kDual && have_prev && prev_x == x && !(ok = issue_prev())) break;
             issue_qk(tmem + x * 128, q_now, k_desc, idesc);
             tc_commit(bar(L::kSFull + x));
             if (have_prev && !(ok = issue_prev())) break;
-            if (nx == 2) {
+            if (!kDual && nx == 2) {
               q_now = qa + (kTileBytes >> 4);
               asm volatile("" : "+l"(q_now));
               issue_qk(tmem + 128, q_now, k_desc, idesc);
@@ -691,14 +717,17 @@ __global__ void __launch_bounds__(Layout<kFormat>::kThreads, 1)
             const int sv = s;
             if (!(ok = wait_tile(!converted, converted || (info & kTileGuard)))) break;
             s = s + 1 == L::kSlots ? 0 : s + 1;
-            if (dual) {
+            if (kDual) {
               prev_x = x;
               prev_acc = j - tb >= 2;
               prev_last = j + 2 >= te;
             } else {
               if (!(ok = run_pv(0, sv, j > tb, width / 16))) break;
               if (last) tc_commit(bar(L::kOFinal + 0));
-              prev_x = 1;
+              if (nx == 1) {
+                tc_commit(bar(L::kSlotEmpty + sv));
+                continue;
+              }
               prev_acc = j > tb;
               prev_last = last;
             }
@@ -743,13 +772,14 @@ __global__ void __launch_bounds__(Layout<kFormat>::kThreads, 1)
         const PrefixItem item = args.items[it];
         share_tiles<kSplit>(share, item, tb, te);
         tokens = item.tokens;
-        first_token = tokens <= args.tile_tokens ? 0 : x * args.tile_tokens;
+        if (!kDual && x == 1 && tokens <= args.tile_tokens) continue;  // no row tile B
+        first_token = kDual ? 0 : x * args.tile_tokens;
         if (row < tile_rows && first_token + token < tokens)
           mine = args.rows[item.row0 + first_token + token];
       }
-      // dual: one row tile only, A takes its even key tiles and B its odd ones
-      const bool dual = tokens <= args.tile_tokens;
-      const int j0 = dual ? tb + x : tb, step = dual ? 2 : 1;
+      // dual: A takes the even key tiles, B the odd ones
+      const int j0 = kDual ? tb + x : tb;
+      constexpr int step = kDual ? 2 : 1;
       float m_run = -INFINITY, l_run = 0.f;
       PrefixTile next = args.tiles[j0 < te ? j0 : tb];
       for (int j = j0; j < te; j += step, ph ^= 1u) {
@@ -837,6 +867,10 @@ __global__ void __launch_bounds__(Layout<kFormat>::kThreads, 1)
       // Epilogue. (m, l) of a warpgroup without tiles stay (-inf, 0).
       if (!ok) break;
       const PrefixItem item = args.items[it];
+      // (the empty asm keeps what follows from group and lane out of registers
+      // that the tile loop needs)
+      int group = args.group, ln = lane;
+      asm volatile("" : "+r"(group), "+r"(ln));
       if (j0 < te) {
         if (!(ok = mbar_wait(bar(L::kOFinal + x), (ph >> 1) & 1u, abort_flag, args.status,
                              kDevTimeoutOFinal, wait_limit)))
@@ -848,7 +882,7 @@ __global__ void __launch_bounds__(Layout<kFormat>::kThreads, 1)
       // lanes of tensor memory, so each merges half of the dims
       float w = 1.f, w2 = 0.f;
       bool both = false;
-      if (dual) {
+      if constexpr (kDual) {
         float2* stat = reinterpret_cast<float2*>(smem + L::kStatOff);
         stat[x * 128 + row] = make_float2(m_run, l_run);
         tc_fence_before();
@@ -867,19 +901,29 @@ __global__ void __launch_bounds__(Layout<kFormat>::kThreads, 1)
       }
       const bool aside = mine.hi >= 0 && *bad_item > li;  // (a row that exists keeps itself)
       const float inv_l = 1.f / l_run;
-      const int chunks = dual ? 2 : 4, c0 = dual ? 2 * x : 0;
+      const int chunks = kDual ? 2 : 4, c0 = kDual ? 2 * x : 0;
       const uint32_t stage = sbase + L::kEpiOff + (warp - kSoftmaxWarp0) * 2048;
+      // own O (a warpgroup without tiles, B of one key tile, has A's), and what
+      // the guard put aside back into the O of the larger weight
+      const uint32_t t_own = j0 < te ? t_o : t_lane + 256;
+      if (__any_sync(0xffffffffu, aside)) {
+        const bool to_own = j0 >= te || w >= w2;
+        put_back<kBf16, kFormat>(args, tb, te, mine, item.head, c0, c0 + chunks, t_own,
+                                 aside && to_own);
+        if (both)
+          put_back<kBf16, kFormat>(args, tb, te, mine, item.head, c0, c0 + chunks,
+                                   t_lane + 256 + (x ^ 1) * 128, aside && !to_own);
+      }
       // split: f32 rows of 512 bytes, their 16-byte units swizzled by the row: of
       // tile A over Q, of B over the first slots (at A's end Q is read no more,
       // at B's no slot is)
-      const uint32_t part = sbase + (dual ? 0 : x) * L::kPartOffB + row * 512;
+      const uint32_t part = sbase + (kDual ? 0 : x) * L::kPartOffB + row * 512;
 #pragma unroll 1
       for (int c = c0; c < c0 + chunks; ++c) {
         uint32_t o[32];
-        if (dual) {
-          // (a warpgroup without tiles has no O of its own: n == 1, and x == 1)
+        if constexpr (kDual) {
           uint32_t o2[32];
-          tmem_ld32((j0 < te ? t_o : t_lane + 256) + 32 * c, o);
+          tmem_ld32(t_own + 32 * c, o);
           if (both) tmem_ld32(t_lane + 256 + (x ^ 1) * 128 + 32 * c, o2);
           tmem_wait_ld();
           reg_fence32(o);
@@ -902,16 +946,10 @@ __global__ void __launch_bounds__(Layout<kFormat>::kThreads, 1)
           tmem_wait_ld();
           reg_fence32(o);
         }
-        if (aside) {
-          const Aside s = find_aside<kBf16, kFormat>(args, tb, te, mine, item.head, c);
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            o[i] = __float_as_uint(with_aside(__uint_as_float(o[i]), s, i));
-        }
         if constexpr (kSplit) {
 #pragma unroll
           for (int v = 0; v < 8; ++v)
-            st_shared_v4(part + (static_cast<uint32_t>(c * 8 + v) ^ lane) * 16, o[4 * v],
+            st_shared_v4(part + (static_cast<uint32_t>(c * 8 + v) ^ ln) * 16, o[4 * v],
                          o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
         } else {
           // 32 dims at a time: the warp's 32 rows of 64 bytes through its 2 KB,
@@ -926,31 +964,31 @@ __global__ void __launch_bounds__(Layout<kFormat>::kThreads, 1)
               y[i] = pack2<kBf16>(__uint_as_float(p[2 * i]) * inv_l,
                                   __uint_as_float(p[2 * i + 1]) * inv_l);
             // a row's unit v at v ^ (row / 2) % 4: two rows share 128 bytes of banks
-            st_shared_v4(stage + lane * 64 + (v ^ ((lane >> 1) & 3)) * 16, y[0], y[1], y[2], y[3]);
+            st_shared_v4(stage + ln * 64 + (v ^ ((ln >> 1) & 3)) * 16, y[0], y[1], y[2], y[3]);
           }
           __syncwarp();
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int rw = 8 * i + (lane >> 2), r = sub * 32 + rw;
-            const int rt = r / args.group, rh = r - rt * args.group;
+            const int rw = 8 * i + (ln >> 2), r = sub * 32 + rw;
+            const int rt = r / group, rh = r - rt * group;
             const int tok = first_token + rt;
             const uint4 v =
-                ld_shared_v4(stage + rw * 64 + ((lane & 3) ^ ((rw >> 1) & 3)) * 16);
+                ld_shared_v4(stage + rw * 64 + ((ln & 3) ^ ((rw >> 1) & 3)) * 16);
             if (r < tile_rows && tok < item.tokens)
               *reinterpret_cast<uint4*>(args.out +
                                         (static_cast<int64_t>(item.row0 + tok) * args.q_heads +
-                                         item.head * args.group + rh) *
+                                         item.head * group + rh) *
                                             kHeadDim +
-                                        c * 32 + (lane & 3) * 8) = v;
+                                        c * 32 + (ln & 3) * 8) = v;
           }
         }
       }
-      if (kSplit && !(dual && x == 1))
-        *reinterpret_cast<float2*>(smem + L::kEpiOff + ((dual ? 0 : x) * 128 + row) * 8) =
+      if (kSplit && !(kDual && x == 1))
+        *reinterpret_cast<float2*>(smem + L::kEpiOff + ((kDual ? 0 : x) * 128 + row) * 8) =
             make_float2(m_run, l_run);
       tc_fence_before();
       __syncwarp();
-      if (dual) {
+      if constexpr (kDual) {
         // the next item's P, and with it PV over O, only once both have read O
         if (!(ok = mbar_wait(bar(L::kTaken + (x ^ 1)), (ph >> 2) & 1u, abort_flag, args.status,
                              kDevTimeoutOFinal, wait_limit)))
@@ -1035,11 +1073,11 @@ __global__ void __launch_bounds__(Layout<kFormat>::kThreads, 1)
   }
 }
 
-template <bool kBf16, int kFormat, bool kSplit>
+template <bool kBf16, int kFormat, bool kSplit, bool kDual>
 cudaError_t launch(const PrefixMaps& m, const PrefixArgs& args, int grid, int splits,
                    cudaStream_t stream) {
   static bool configured[kMaxDevices] = {};
-  auto kernel = prefix_attention_kernel<kBf16, kFormat, kSplit>;
+  auto kernel = prefix_attention_kernel<kBf16, kFormat, kSplit, kDual>;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
@@ -1067,20 +1105,24 @@ cudaError_t launch(const PrefixMaps& m, const PrefixArgs& args, int grid, int sp
   return cudaLaunchKernelEx(&cfg, kernel, m.q, m.k, m.v, m.pk, m.pv, args);
 }
 
+template <bool kBf16, int kFormat>
+cudaError_t launch_format(const PrefixMaps& m, const PrefixArgs& a, int grid,
+                          cudaStream_t stream) {
+  const bool split = a.splits > 1;
+  if (a.one_tile)
+    return split ? launch<kBf16, kFormat, true, true>(m, a, grid, a.splits, stream)
+                 : launch<kBf16, kFormat, false, true>(m, a, grid, a.splits, stream);
+  return split ? launch<kBf16, kFormat, true, false>(m, a, grid, a.splits, stream)
+               : launch<kBf16, kFormat, false, false>(m, a, grid, a.splits, stream);
+}
+
 template <bool kBf16>
-cudaError_t launch_typed(const PrefixMaps& m, const PrefixArgs& a, int format, int grid, int splits,
+cudaError_t launch_typed(const PrefixMaps& m, const PrefixArgs& a, int format, int grid,
                          cudaStream_t stream) {
-  const bool split = splits > 1;
   switch (format) {
-    case kKvE4M3:
-      return split ? launch<kBf16, kKvE4M3, true>(m, a, grid, splits, stream)
-                   : launch<kBf16, kKvE4M3, false>(m, a, grid, splits, stream);
-    case kKvInt8:
-      return split ? launch<kBf16, kKvInt8, true>(m, a, grid, splits, stream)
-                   : launch<kBf16, kKvInt8, false>(m, a, grid, splits, stream);
-    default:
-      return split ? launch<kBf16, kKvPlain, true>(m, a, grid, splits, stream)
-                   : launch<kBf16, kKvPlain, false>(m, a, grid, splits, stream);
+    case kKvE4M3: return launch_format<kBf16, kKvE4M3>(m, a, grid, stream);
+    case kKvInt8: return launch_format<kBf16, kKvInt8>(m, a, grid, stream);
+    default: return launch_format<kBf16, kKvPlain>(m, a, grid, stream);
   }
 }
 
@@ -1088,7 +1130,7 @@ cudaError_t launch_typed(const PrefixMaps& m, const PrefixArgs& a, int format, i
 
 int prefix_active_clusters(int splits) {
   using L = Layout<kKvInt8>;
-  auto kernel = prefix_attention_kernel<false, kKvInt8, true>;
+  auto kernel = prefix_attention_kernel<false, kKvInt8, true, true>;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmemBytes) !=
       cudaSuccess)
     return 0;
@@ -1110,8 +1152,8 @@ int prefix_active_clusters(int splits) {
 cudaError_t launch_prefix_attention(const PrefixMaps& maps, const PrefixArgs& args, int bf16,
                                     int format, int grid, cudaStream_t stream) {
   if (grid <= 0) return cudaSuccess;
-  return bf16 ? launch_typed<true>(maps, args, format, grid, args.splits, stream)
-              : launch_typed<false>(maps, args, format, grid, args.splits, stream);
+  return bf16 ? launch_typed<true>(maps, args, format, grid, stream)
+              : launch_typed<false>(maps, args, format, grid, stream);
 }
 
 }  // namespace qwa

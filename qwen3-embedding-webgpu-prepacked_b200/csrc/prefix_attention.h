@@ -19,6 +19,7 @@ struct PrefixArgs {
   const PrefixRow* rows;
   const int* cta_offsets;  // not split: CTA c runs items [off[c], off[c + 1])
   int splits;              // CTAs of a cluster that share a block's tiles
+  int one_tile;            // blocks have at most tile_tokens tokens, not twice as many
   const void *k_prefix, *v_prefix;  // first row of the prefix (codes or 16-bit values)
   const uint8_t *k_scale, *v_scale;
   const uint16_t* v_own;

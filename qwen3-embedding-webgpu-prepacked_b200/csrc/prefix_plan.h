@@ -199,8 +199,8 @@ inline PrefixWork build_prefix_work(const PrefixShape& s, const int32_t* cu_q,
     emit(1);
     item.tile_end = static_cast<int>(w.tiles.size());
     w.items.push_back(item);
-    // one row tile takes two key tiles a period; 0.6 goes to the item's ends
-    w.cost.push_back(0.6 + (tokens <= s.tile_tokens ? std::max(1.0, cost / 2) : cost));
+    // blocks of one row tile take two key tiles a period; 0.6 goes to the item's ends
+    w.cost.push_back(0.6 + (s.block_tokens == s.tile_tokens ? std::max(1.0, cost / 2) : cost));
   }
   w.gap_end = std::max(w.gap_end, w.gap_beg);
   return w;
