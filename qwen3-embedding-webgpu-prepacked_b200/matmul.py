@@ -189,6 +189,12 @@ def qkv_projection(input: torch.Tensor, weight: torch.Tensor, q_weight: torch.Te
               f"{name} must be a contiguous CUDA float32 tensor of 128 elements")
     ctx = Context.for_device(dev.index)
     cu = _lib.cu_array(cu_seqlens)
+    if rope_table is not None:
+        longest = max((cu[b + 1] - cu[b] for b in range(len(cu) - 1)), default=0)
+        _need(rope_table.is_cuda and rope_table.dtype == torch.float32
+              and rope_table.is_contiguous() and rope_table.numel() >= longest * 128,
+              "rope_table must be a contiguous CUDA float32 [positions, 64, 2] of the longest "
+              "request's positions at least")
     if weight.dtype == torch.uint8:
         _need(weight.is_cuda and weight.numel() >= packed_bytes(4096, k),
               "packed weight must be a CUDA tile32-compact buffer of [4096, k]")

@@ -18,6 +18,10 @@ reference's dequantised values). Requests are packed back to back
 (``cu_seqlens``) or padded like the reference (``create_plan``); the
 engine (engine.py) drives either.
 
+Requests that begin with the same text can have it cached (``cache_prefix``):
+its keys and values of every layer are kept in 8 bits, and the requests' own
+tokens run alone, at positions behind it, over ``prefix.prefix_attention``.
+
 ``synthetic_model_file`` builds a complete ``.wgpack`` with seeded random
 weights of the model's shapes: the 384 MiB release file is not available
 here, so embeddings are not the trained model's.
@@ -26,12 +30,16 @@ from __future__ import annotations
 
 from typing import List, Optional, Sequence
 
+from dataclasses import dataclass
+
 import numpy as np
 import torch
 
 from . import attention as attn
-from . import ffn, matmul, norm, prepacked
+from . import ffn, matmul, norm, prepacked, rotary
+from .kv_cache import KVCache, kv_cache_write
 from .pooling import last_token_pool
+from .prefix import prefix_attention
 
 HIDDEN, INTERMEDIATE, Q_WIDTH, LAYERS = 1024, 3072, 2048, 28  # model.ts:18-21
 EPSILON = 1e-6
@@ -74,6 +82,18 @@ def synthetic_model_file(layers: int = LAYERS, vocab: int = 4096, seed: int = 0)
     meta = {"general.architecture": "qwen3", "general.name": "synthetic",
             "qwen3.block_count": layers}
     return pp.build_prepacked_file("0" * 64, 0, meta, tensors)
+
+
+@dataclass
+class CachedPrefix:
+    """The keys and values of a text that requests begin with, by layer, and
+    the attention mode that it was computed in."""
+    length: int
+    mode: int
+    caches: List[KVCache]
+
+    def nbytes(self) -> int:
+        return sum(c.nbytes() for c in self.caches)
 
 
 class Qwen3EmbeddingModel:
@@ -119,14 +139,60 @@ class Qwen3EmbeddingModel:
                                for key in ("attn_norm", "attn_q_norm", "attn_k_norm",
                                            "ffn_norm")})
         self.output_norm = weights.weight("output_norm.weight").float().contiguous()
+        self._rope: Optional[torch.Tensor] = None  # table of requests behind a prefix
+
+    def _rope_rows(self, first: int, count: int) -> torch.Tensor:
+        """(cos, sin) rows of positions ``first`` .. ``first + count - 1`` at least."""
+        need = first + count
+        if self._rope is None or self._rope.shape[0] < need:
+            rows = 1024
+            while rows < need:
+                rows *= 2
+            self._rope = rotary.rope_table(rows, attn.HEAD_DIM, attn.ROPE_THETA,
+                                           device=self.device)
+        return self._rope[first:]
+
+    def cache_prefix(self, ids: torch.Tensor, format: str = "e4m3",
+                     mode: int = attn.MODE_AUTO) -> CachedPrefix:
+        """Compute the text that requests will begin with (``ids``, CUDA int32)
+        once and keep its keys and values of every layer in ``format`` ("none":
+        float16, "e4m3" or "int8"). AUTO resolves the attention mode on the
+        prefix alone, and requests behind it keep that mode."""
+        length = int(ids.numel())
+        if length < 1:
+            raise ValueError("a prefix has at least one token")
+        if mode == attn.MODE_AUTO:
+            from . import sharding
+            mode = attn.MODE_SPARSE if sharding.resolve_sparse(mode, [length]) else attn.MODE_FULL
+        caches = [KVCache(length, format, device=self.device) for _ in range(self.layers)]
+        self.forward(ids, [0, length], mode, store=caches)
+        return CachedPrefix(length, mode, caches)
+
+    def with_prefix(self, prefix: CachedPrefix) -> "PrefixedModel":
+        """A runtime whose requests all stand behind ``prefix``."""
+        return PrefixedModel(self, prefix)
 
     def forward(self, ids: torch.Tensor, cu_seqlens: Sequence[int], mode: int = attn.MODE_AUTO,
-                trace: Optional[List[torch.Tensor]] = None) -> torch.Tensor:
+                trace: Optional[List[torch.Tensor]] = None,
+                prefix: Optional[CachedPrefix] = None,
+                store: Optional[List[KVCache]] = None) -> torch.Tensor:
         """Final normalized hidden state f16 [T, 1024] for packed ``ids``
         (CUDA int32). ``trace``: if a list, receives a copy of the residual
-        stream after every layer."""
+        stream after every layer. ``prefix``: every request continues that text (its
+        ``mode`` is used). ``store``: a cache for each layer, whose slots 0 .. T - 1
+        receive the layer's keys and values."""
         T = int(cu_seqlens[-1])
         dev = self.device
+        rope_rows = slots = None
+        if prefix is not None:
+            if len(prefix.caches) < self.layers:
+                raise ValueError(f"the prefix holds {len(prefix.caches)} layers; the model has "
+                                 f"{self.layers}")
+            longest = max((int(b) - int(a) for a, b in zip(cu_seqlens[:-1], cu_seqlens[1:])),
+                          default=0)
+            rope_rows = self._rope_rows(prefix.length, longest)
+        if store is not None:
+            slots = torch.arange(T, dtype=torch.int32, device=dev)
         f16 = dict(dtype=torch.float16, device=dev)
         x = ffn.embedding_lookup(ids, self.embed_table, HIDDEN, self.vocab)
         normalized = norm.rms_norm(x, self.gains[0]["attn_norm"])
@@ -139,9 +205,16 @@ class Qwen3EmbeddingModel:
         for l in range(self.layers):
             w, g = self.f16[l], self.gains[l]
             matmul.qkv_projection(normalized, w["attn_qkv"], g["attn_q_norm"], g["attn_k_norm"],
-                                  cu_seqlens, EPSILON, q_out=q, k_out=k, v_out=v)
-            attn.attention(q, k, v, cu_seqlens, value_stride=1024, value_offset=0, mode=mode,
-                           out=o)
+                                  cu_seqlens, EPSILON, q_out=q, k_out=k, v_out=v,
+                                  rope_table=rope_rows)
+            if store is not None:
+                kv_cache_write(store[l], k, v.view(T, 8, 128), slots)
+            if prefix is not None:
+                prefix_attention(q, k, v.view(T, 8, 128), cu_seqlens, prefix.caches[l],
+                                 prefix.length, mode=prefix.mode, out=o)
+            else:
+                attn.attention(q, k, v, cu_seqlens, value_stride=1024, value_offset=0, mode=mode,
+                               out=o)
             if T <= SMALL_ROWS:  # few rows: read the Q4_0 records (less weight traffic)
                 matmul.q40_matmul(o.view(T, Q_WIDTH), self.packed[l]["attn_output"], HIDDEN,
                                   Q_WIDTH, out=delta)
@@ -160,12 +233,40 @@ class Qwen3EmbeddingModel:
                 trace.append(x.clone())
         return normalized
 
-    def embed(self, ids: torch.Tensor, cu_seqlens: Sequence[int]) -> torch.Tensor:
-        """L2-normalised last-token embeddings f32 [batch, 1024]."""
-        return last_token_pool(self.forward(ids, cu_seqlens), cu_seqlens)
+    def embed(self, ids: torch.Tensor, cu_seqlens: Sequence[int],
+              prefix: Optional[CachedPrefix] = None) -> torch.Tensor:
+        """L2-normalised last-token embeddings f32 [batch, 1024]; ``prefix``: of
+        requests that continue that text."""
+        return last_token_pool(self.forward(ids, cu_seqlens, prefix=prefix), cu_seqlens)
 
     # the engine's runtime interface (engine.py)
     hidden = HIDDEN
+
+    def create_plan(self, batch: int, sequence: int):
+        from .engine import _PaddedPlan
+        return _PaddedPlan(self, batch, sequence)
+
+    def create_varlen_plan(self, batch: int, capacity: int):
+        from .engine import _VarlenPlan
+        return _VarlenPlan(self, batch, capacity)
+
+
+class PrefixedModel:
+    """A model whose requests all continue one cached text (the instruction of
+    a service): it offers the engine's runtime interface, so ``EmbeddingEngine``
+    batches requests of the remaining tokens alone."""
+
+    hidden = HIDDEN
+
+    def __init__(self, model: Qwen3EmbeddingModel, prefix: CachedPrefix):
+        self.model, self.prefix = model, prefix
+        self.device, self._attn = model.device, model._attn
+
+    def forward(self, ids: torch.Tensor, cu_seqlens: Sequence[int]) -> torch.Tensor:
+        return self.model.forward(ids, cu_seqlens, prefix=self.prefix)
+
+    def embed(self, ids: torch.Tensor, cu_seqlens: Sequence[int]) -> torch.Tensor:
+        return self.model.embed(ids, cu_seqlens, prefix=self.prefix)
 
     def create_plan(self, batch: int, sequence: int):
         from .engine import _PaddedPlan
