@@ -61,30 +61,37 @@ class KVCache:
         return self
 
     def _set(self, k, v, k_scale, v_scale, dtype) -> None:
-        _need(dtype in _DTYPES, "dtype must be float16 or bfloat16")
-        fmt = _FORMAT_OF.get(k.dtype)
-        if fmt is None and k.dtype == dtype:
+        code = _DTYPES.get(dtype)
+        _need(code is not None, "dtype must be float16 or bfloat16")
+        kind, index, shape = k.dtype, k.get_device(), k.shape
+        fmt = _FORMAT_OF.get(kind)
+        if fmt is None and kind == dtype:
             fmt = "none"
         _need(fmt is not None, "k must hold float8_e4m3fn, int8 or values of dtype")
-        index, shape = k.get_device(), k.shape
-        _need(index >= 0 and len(shape) == 3 and k.is_contiguous() and v.is_contiguous()
-              and v.shape == shape and v.dtype == k.dtype and v.get_device() == index,
+        _need(index >= 0 and len(shape) == 3 and v.shape == shape and v.dtype == kind
+              and v.get_device() == index and k.is_contiguous() and v.is_contiguous(),
               "k and v must be contiguous CUDA tensors [slots, heads, head_dim] of one kind")
+        slots, heads, dim = shape
         ks = vs = None
         if fmt == "none":
             _need(k_scale is None and v_scale is None, "16-bit values have no scales")
         else:
-            held = (shape[0], shape[1])
-            for s in (k_scale, v_scale):
-                _need(s is not None and s.dtype == torch.uint8 and s.shape == held
-                      and s.get_device() == index and s.is_contiguous(),
-                      "scales must be contiguous uint8 tensors [slots, heads]")
+            _need(k_scale is not None and v_scale is not None
+                  and k_scale.shape == (slots, heads) and v_scale.shape == (slots, heads)
+                  and k_scale.dtype == torch.uint8 and v_scale.dtype == torch.uint8
+                  and k_scale.get_device() == index and v_scale.get_device() == index
+                  and k_scale.is_contiguous() and v_scale.is_contiguous(),
+                  "scales must be contiguous uint8 tensors [slots, heads]")
             ks, vs = k_scale.data_ptr(), v_scale.data_ptr()
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.format, self.dtype, self.device = fmt, dtype, k.device
-        self.slots, self.heads, self.head_dim = shape
-        self.struct = _lib.KvCacheStruct(_DTYPES[dtype], FORMATS[fmt], self.heads, self.head_dim,
-                                         self.slots, k.data_ptr(), v.data_ptr(), ks, vs)
+        self.format, self.dtype, self.index = fmt, dtype, index
+        self.slots, self.heads, self.head_dim = slots, heads, dim
+        self.struct = _lib.KvCacheStruct(code, FORMATS[fmt], heads, dim, slots, k.data_ptr(),
+                                         v.data_ptr(), ks, vs)
+
+    @property
+    def device(self) -> torch.device:
+        return self.k.device
 
     def nbytes(self) -> int:
         held = (self.k, self.v, self.k_scale, self.v_scale)
@@ -111,7 +118,7 @@ def _rows(t: torch.Tensor, name: str, cache: KVCache, tokens: int, index: int) -
 
 def _write_args(ctx: Context, cache: KVCache, k, v, slots) -> tuple:
     index = ctx.device
-    _need(cache.device.index == index, "the cache must be on the kernel's device")
+    _need(cache.index == index, "the cache must be on the kernel's device")
     n = _slots(slots, index)
     return (ctypes.byref(cache.struct), k.data_ptr(), _rows(k, "k", cache, n, index),
             v.data_ptr(), _rows(v, "v", cache, n, index), slots.data_ptr(), n)
@@ -119,7 +126,7 @@ def _write_args(ctx: Context, cache: KVCache, k, v, slots) -> tuple:
 
 def _read_args(ctx: Context, cache: KVCache, slots, k_output, v_output) -> tuple:
     index = ctx.device
-    _need(cache.device.index == index, "the cache must be on the kernel's device")
+    _need(cache.index == index, "the cache must be on the kernel's device")
     n = _slots(slots, index)
     width = cache.heads * cache.head_dim
     _need(_rows(k_output, "k_output", cache, n, index) == width
@@ -158,7 +165,7 @@ def kv_cache_write(cache: KVCache, k: torch.Tensor, v: torch.Tensor, slots: torc
                    stream=None) -> None:
     """Quantise rows k, v [tokens, heads, head_dim] into the cache's ``slots``
     (int32 [tokens], all different)."""
-    ctx = Context.for_device(cache.device.index)
+    ctx = Context.for_device(cache.index)
     _launch(ctx, stream, ctx.lib.qwa_kv_cache_write, *_write_args(ctx, cache, k, v, slots))
 
 
@@ -172,6 +179,6 @@ def kv_cache_read(cache: KVCache, slots: torch.Tensor, k_out: Optional[torch.Ten
             k_out = cache.k.new_empty(shape, dtype=cache.dtype)
         if v_out is None:
             v_out = torch.empty_like(k_out)
-    ctx = Context.for_device(cache.device.index)
+    ctx = Context.for_device(cache.index)
     _launch(ctx, stream, ctx.lib.qwa_kv_cache_read, *_read_args(ctx, cache, slots, k_out, v_out))
     return k_out, v_out

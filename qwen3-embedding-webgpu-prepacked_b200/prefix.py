@@ -17,7 +17,6 @@ from __future__ import annotations
 
 import ctypes
 import threading
-from collections import OrderedDict
 from typing import Optional, Sequence
 
 import torch
@@ -69,7 +68,7 @@ class PrefixPlan:
         (memory is not freed then) they are released by the next plan."""
         if self.handle:
             handle, self.handle = self.handle, None
-            if torch.cuda.is_current_stream_capturing():
+            if _capturing(self.ctx.device):
                 _retired.append((self.ctx.lib, handle))
             else:
                 self.ctx.lib.qwa_prefix_plan_destroy(handle)
@@ -104,7 +103,7 @@ def _attention_args(ctx: Context, plan: PrefixPlan, q, k, v, output, cache, firs
     struct = workspace = None
     need = 0
     if cache is not None:
-        _need(cache.device.index == index, "the cache must be on q's device")
+        _need(cache.index == index, "the cache must be on q's device")
         struct = ctypes.byref(cache.struct)
         need = plan.workspace[cache.format]
         if need:
@@ -147,37 +146,40 @@ class PrefixAttentionKernel:
 
 
 MAX_PLANS = 64
-_plans: "OrderedDict" = OrderedDict()
-_captured: dict = {}  # plans that a graph was captured with are kept
+# (device, lengths, ...) -> [plan, use, kept]: `use` counts up with every use, and
+# plans that a graph was captured with are kept for good
+_plans: dict = {}
 _plans_lock = threading.Lock()
+_uses = 0
 
 
 def _capturing(device: int) -> bool:
     """Whether the device's current stream is being captured."""
-    if torch.cuda.current_device() == device:
-        return torch.cuda.is_current_stream_capturing()
+    if torch._C._cuda_getDevice() == device:
+        return torch._C._cuda_isCurrentStreamCapturing()
     with torch.cuda.device(device):
-        return torch.cuda.is_current_stream_capturing()
+        return torch._C._cuda_isCurrentStreamCapturing()
 
 
 def _plan_for(ctx: Context, *key) -> PrefixPlan:
-    full = (ctx.device,) + key
+    global _uses
+    full = (ctx.device, *key)
     with _plans_lock:
-        plan = _captured.get(full)
-        if plan is None:
-            plan = _plans.get(full)
-            if plan is not None:
-                _plans.move_to_end(full)
-                if _capturing(ctx.device):
-                    _captured[full] = plan
-    if plan is None:
-        cu_q, cu_k, prefix_len, q_heads, kv_heads, mode, sparse_prefix, window = key
-        plan = PrefixPlan(cu_q, prefix_len, q_heads, kv_heads, cu_k, mode, sparse_prefix, window,
-                          ctx=ctx)
-        with _plans_lock:
-            _plans[full] = plan
-            while len(_plans) > MAX_PLANS:
-                _plans.popitem(last=False)
+        entry = _plans.get(full)
+        if entry is not None:
+            _uses = entry[1] = _uses + 1
+            if not entry[2] and _capturing(ctx.device):
+                entry[2] = True
+            return entry[0]
+    cu_q, cu_k, prefix_len, q_heads, kv_heads, mode, sparse_prefix, window = key
+    plan = PrefixPlan(cu_q, prefix_len, q_heads, kv_heads, cu_k, mode, sparse_prefix, window,
+                      ctx=ctx)
+    with _plans_lock:
+        _uses += 1
+        _plans[full] = [plan, _uses, False]
+        loose = [(e[1], k) for k, e in _plans.items() if not e[2]]
+        if len(loose) > MAX_PLANS:
+            del _plans[min(loose)[1]]
     return plan
 
 
