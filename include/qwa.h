@@ -435,6 +435,12 @@ QWA_API qwa_status qwa_prefix_plan_create(qwa_ctx *ctx, const int32_t *cu_seqlen
                                           int sparse_prefix, int window, qwa_prefix_plan **out);
 QWA_API qwa_status qwa_prefix_plan_destroy(qwa_prefix_plan *plan);
 
+/* How a plan deals its work: query tokens of a block of rows (one or
+ * two tiles of 128 / group tokens, group = q_heads / kv_heads), and CTAs of a cluster that
+ * share a block's keys (1: none). Either pointer may be NULL. */
+QWA_API qwa_status qwa_prefix_plan_deal(const qwa_prefix_plan *plan, int *block_tokens,
+                                        int *splits);
+
 /* Bytes of device memory with which qwa_prefix_attention converts an 8-bit
  * prefix once instead of once for every block of rows; 0 where that does not
  * pay. format: a qwa_kv_format. */

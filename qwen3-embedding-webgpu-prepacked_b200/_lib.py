@@ -87,6 +87,7 @@ SIGNATURES = {
     "qwa_prefix_plan_create": (I32, [P, I32P, I32P, I32, I32, I32, I32, I32, I32, I32,
                                      ctypes.POINTER(P)]),
     "qwa_prefix_plan_destroy": (I32, [P]),
+    "qwa_prefix_plan_deal": (I32, [P, ctypes.POINTER(I32), ctypes.POINTER(I32)]),
     "qwa_prefix_attention_workspace": (ctypes.c_size_t, [P, I32]),
     "qwa_prefix_attention": (I32, [P, P, I32, P, I64, P, I64, P, I64, P, KvCacheP, I64, P,
                                    ctypes.c_size_t, P]),

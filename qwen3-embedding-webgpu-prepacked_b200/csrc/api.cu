@@ -1314,9 +1314,10 @@ qwa_status make_code_map(qwa_ctx* ctx, CUtensorMap* map, const void* base, int h
 }
 
 // An 8-bit prefix is converted once into a workspace, or tile by tile on the way of
-// each block. Once pays from two blocks on unless the prefix is short: E4M3, 3
-// blocks behind 1000 keys 39 us against 41, 2 behind 4000 50 against 53, 10 behind 200
-// 19 against 24; but 5 behind 200 23.3 against 22.0, 1 behind 8000 32 against 30.
+// each block. Once pays from two blocks on unless the prefix is short (E4M3, 16/8
+// heads; tokens behind keys: once / by block): 200 behind 1000 16.6 / 19.6 us, 600
+// behind 4000 46 / 53, 4000 behind 4000 168 / 193; but 128 behind 8000 33.7 / 35.0 and
+// 600 behind 200 13.1 / 13.0, and then without a workspace.
 bool convert_once(int blocks, int prefix_len) {
   return blocks >= 2 && static_cast<int64_t>(blocks) * prefix_len >= 2000;
 }
@@ -1390,7 +1391,7 @@ qwa_status create_prefix_plan(qwa_ctx* ctx, const int32_t* cu_q, const int32_t* 
       low.block_tokens = shape.tile_tokens;
       PrefixWork w_low = build_prefix_work(low, cu_q, cu_k);
       const PrefixDeal deal_low = prefix_deal(ctx, w_low, low);
-      if (deal_low.cost < 0.95 * deal.cost) {
+      if (plan->total_q <= shape.tile_tokens || deal_low.cost < 0.95 * deal.cost) {
         shape = low;
         deal = deal_low;
         w = std::move(w_low);
@@ -1503,6 +1504,13 @@ qwa_status qwa_prefix_plan_destroy(qwa_prefix_plan* plan) {
     if (plan->memory) cudaFree(plan->memory);  // waits for launches that read it
   }
   delete plan;
+  return QWA_OK;
+}
+
+qwa_status qwa_prefix_plan_deal(const qwa_prefix_plan* plan, int* block_tokens, int* splits) {
+  if (!plan) return QWA_ERR_INVALID_ARG;
+  if (block_tokens) *block_tokens = plan->shape.block_tokens;
+  if (splits) *splits = plan->splits;
   return QWA_OK;
 }
 

@@ -60,6 +60,10 @@ class PrefixPlan:
         self.queries = cu_q[len(cu_q) - 1]
         self.keys = cu_k[len(cu_k) - 1] if cu_k is not None else self.queries
         self.prefix_len, self.q_heads, self.kv_heads = prefix_len, q_heads, kv_heads
+        deal = ctypes.c_int(), ctypes.c_int()
+        _lib.check(self.ctx.lib.qwa_prefix_plan_deal(h, ctypes.byref(deal[0]),
+                                                     ctypes.byref(deal[1])))
+        self.block_tokens, self.splits = deal[0].value, deal[1].value
         fn = self.ctx.lib.qwa_prefix_attention_workspace
         self.workspace = {name: fn(h, code) for name, code in FORMATS.items()}  # bytes
 

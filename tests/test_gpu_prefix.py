@@ -117,6 +117,30 @@ def test_many_blocks(pkg, cuda_dev, dtype, fmt):
     check(pkg, p, 33, FULL)
 
 
+# lengths that the plan deals in each of its ways: (queries, prefix) -> tiles of a
+# block, split or not (on the 148 SMs of a B200)
+DEALS = {(1, True): ([20, 30, 10], 600), (1, False): ([60] * 18, 40),
+         (2, True): ([128] * 3, 4000), (2, False): ([700] * 8, 300)}
+
+
+@pytest.mark.parametrize("tiles,split", list(DEALS))
+@pytest.mark.parametrize("dtype,fmt", [(torch.float16, "e4m3"), (torch.bfloat16, "none"),
+                                       (torch.float16, "int8")])
+def test_every_deal(pkg, cuda_dev, tiles, split, dtype, fmt):
+    queries, prefix = DEALS[tiles, split]
+    plan = pkg.prefix.PrefixPlan(offsets(queries), prefix, 16, 8, mode=FULL)
+    assert (plan.block_tokens, plan.splits > 1) == (64 * tiles, split)
+    p = problem(pkg, tiles + 2 * split, queries, queries, prefix, 16, 8, dtype, fmt)
+    out = check(pkg, p, prefix, FULL)
+    # an 8-bit prefix converted tile by tile, and once: the same numbers
+    q, k, v, cache, _, _, cu, _ = p
+    kern = pkg.prefix.PrefixAttentionKernel(0)
+    plan.workspace = dict.fromkeys(plan.workspace, 0)
+    other = torch.empty_like(out)
+    kern.encode(None, kern.create_run(q, k, v, other, plan, cache))
+    assert torch.equal(out, other)
+
+
 def test_same_as_attention_without_a_prefix(pkg, cuda_dev):
     """With a prefix of no keys both operators compute the same (other tiles: a
     rounding apart); AUTO resolves to the same rule."""
@@ -149,16 +173,16 @@ def test_strides_slots_and_rows_behind(pkg, cuda_dev, fmt):
 
 @pytest.mark.parametrize("mode", [FULL, SPARSE])
 @pytest.mark.parametrize("fmt", ["none", "e4m3"])
-@pytest.mark.parametrize("split", [True, False])
-def test_values_that_are_not_finite_stay_with_their_rows(pkg, cuda_dev, mode, fmt, split):
+@pytest.mark.parametrize("queries", [[20, 30, 25], [60] * 18, [400] * 20, [128, 25, 100]])
+def test_values_that_are_not_finite_stay_with_their_rows(pkg, cuda_dev, mode, fmt, queries):
     """inf and NaN in V of one request, in its late keys and in the prefix: only
-    rows that keep the key see it. A NaN key (K) poisons only rows that keep it."""
-    queries, prefix = ([20, 30, 25] if split else [400] * 20), 300
+    rows that keep the key see it."""
+    prefix = 300
     p = problem(pkg, 5, queries, queries, prefix, 16, 8, torch.float16, fmt)
     q, k, v, cache, pk, pv, cu, _ = p
     for row, dim, x in ((cu[1] + 12, 3, float("inf")), (cu[1] + 20, 3, float("-inf")),
                         (cu[1] + 18, 100, float("nan")), (cu[2] - 1, 5, float("-inf")),
-                        (cu[0], 9, float("inf"))):
+                        (cu[0], 9, float("inf")), (cu[2] + 2, 64, float("-inf"))):
         v[row, 2, dim] = x
         v[row, 7, dim] = x
     if mode == SPARSE:  # keys of the prefix that later rows drop
@@ -182,6 +206,20 @@ def test_nan_key_reaches_only_rows_that_keep_it(pkg, cuda_dev):
     hit = torch.zeros(50, 16, dtype=torch.bool, device="cuda")
     hit[cu[1] + 4:, 6:8] = True
     assert torch.isnan(out[hit]).all() and torch.equal(out[~hit], clean[~hit])
+
+
+@pytest.mark.parametrize("fmt", ["none", "e4m3"])
+def test_prefix_past_32_bits(pkg, cuda_dev, fmt):
+    """The prefix at an offset above 2^31 bytes of its cache."""
+    per_slot = 1024 * (2 if fmt == "none" else 1)
+    prefix, first = 150, 2 ** 31 // per_slot + 7
+    p = problem(pkg, 4, [40, 30], [40, 30], prefix, 16, 8, torch.float16, fmt)
+    big = pkg.kv_cache.KVCache(first + prefix + 1, fmt)
+    slots = torch.arange(first, first + prefix, dtype=torch.int32, device="cuda")
+    pkg.kv_cache.kv_cache_write(big, p[4].half(), p[5].half(), slots)
+    back = pkg.kv_cache.kv_cache_read(big, slots)
+    check(pkg, (p[0], p[1], p[2], big, back[0].double(), back[1].double(), p[6], p[7]), prefix,
+          FULL, first_slot=first)
 
 
 def test_large_scores(pkg, cuda_dev):
