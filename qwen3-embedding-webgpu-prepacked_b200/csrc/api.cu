@@ -1325,16 +1325,19 @@ bool convert_once(int blocks, int prefix_len) {
 constexpr int kMaxSplits = 8;  // the portable cluster size
 
 // How a call's blocks go over the SMs: the CTAs of a cluster that share a block's
-// tiles (1: none, whole blocks dealt to the SMs), and an estimate of its time. Its unit is the
-// period of one key tile for two row tiles (2.3 us). A cluster costs a start and
-// a merge more, which moves 512 bytes a row between SMs, and as many rounds as the
-// clusters do not fit at once (of 8 CTAs 15 fit, not 18: the GPCs are not even).
+// tiles (1: none, whole blocks dealt to the SMs), and an estimate of its time in
+// us. Whole blocks start in 4.6 us (one row tile) or 4.8 (two). A cluster takes 6.6 or
+// 5.0 us besides its share of the tiles, and to merge, 0.02 us a row of one row tile
+// and 0.03 of two (512 bytes a row move between SMs); as many rounds as the clusters do not fit
+// at once (of 8 CTAs 15 fit, not 18: the GPCs are not even). Measured against every
+// other deal for 1 to 41 blocks of 16/8 and 4/2 heads behind 60 to 4000 keys.
 struct PrefixDeal {
   int splits = 1;
   double cost = 0;
 };
 PrefixDeal prefix_deal(qwa_ctx* ctx, const PrefixWork& w, const PrefixShape& s) {
   const int64_t items = static_cast<int64_t>(w.items.size()) * s.kv_heads;
+  const bool one_tile = s.block_tokens == s.tile_tokens;
   int least = 1 << 30, most = 0, tokens = 0;
   double longest = 0, total = 0;
   for (size_t i = 0; i < w.items.size(); ++i) {
@@ -1352,20 +1355,20 @@ PrefixDeal prefix_deal(qwa_ctx* ctx, const PrefixWork& w, const PrefixShape& s) 
     const int64_t rounds = (items + ctx->sms - 1) / ctx->sms;
     best.cost = std::max(best.cost, rounds * total / static_cast<double>(items));
   }
+  best.cost += one_tile ? 4.6 : 4.8;
   if (items >= ctx->sms) return best;
   if (ctx->clusters[1] == 0) {
     ctx->clusters[1] = ctx->sms;
     for (int i = 2; i <= kMaxSplits; ++i) ctx->clusters[i] = prefix_active_clusters(i);
   }
-  const bool one_tile = s.block_tokens == s.tile_tokens;
   const int rows = tokens * (s.q_heads / s.kv_heads);
-  const double merge = 0.8 + rows / 128.0;
   for (int n = 2; n <= std::min(kMaxSplits, least); ++n) {
     if (ctx->clusters[n] < 1) continue;
     const int64_t rounds = (items + ctx->clusters[n] - 1) / ctx->clusters[n];
     const int share = (most + n - 1) / n;
-    const double cost = rounds * ((one_tile ? (share + 1) / 2 : share) + 0.6 + merge) +
-                        (rounds - 1) * 2.0;
+    const double cost =
+        rounds * (one_tile ? 6.6 + kDualTileUs * share + 0.02 * rows
+                           : 5.0 + kTileUs * share + 0.03 * rows);
     if (cost < best.cost) {
       best.splits = n;
       best.cost = cost;

@@ -55,11 +55,15 @@ struct PrefixShape {
   int block_tokens;  // of a block: tile_tokens or 2 * tile_tokens
 };
 
+// Measured: a key tile of a block of two row tiles, and of a block of one (dual), in
+// us.
+constexpr double kTileUs = 2.14, kDualTileUs = 1.325;
+
 struct PrefixWork {
   std::vector<PrefixItem> items;  // without the head; one per block
   std::vector<PrefixTile> tiles;
   std::vector<PrefixRow> rows;
-  std::vector<double> cost;       // of an item: periods of one key tile for two row tiles
+  std::vector<double> cost;       // of an item among others, us (on a B200)
   // prefix keys that no tile reaches: [gap_beg, gap_end)
   int gap_beg = 0, gap_end = 0;
 };
@@ -199,8 +203,9 @@ inline PrefixWork build_prefix_work(const PrefixShape& s, const int32_t* cu_q,
     emit(1);
     item.tile_end = static_cast<int>(w.tiles.size());
     w.items.push_back(item);
-    // blocks of one row tile take two key tiles a period; 0.6 goes to the item's ends
-    w.cost.push_back(0.6 + (s.block_tokens == s.tile_tokens ? std::max(1.0, cost / 2) : cost));
+    const int n = item.tile_end - item.tile_beg;
+    w.cost.push_back(s.block_tokens == s.tile_tokens ? 2.0 + kDualTileUs * n
+                                                     : 3.0 + kTileUs * cost);
   }
   w.gap_end = std::max(w.gap_end, w.gap_beg);
   return w;
