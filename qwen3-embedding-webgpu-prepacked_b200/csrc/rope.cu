@@ -22,7 +22,8 @@ namespace {
 // A thread takes one frequency over kTableRun positions: sin and cos of the
 // first, then turns by f in 64 bits (16 turns add less than 2^-47, far below the
 // rounding to f32). With sincos for every entry the kernel was bound by its 64-bit
-// arithmetic (27 us for 131072 x 64 entries, against 10 us to write them).
+// arithmetic (27 us for 131072 x 64 entries); now by its writes (12.4 us, 5.4 TB/s, 0.84
+// of measured; runs of 8, 32 and 64 positions took 13.6, 12.9 and 12.8).
 constexpr int kTableRun = 16;
 constexpr int kTableThreads = 128;
 
@@ -98,7 +99,10 @@ __global__ void __launch_bounds__(kRopeThreads) rope_any_kernel(const RopeArgs a
 //                then the units behind the rotated part, copied
 //   interleaved: 4 pairs, of which those past the rotated part are copied
 // HBM-bound: a thread issues the loads of kHeads heads before any arithmetic,
-// six in both layouts.
+// six in both layouts (two to eight, and blocks of 96 to 256, were slower). Loading
+// before the position is known cost registers and was slower too (25 us against 20).
+// 8000 tokens of 16 + 8 heads, f16 in halves: 19.8 us, 5.2 TB/s (0.80 of measured);
+// 20011 in bf16, half of each head: 44.3 us, 5.7 TB/s (0.88); 16 tokens: 2.2 us.
 constexpr int kRowThreads = 128;
 
 template <bool kBf16>
@@ -204,10 +208,13 @@ cudaError_t launch_rope(RopeArgs a, int bf16, cudaStream_t stream) {
                     whole_units(a.k) && (a.layout == 1 || a.rotary % 16 == 0);
   if (rows) {
     a.units = a.layout == 1 ? a.head_dim / 8 : a.rotary / 16 + (a.head_dim - a.rotary) / 8;
-    // Heads of one thread: as many as it has loads in flight for, so that few
-    // threads read a token's cosines; one where there are few tokens, for latency.
+    // Heads of one thread: one until such threads fill the SMs (16 + 8 heads of 128
+    // in halves: 64 tokens 2.3 us against 2.5, 512 3.8 / 3.9, 1024 4.9 / 4.9), then as
+    // many as it has loads in flight for, so that fewer threads read a token's
+    // cosines (2048: 7.6 against 6.8, 4096: 12.6 / 10.8).
     const int most = a.layout == 1 ? 6 : 3;
-    const int step = a.tokens >= 1024 ? (heads + most - 1) / most : heads;
+    const bool few = static_cast<int64_t>(a.tokens) * heads * a.units < 200000;
+    const int step = few ? heads : (heads + most - 1) / most;
     a.head_step = step * a.units <= kRowThreads ? step : kRowThreads / a.units;
     a.token_threads = a.units * a.head_step;
     a.block_tokens = kRowThreads / a.token_threads;
