@@ -124,16 +124,22 @@ def _write_args(ctx: Context, cache: KVCache, k, v, slots) -> tuple:
             v.data_ptr(), _rows(v, "v", cache, n, index), slots.data_ptr(), n)
 
 
-def _read_args(ctx: Context, cache: KVCache, slots, k_output, v_output) -> tuple:
+def _read_args(ctx: Context, cache: KVCache, slots, k_output, v_output):
+    """(k's output, v's output, the C call's arguments); outputs of None are made"""
     index = ctx.device
     _need(cache.index == index, "the cache must be on the kernel's device")
     n = _slots(slots, index)
     width = cache.heads * cache.head_dim
-    _need(_rows(k_output, "k_output", cache, n, index) == width
-          and _rows(v_output, "v_output", cache, n, index) == width,
-          "k_output and v_output must be contiguous")
-    return (ctypes.byref(cache.struct), slots.data_ptr(), n, k_output.data_ptr(),
-            v_output.data_ptr())
+    if k_output is None:
+        k_output = cache.k.new_empty((n, cache.heads, cache.head_dim), dtype=cache.dtype)
+    else:
+        _need(_rows(k_output, "k_output", cache, n, index) == width, "k_output must be contiguous")
+    if v_output is None:
+        v_output = torch.empty_like(k_output)
+    else:
+        _need(_rows(v_output, "v_output", cache, n, index) == width, "v_output must be contiguous")
+    return k_output, v_output, (ctypes.byref(cache.struct), slots.data_ptr(), n,
+                                k_output.data_ptr(), v_output.data_ptr())
 
 
 class KVCacheKernel:
@@ -155,7 +161,8 @@ class KVCacheKernel:
                         v_output: torch.Tensor) -> EncodableRun:
         """k_output, v_output [tokens, heads, head_dim]; a slot outside the cache
         gives zeros."""
-        args = _read_args(self.ctx, cache, slots, k_output, v_output)
+        _need(k_output is not None and v_output is not None, "outputs are required")
+        _, _, args = _read_args(self.ctx, cache, slots, k_output, v_output)
         lib, h = self.ctx.lib, self.ctx.handle
         return EncodableRun(lambda s: lib.qwa_kv_cache_read(h, *args, s), self.ctx,
                             "KV cache read")
@@ -173,12 +180,7 @@ def kv_cache_read(cache: KVCache, slots: torch.Tensor, k_out: Optional[torch.Ten
                   v_out: Optional[torch.Tensor] = None, stream=None
                   ) -> Tuple[torch.Tensor, torch.Tensor]:
     """(k, v) [tokens, heads, head_dim] of ``slots`` in the cache's dtype."""
-    if k_out is None or v_out is None:
-        shape = (slots.numel(), cache.heads, cache.head_dim)
-        if k_out is None:
-            k_out = cache.k.new_empty(shape, dtype=cache.dtype)
-        if v_out is None:
-            v_out = torch.empty_like(k_out)
     ctx = Context.for_device(cache.index)
-    _launch(ctx, stream, ctx.lib.qwa_kv_cache_read, *_read_args(ctx, cache, slots, k_out, v_out))
+    k_out, v_out, args = _read_args(ctx, cache, slots, k_out, v_out)
+    _launch(ctx, stream, ctx.lib.qwa_kv_cache_read, *args)
     return k_out, v_out

@@ -95,15 +95,19 @@ def _packed(t: torch.Tensor, name: str, tokens: int, heads: int, dtype, index: i
 
 
 def _attention_args(ctx: Context, plan: PrefixPlan, q, k, v, output, cache, first_slot):
-    """(workspace or None, the C call's arguments between plan and stream)"""
+    """(output, made if None; workspace or None; the C call's arguments between plan
+    and stream)"""
     dtype, index = q.dtype, ctx.device
     code = _DTYPES.get(dtype)
     _need(code is not None, "q must be float16 or bfloat16")
     _need(plan.ctx.device == index, "the plan must be on the kernel's device")
     _need(plan.handle is not None, "the plan is closed")
     n, hq, m, hk = plan.queries, plan.q_heads, plan.keys, plan.kv_heads
-    _need(_packed(output, "output", n, hq, dtype, index) == hq * HEAD_DIM,
-          "output must be contiguous")
+    if output is None:
+        output = torch.empty_like(q, memory_format=torch.contiguous_format)
+    else:
+        _need(_packed(output, "output", n, hq, dtype, index) == hq * HEAD_DIM,
+              "output must be contiguous")
     struct = workspace = None
     need = 0
     if cache is not None:
@@ -114,7 +118,7 @@ def _attention_args(ctx: Context, plan: PrefixPlan, q, k, v, output, cache, firs
             workspace = q.new_empty(need, dtype=torch.uint8)
     else:
         _need(plan.prefix_len == 0, "a prefix needs its cache")
-    return workspace, (
+    return output, workspace, (
         code, q.data_ptr(), _packed(q, "q", n, hq, dtype, index), k.data_ptr(),
         _packed(k, "k", m, hk, dtype, index), v.data_ptr(), _packed(v, "v", m, hk, dtype, index),
         output.data_ptr(), struct, first_slot,
@@ -134,7 +138,8 @@ class PrefixAttentionKernel:
         request after request, output as q, contiguous; the prefix is in the
         cache's slots ``first_slot`` .. ``first_slot + plan.prefix_len - 1``. A run
         with ``owned_buffers`` is issued on one stream at a time."""
-        workspace, args = _attention_args(self.ctx, plan, q, k, v, output, cache, first_slot)
+        _need(output is not None, "an output is required")
+        _, workspace, args = _attention_args(self.ctx, plan, q, k, v, output, cache, first_slot)
         lib, h = self.ctx.lib, self.ctx.handle
 
         def launch(stream):
@@ -202,13 +207,11 @@ def prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     q_shape, k_shape = q.shape, k.shape
     _need(q.is_cuda and len(q_shape) == 3 and len(k_shape) == 3,
           "q and k must be CUDA tensors [tokens, heads, 128]")
-    if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     ctx = Context.for_device(q.get_device())
     plan = _plan_for(ctx, tuple(cu_seqlens),
                      tuple(cu_seqlens_k) if cu_seqlens_k is not None else None, prefix_len,
                      q_shape[1], k_shape[1], mode, sparse_prefix, window)
-    workspace, args = _attention_args(ctx, plan, q, k, v, out, cache, first_slot)
+    out, workspace, args = _attention_args(ctx, plan, q, k, v, out, cache, first_slot)
     _launch(ctx, stream, ctx.lib.qwa_prefix_attention, plan.handle, *args)
     if workspace is not None and stream is not None:
         # its memory must not be handed out again before that stream is done with it

@@ -71,46 +71,56 @@ def rope_table(positions: int, rotary_dim: int = 128, theta: float = ROPE_THETA,
     return out
 
 
-def _side(x: Optional[torch.Tensor], y: Optional[torch.Tensor], name: str, tokens: int, dim: int,
-          dtype, index: int):
-    """Checks one of q and k with its output; its qwa_rope_tensor."""
-    if x is None:
-        return None
-    if y is None:
-        raise ValueError(f"{name} needs an output")
+def _side(x: torch.Tensor, y: Optional[torch.Tensor], name: str, tokens: int, dim: int, dtype,
+          index: int):
+    """Checks one of q and k with its output (None: one is made); the output and
+    their qwa_rope_tensor."""
     shape = x.shape
-    if len(shape) != 3 or shape[0] != tokens or shape[2] != dim or y.shape != shape:
-        raise ValueError(f"{name} and its output must be [tokens, heads, head_dim] of one shape")
-    if x.dtype != dtype or y.dtype != dtype or x.get_device() != index or y.get_device() != index:
-        raise ValueError(f"{name} and its output must agree with the others in dtype and device")
+    if len(shape) != 3 or shape[0] != tokens or shape[2] != dim:
+        raise ValueError(f"{name} must be [tokens, heads, head_dim] as the others")
+    if x.dtype != dtype or x.get_device() != index:
+        raise ValueError(f"{name} must agree with the others in dtype and device")
     x0, x1, x2 = x.stride()
-    y0, y1, y2 = y.stride()
+    if y is None:
+        y = torch.empty_like(x, memory_format=torch.contiguous_format)
+        y0, y1, y2 = shape[1] * dim, dim, 1
+    else:
+        if y.shape != shape or y.dtype != dtype or y.get_device() != index:
+            raise ValueError(f"{name}'s output must be of its shape, dtype and device")
+        y0, y1, y2 = y.stride()
     if x2 != 1 or y2 != 1:
         raise ValueError(f"{name}: a head's values must be contiguous")
-    return _lib.RopeTensor(x.data_ptr(), x0, x1, y.data_ptr(), y0, y1, shape[1])
+    return y, _lib.RopeTensor(x.data_ptr(), x0, x1, y.data_ptr(), y0, y1, shape[1])
 
 
-def _rope_args(ctx: Context, q, k, table, positions, q_output, k_output, layout, inverse) -> tuple:
+def _rope_args(ctx: Context, q, k, table, positions, q_output, k_output, layout, inverse):
+    """(q's output, k's output, the C call's arguments between context and stream)"""
     some = q if q is not None else k
     dtype, index, shape = some.dtype, ctx.device, some.shape
-    code = _DTYPES.get(dtype)
-    _need(code is not None and len(shape) == 3,
-          "q or k must be a CUDA float16 or bfloat16 tensor [tokens, heads, head_dim]")
-    _need(layout in _LAYOUTS, "layout must be 'half' or 'interleaved'")
+    code, order = _DTYPES.get(dtype), _LAYOUTS.get(layout)
+    if code is None or len(shape) != 3:
+        raise ValueError("q or k must be a CUDA float16 or bfloat16 tensor [tokens, heads, "
+                         "head_dim]")
+    if order is None:
+        raise ValueError("layout must be 'half' or 'interleaved'")
     tokens, _, dim = shape
-    qs = _side(q, q_output, "q", tokens, dim, dtype, index)
-    ks = _side(k, k_output, "k", tokens, dim, dtype, index)
-    rows = table.shape
-    _need(table.dtype == torch.float32 and table.get_device() == index and len(rows) == 3
-          and rows[2] == 2 and table.is_contiguous(),
-          "table must be a contiguous float32 [rows, rotary_dim / 2, 2] on q's device")
-    _need(positions.dtype == torch.int32 and positions.get_device() == index
-          and positions.is_contiguous() and positions.numel() >= tokens,
-          "positions must be a contiguous int32 tensor of one position a token")
-    return (code, ctypes.byref(qs) if qs is not None else None,
-            ctypes.byref(ks) if ks is not None else None, tokens, dim, 2 * rows[1],
-            _LAYOUTS[layout], 1 if inverse else 0, positions.data_ptr(), table.data_ptr(),
-            rows[0])
+    rows, half, two = table.shape
+    if two != 2 or table.dtype != torch.float32 or table.get_device() != index \
+            or not table.is_contiguous():
+        raise ValueError("table must be a contiguous float32 [rows, rotary_dim / 2, 2] on q's "
+                         "device")
+    if positions.dtype != torch.int32 or positions.get_device() != index \
+            or positions.numel() < tokens or not positions.is_contiguous():
+        raise ValueError("positions must be a contiguous int32 tensor of one position a token")
+    qs = ks = None
+    if q is not None:
+        q_output, qs = _side(q, q_output, "q", tokens, dim, dtype, index)
+        qs = ctypes.byref(qs)
+    if k is not None:
+        k_output, ks = _side(k, k_output, "k", tokens, dim, dtype, index)
+        ks = ctypes.byref(ks)
+    return q_output, k_output, (code, qs, ks, tokens, dim, 2 * half, order, 1 if inverse else 0,
+                                positions.data_ptr(), table.data_ptr(), rows)
 
 
 class RopeKernel:
@@ -127,7 +137,10 @@ class RopeKernel:
         either may be None. An output may be its input (in place). A token
         whose position is not a row of the table is left unwritten."""
         _need(q is not None or k is not None, "one of q and k is required")
-        args = _rope_args(self.ctx, q, k, table, positions, q_output, k_output, layout, inverse)
+        _need((q is None or q_output is not None) and (k is None or k_output is not None),
+              "q and k need their outputs")
+        _, _, args = _rope_args(self.ctx, q, k, table, positions, q_output, k_output, layout,
+                                inverse)
         lib, h = self.ctx.lib, self.ctx.handle
         return EncodableRun(lambda s: lib.qwa_rope(h, *args, s), self.ctx, "rotary positions")
 
@@ -139,11 +152,7 @@ def rope(q: Optional[torch.Tensor], k: Optional[torch.Tensor], table: torch.Tens
     """(q, k) rotated at each token's position (the way back with ``inverse``)."""
     some = q if q is not None else k
     _need(some is not None and some.is_cuda, "q or k must be a CUDA tensor")
-    if q is not None and q_out is None:
-        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    if k is not None and k_out is None:
-        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
     ctx = Context.for_device(some.get_device())
-    _launch(ctx, stream, ctx.lib.qwa_rope,
-            *_rope_args(ctx, q, k, table, positions, q_out, k_out, layout, inverse))
+    q_out, k_out, args = _rope_args(ctx, q, k, table, positions, q_out, k_out, layout, inverse)
+    _launch(ctx, stream, ctx.lib.qwa_rope, *args)
     return q_out, k_out
