@@ -254,7 +254,7 @@ struct RopeArgs {
   int smem_heads;  // any rows: heads that a block stages at a time
   // rows of whole 16-byte units: units of a head, heads between those of one
   // thread, threads of a token, tokens of a block
-  int units, head_step, token_threads, block_tokens;
+  int units, head_step, token_threads, block_tokens, units_m, token_threads_m;
   __device__ __forceinline__ const uint16_t* in_row(int64_t t, int h) const {
     return h < q.heads ? q.in + t * q.in_stride + h * q.in_head_stride
                        : k.in + t * k.in_stride + (h - q.heads) * k.in_head_stride;
@@ -273,7 +273,10 @@ struct KvCacheArgs {
   uint8_t *k_scale, *v_scale;  // [slots, heads] exponent + 127
   int64_t slots;
   int heads, head_dim, tokens;
-  uint32_t vectors;        // 2 * tokens * heads
+  uint32_t vectors;        // 2 * tokens * heads, at most 2^31
+  // n / heads = (n * heads_m) >> heads_s for n < 2^31 (kv_cache_divisor)
+  uint32_t heads_m;
+  int heads_s;
   const int32_t* slot_of;  // [tokens]; reading, nullptr: slots in order (below)
   int64_t first_slot;      // of the first row; rows from `head` on lie `gap` rows
   int head, gap;           // further, in the cache and in the output
@@ -281,6 +284,15 @@ struct KvCacheArgs {
   int64_t k_stride, v_stride;  // elements a token
   void *k_out, *v_out;
 };
+// Division by an invariant by a multiplication: with s = 31 + ceil(log2 d) and m =
+// ceil(2^s / d), n m / 2^s exceeds n / d by less than n / 2^31 / d < 1 / d, so its
+// floor is that of n / d. m < 2^32.
+inline void kv_cache_divisor(KvCacheArgs* a) {
+  int s = 31;
+  while ((1ll << (s - 31)) < a->heads) ++s;
+  a->heads_s = s;
+  a->heads_m = static_cast<uint32_t>(((1ull << s) + a->heads - 1) / a->heads);
+}
 cudaError_t launch_kv_write(const KvCacheArgs& args, int bf16, int format, cudaStream_t stream);
 cudaError_t launch_kv_read(const KvCacheArgs& args, int bf16, int format, cudaStream_t stream);
 

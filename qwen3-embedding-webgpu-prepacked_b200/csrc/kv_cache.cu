@@ -134,14 +134,14 @@ struct Where {
   int kv, head;
 };
 __device__ __forceinline__ Where where(const KvCacheArgs& a, uint32_t vec) {
-  const uint32_t th = vec / a.heads;
+  const uint32_t th = static_cast<uint32_t>((static_cast<uint64_t>(vec) * a.heads_m) >> a.heads_s);
   return {th >> 1, static_cast<int>(th & 1), static_cast<int>(vec - th * a.heads)};
 }
 
 // head_dim / 16 lanes hold a vector, 16 values each (two loads, one 16-byte
 // store of codes). HBM-bound: a thread's kVectors loads are in flight together, and
-// wait for nothing. 80000 tokens of 8 heads into INT8: 88 us, 5.6 TB/s (0.86 of measured);
-// 16 tokens: 2.0 us.
+// wait for nothing. 80000 tokens of 8 heads into INT8: 81 us, 6.1 TB/s (0.95 of measured; 91 us with
+// divisions by `heads`, which made it bound by its arithmetic); 16 tokens: 1.7 us.
 template <bool kBf16, int kFormat, int kVectors>
 __global__ void __launch_bounds__(kThreads) kv_write_kernel(const KvCacheArgs a) {
   using C = Code<kBf16, kFormat == kKvPlain ? kKvE4M3 : kFormat>;
@@ -150,13 +150,16 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(const KvCacheArgs a)
   const uint32_t v0 = blockIdx.x * (per_pass * kVectors) + threadIdx.x / lanes;
   uint4 x[kVectors][2];
   int64_t row[kVectors];  // (slot, head), -1: nothing to write
+  bool is_v[kVectors];
 #pragma unroll
   for (int i = 0; i < kVectors; ++i) {
     const uint32_t vec = v0 + i * per_pass;
     row[i] = -1;
+    is_v[i] = false;
     x[i][0] = x[i][1] = make_uint4(0u, 0u, 0u, 0u);
     if (vec >= a.vectors) continue;
     const Where w = where(a, vec);
+    is_v[i] = w.kv;
     // the rows are read whether their slot exists or not: nothing waits for it
     const uint4* src = reinterpret_cast<const uint4*>(
         static_cast<const uint16_t*>(w.kv ? a.v_in : a.k_in) +
@@ -169,8 +172,7 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(const KvCacheArgs a)
   }
 #pragma unroll
   for (int i = 0; i < kVectors; ++i) {
-    const uint32_t vec = v0 + i * per_pass;
-    const bool v = (vec / a.heads) & 1;
+    const bool v = is_v[i];
     const int64_t at = row[i] * a.head_dim + l * 16;
     if constexpr (kFormat == kKvPlain) {
       if (row[i] >= 0) {
@@ -215,7 +217,7 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(const KvCacheArgs a)
 }
 
 // The way back: 16 codes a lane (one load, two stores). 8000 scattered slots of 8
-// heads from E4M3: 11.5 us, 4.3 TB/s (0.67 of measured; 2 us of it are the launch).
+// heads from E4M3: 10.8 us, 4.6 TB/s (0.71 of measured; 2 us of it are the launch).
 template <bool kBf16, int kFormat, int kVectors>
 __global__ void __launch_bounds__(kThreads) kv_read_kernel(const KvCacheArgs a) {
   const int lanes = a.head_dim / 16, per_pass = kThreads / lanes;
@@ -223,13 +225,14 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const KvCacheArgs a) 
   const uint32_t v0 = blockIdx.x * (per_pass * kVectors) + threadIdx.x / lanes;
   uint4 x[kVectors][2];
   int e[kVectors];
+  Where at_row[kVectors];
 #pragma unroll
   for (int i = 0; i < kVectors; ++i) {
     const uint32_t vec = v0 + i * per_pass;
     x[i][0] = x[i][1] = make_uint4(0u, 0u, 0u, 0u);
     e[i] = 0;
     if (vec >= a.vectors) continue;
-    const Where w = where(a, vec);
+    const Where w = at_row[i] = where(a, vec);
     // without a list: the slots from first_slot on, a gap left out after `head`
     const int64_t slot = a.slot_of ? __ldg(a.slot_of + w.token)
                                    : a.first_slot + w.token + (w.token >= a.head ? a.gap : 0);
@@ -249,7 +252,7 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const KvCacheArgs a) 
   for (int i = 0; i < kVectors; ++i) {
     const uint32_t vec = v0 + i * per_pass;
     if (vec >= a.vectors) break;
-    const Where w = where(a, vec);
+    const Where w = at_row[i];
     if constexpr (kFormat != kKvPlain) {
       const uint32_t c[4] = {x[i][0].x, x[i][0].y, x[i][0].z, x[i][0].w};
       const uint32_t s2 = pair_pow2<kBf16>(e[i]);
@@ -269,7 +272,8 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const KvCacheArgs a) 
 }
 
 template <bool kWrite, bool kBf16, int kVectors>
-cudaError_t launch_format(const KvCacheArgs& a, int format, cudaStream_t stream) {
+cudaError_t launch_format(KvCacheArgs a, int format, cudaStream_t stream) {
+  kv_cache_divisor(&a);
   const int64_t per_block = kThreads / (a.head_dim / 16) * kVectors;
   const unsigned blocks = static_cast<unsigned>((a.vectors + per_block - 1) / per_block);
   auto go = [&](auto kernel) { kernel<<<blocks, kThreads, 0, stream>>>(a); };
