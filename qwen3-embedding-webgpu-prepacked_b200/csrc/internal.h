@@ -254,7 +254,7 @@ struct RopeArgs {
   int smem_heads;  // any rows: heads that a block stages at a time
   // rows of whole 16-byte units: units of a head, heads between those of one
   // thread, threads of a token, tokens of a block
-  int units, head_step, token_threads, block_tokens, units_m, token_threads_m;
+  int units, head_step, token_threads, block_tokens;
   __device__ __forceinline__ const uint16_t* in_row(int64_t t, int h) const {
     return h < q.heads ? q.in + t * q.in_stride + h * q.in_head_stride
                        : k.in + t * k.in_stride + (h - q.heads) * k.in_head_stride;

@@ -114,12 +114,11 @@ __device__ __forceinline__ uint32_t turn_pair(uint32_t x, float c, float s) {
 template <bool kBf16, bool kInterleaved>
 __global__ void __launch_bounds__(kRowThreads) rope_rows_kernel(const RopeArgs a) {
   constexpr int kHeads = kInterleaved ? 6 : 3;
-  // (divisions of numbers below 128 by a multiplication, launch_rope)
-  const int group = (threadIdx.x * a.token_threads_m) >> 16;  // token of the block
+  const int group = threadIdx.x / a.token_threads;  // token of the block
   const int r = threadIdx.x - group * a.token_threads;
   const int64_t t = static_cast<int64_t>(blockIdx.x) * a.block_tokens + group;
   if (group >= a.block_tokens || t >= a.tokens) return;
-  const int hs = (r * a.units_m) >> 16, u = r - hs * a.units;
+  const int u = r % a.units, hs = r / a.units;
   const int pos = __ldg(a.positions + t);
   if (pos < 0 || pos >= a.table_rows) return;
   const int half = a.rotary / 2, heads = a.q.heads + a.k.heads;
@@ -219,9 +218,6 @@ cudaError_t launch_rope(RopeArgs a, int bf16, cudaStream_t stream) {
     a.head_step = step * a.units <= kRowThreads ? step : kRowThreads / a.units;
     a.token_threads = a.units * a.head_step;
     a.block_tokens = kRowThreads / a.token_threads;
-    // n / d = n ceil(2^16 / d) / 2^16 for n, d <= 128: the error is below n / 2^16 < 1 / d
-    a.units_m = (65536 + a.units - 1) / a.units;
-    a.token_threads_m = (65536 + a.token_threads - 1) / a.token_threads;
     const unsigned blocks = static_cast<unsigned>((a.tokens + a.block_tokens - 1) / a.block_tokens);
     auto go = [&](auto kernel) { kernel<<<blocks, kRowThreads, 0, stream>>>(a); };
     if (bf16) a.layout == 1 ? go(rope_rows_kernel<true, true>) : go(rope_rows_kernel<true, false>);
