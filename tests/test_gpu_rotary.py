@@ -34,6 +34,8 @@ def near(got, ref, tol):
     (4, 2, 2, 80, 34),        # a head that is no multiple of 32 values
     (3, 5, 1, 18, 2),         # nothing aligned
     (11, 40, 8, 128, 32),
+    (2, 100, 28, 256, 66),    # more heads than a block holds at a time
+    (1500, 2, 1, 64, 64),     # several heads a thread
 ])
 def test_matches_64_bits(pkg, cuda_dev, dtype, layout, n, hq, hk, dim, rotary):
     g = torch.Generator(device="cuda").manual_seed(n * dim + rotary)
@@ -48,8 +50,9 @@ def test_matches_64_bits(pkg, cuda_dev, dtype, layout, n, hq, hk, dim, rotary):
             assert torch.equal(y[..., rotary:], x[..., rotary:])
 
 
+@pytest.mark.parametrize("rotary", [128, 34, 64])
 @pytest.mark.parametrize("layout", ["half", "interleaved"])
-def test_strides_in_place_and_skipped_rows(pkg, cuda_dev, layout):
+def test_strides_in_place_and_skipped_rows(pkg, cuda_dev, layout, rotary):
     """q and k inside rows of a projection, rotated where they are; tokens with
     a position outside the table stay as they were, and so do the v columns."""
     g = torch.Generator(device="cuda").manual_seed(3)
@@ -57,12 +60,12 @@ def test_strides_in_place_and_skipped_rows(pkg, cuda_dev, layout):
     rows = torch.randn(n, 4096, generator=g, device="cuda").half()
     before = rows.clone()
     q, k = rows[:, :2048].view(n, 16, 128), rows[:, 2048:3072].view(n, 8, 128)
-    table = pkg.rotary.rope_table(50, 128)
+    table = pkg.rotary.rope_table(50, rotary)
     pos = torch.arange(n, dtype=torch.int32, device="cuda") * 3 - 3  # -3 .. 57
     pkg.rotary.rope(q, k, table, pos, layout=layout, q_out=q, k_out=k)
     inside = ((pos >= 0) & (pos < 50)).cpu()
     assert inside.sum() not in (0, n)
-    ref = po.rope(before[:, :3072].view(n, 24, 128), table, pos.clamp(0, 49), 128, layout, False)
+    ref = po.rope(before[:, :3072].view(n, 24, 128), table, pos.clamp(0, 49), rotary, layout, False)
     tol = po.rope_tolerance(before[:, :3072].view(n, 24, 128), ref, table, pos, torch.float16)
     near(rows[:, :3072].view(n, 24, 128)[inside], ref[inside], tol[inside])
     assert torch.equal(rows[~inside], before[~inside])
