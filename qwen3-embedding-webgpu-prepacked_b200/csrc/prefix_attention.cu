@@ -761,6 +761,11 @@ __global__ void __launch_bounds__(Layout<kFormat>::kThreads, 1)
     const float scale = args.scale_log2;
     const int token = row / args.group;  // of this row in its tile
     bool ok = true;
+    // a warp leaves a wait as one: what follows are instructions of whole warps
+    auto wait = [&](uint32_t b, uint32_t parity, int code) -> bool {
+      const bool got = mbar_wait(b, parity, abort_flag, args.status, code, wait_limit);
+      return __all_sync(0xffffffffu, got);
+    };
     // parities of this warpgroup's next key tile (bit 0), item with any (1) and
     // dual item (2)
     uint32_t ph = 0;
@@ -785,8 +790,7 @@ __global__ void __launch_bounds__(Layout<kFormat>::kThreads, 1)
       for (int j = j0; j < te; j += step, ph ^= 1u) {
         const PrefixTile tile = next;
         next = args.tiles[j + step < te ? j + step : j];
-        if (!(ok = mbar_wait(bar(L::kSFull + x), ph & 1u, abort_flag, args.status, kDevTimeoutSFull,
-                             wait_limit)))
+        if (!(ok = wait(bar(L::kSFull + x), ph & 1u, kDevTimeoutSFull)))
           break;
         tc_fence_after();
         const bool narrow = (tile.info & kTileWidthMask) <= 64;
@@ -872,8 +876,7 @@ __global__ void __launch_bounds__(Layout<kFormat>::kThreads, 1)
       int group = args.group, ln = lane;
       asm volatile("" : "+r"(group), "+r"(ln));
       if (j0 < te) {
-        if (!(ok = mbar_wait(bar(L::kOFinal + x), (ph >> 1) & 1u, abort_flag, args.status,
-                             kDevTimeoutOFinal, wait_limit)))
+        if (!(ok = wait(bar(L::kOFinal + x), (ph >> 1) & 1u, kDevTimeoutOFinal)))
           break;
         ph ^= 2u;
         tc_fence_after();
@@ -887,8 +890,7 @@ __global__ void __launch_bounds__(Layout<kFormat>::kThreads, 1)
         stat[x * 128 + row] = make_float2(m_run, l_run);
         tc_fence_before();
         mbar_arrive(bar(L::kStat + x));
-        if (!(ok = mbar_wait(bar(L::kStat + (x ^ 1)), (ph >> 2) & 1u, abort_flag, args.status,
-                             kDevTimeoutOFinal, wait_limit)))
+        if (!(ok = wait(bar(L::kStat + (x ^ 1)), (ph >> 2) & 1u, kDevTimeoutOFinal)))
           break;
         tc_fence_after();
         const float2 ml = stat[(x ^ 1) * 128 + row];
@@ -990,8 +992,7 @@ __global__ void __launch_bounds__(Layout<kFormat>::kThreads, 1)
       __syncwarp();
       if constexpr (kDual) {
         // the next item's P, and with it PV over O, only once both have read O
-        if (!(ok = mbar_wait(bar(L::kTaken + (x ^ 1)), (ph >> 2) & 1u, abort_flag, args.status,
-                             kDevTimeoutOFinal, wait_limit)))
+        if (!(ok = wait(bar(L::kTaken + (x ^ 1)), (ph >> 2) & 1u, kDevTimeoutOFinal)))
           break;
         ph ^= 4u;
       }
