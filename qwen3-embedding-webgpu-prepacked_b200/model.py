@@ -39,7 +39,7 @@ from . import attention as attn
 from . import ffn, matmul, norm, prepacked, rotary
 from .kv_cache import KVCache, kv_cache_write
 from .pooling import last_token_pool
-from .prefix import prefix_attention
+from .prefix import _capturing, prefix_attention
 
 HIDDEN, INTERMEDIATE, Q_WIDTH, LAYERS = 1024, 3072, 2048, 28  # model.ts:18-21
 EPSILON = 1e-6
@@ -139,18 +139,23 @@ class Qwen3EmbeddingModel:
                                for key in ("attn_norm", "attn_q_norm", "attn_k_norm",
                                            "ffn_norm")})
         self.output_norm = weights.weight("output_norm.weight").float().contiguous()
-        self._rope: Optional[torch.Tensor] = None  # table of requests behind a prefix
+        self._rope: List[torch.Tensor] = []  # tables of requests behind a prefix
 
     def _rope_rows(self, first: int, count: int) -> torch.Tensor:
         """(cos, sin) rows of positions ``first`` .. ``first + count - 1`` at least."""
         need = first + count
-        if self._rope is None or self._rope.shape[0] < need:
+        if not self._rope or self._rope[-1].shape[0] < need:
+            if _capturing(attn.Context.for_device(torch.device(self.device).index).device):
+                raise ValueError("positions met for the first time: run once before the capture")
             rows = 1024
             while rows < need:
                 rows *= 2
-            self._rope = rotary.rope_table(rows, attn.HEAD_DIM, attn.ROPE_THETA,
-                                           device=self.device)
-        return self._rope[first:]
+            # Shorter tables stay: launches on their way and captured graphs read
+            # them. Waited for, so that any stream may use the new one.
+            self._rope.append(rotary.rope_table(rows, attn.HEAD_DIM, attn.ROPE_THETA,
+                                                device=self.device))
+            torch.cuda.current_stream(self.device).synchronize()
+        return self._rope[-1][first:]
 
     def cache_prefix(self, ids: torch.Tensor, format: str = "e4m3",
                      mode: int = attn.MODE_AUTO) -> CachedPrefix:
@@ -192,6 +197,8 @@ class Qwen3EmbeddingModel:
                           default=0)
             rope_rows = self._rope_rows(prefix.length, longest)
         if store is not None:
+            if len(store) < self.layers or any(c.slots < T for c in store):
+                raise ValueError("store needs a cache of all tokens for each layer")
             slots = torch.arange(T, dtype=torch.int32, device=dev)
         f16 = dict(dtype=torch.float16, device=dev)
         x = ffn.embedding_lookup(ids, self.embed_table, HIDDEN, self.vocab)

@@ -94,3 +94,38 @@ def test_refusals(pkg, cuda_dev, model):
     cached.caches.pop()
     with pytest.raises(ValueError):
         model.embed(torch.zeros(3, dtype=torch.int32, device="cuda"), [0, 3], prefix=cached)
+    # caches that do not hold all tokens, or not all layers
+    ids = torch.zeros(6, dtype=torch.int32, device="cuda")
+    caches = [pkg.kv_cache.KVCache(5) for _ in range(3)]
+    with pytest.raises(ValueError):
+        model.forward(ids, [0, 6], store=caches)
+    with pytest.raises(ValueError):
+        model.forward(ids[:5], [0, 5], store=caches[:2])
+
+
+def test_captured_before_longer_requests(pkg, cuda_dev, model):
+    """A captured graph keeps its rotary table when longer requests need another;
+    positions met for the first time are refused inside a capture."""
+    rng = np.random.default_rng(11)
+    (head,), parts = tokens(rng, [300]), tokens(rng, [20, 9])
+    cached = model.cache_prefix(on_gpu([head])[0])
+    ids, cu = on_gpu(parts)
+    ref = model.forward(ids, cu, prefix=cached)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = model.forward(ids, cu, prefix=cached)
+        far = pkg.model.CachedPrefix(10 ** 6, cached.mode, cached.caches)
+        with pytest.raises(ValueError, match="before the capture"):
+            model.forward(ids, cu, prefix=far)
+    longer = on_gpu(tokens(rng, [2500]))
+    side = torch.cuda.Stream()
+    model.forward(*longer, prefix=cached)
+    with torch.cuda.stream(side):  # the new table serves any stream
+        again = model.forward(ids, cu, prefix=cached)
+    side.synchronize()
+    junk = [torch.full((1024, 64, 2), float("nan"), device="cuda") for _ in range(8)]
+    out.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    del junk
+    assert torch.equal(out, ref) and torch.equal(again, ref)
