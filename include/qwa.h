@@ -370,7 +370,7 @@ typedef struct qwa_rope_tensor {
  * in f32, rounded once. inverse != 0 takes -s: the way back, which is also the
  * gradient (dx from dy). positions_device: DEVICE int32 [tokens]; a token
  * whose position is not in 0..table_rows-1 is skipped, nothing of it is
- * written. head_dim 2..1024; rotary_dim even, at most head_dim and 256. Rows,
+ * written. head_dim 2..1024, heads to 2^20; rotary_dim even, at most head_dim and 256. Rows,
  * strides and pointers in multiples of 16 bytes take the fast path. */
 QWA_API qwa_status qwa_rope(qwa_ctx *ctx, int dtype, const qwa_rope_tensor *q,
                             const qwa_rope_tensor *k, int tokens, int head_dim, int rotary_dim,
@@ -385,7 +385,7 @@ typedef enum qwa_kv_format {
 
 /* Key/value cache, all device memory of the caller: k, v [slots, heads,
  * head_dim] of 16-bit values or 8-bit codes; k_scale, v_scale (8-bit formats)
- * [slots, heads] bytes e + 127. A value is code * 2^e. dtype: of the 16-bit values that
+ * [slots, heads] bytes e + 127, 2^e a number of dtype. A value is code * 2^e. dtype: of the 16-bit values that
  * are written and read. head_dim a power of two in 16..256; k and v 16-byte
  * aligned. */
 typedef struct qwa_kv_cache {

@@ -1090,12 +1090,15 @@ bool good_dtype(int dtype) { return dtype == QWA_F16 || dtype == QWA_BF16; }
 // One of rope's tensors: its pointers and strides, in 16-bit values.
 qwa_status check_rope_side(qwa_ctx* ctx, const qwa_rope_tensor* t, int tokens, int head_dim,
                            const char* name) {
-  if (t->heads < 1) return fail(ctx, QWA_ERR_INVALID_ARG, "%s: heads must be >= 1", name);
+  if (t->heads < 1 || t->heads > (1 << 20))
+    return fail(ctx, QWA_ERR_INVALID_ARG, "%s: heads must be in 1..2^20", name);
   if (!t->in || !t->out) return fail(ctx, QWA_ERR_INVALID_ARG, "%s: NULL tensor pointer", name);
   if ((reinterpret_cast<uintptr_t>(t->in) & 1u) || (reinterpret_cast<uintptr_t>(t->out) & 1u))
     return fail(ctx, QWA_ERR_INVALID_ARG, "%s: pointers must be 2-byte aligned", name);
-  if (t->in_stride < 0 || t->in_head_stride < 0 || t->out_stride < 0 || t->out_head_stride < 0)
-    return fail(ctx, QWA_ERR_INVALID_ARG, "%s: strides must be >= 0", name);
+  constexpr int64_t kMost = 1ll << 40;
+  for (int64_t s : {t->in_stride, t->in_head_stride, t->out_stride, t->out_head_stride})
+    if (s < 0 || s > kMost)
+      return fail(ctx, QWA_ERR_INVALID_ARG, "%s: strides must be in 0..2^40", name);
   // heads inside a token's row, or tokens inside a head's
   const bool token_major =
       (t->heads == 1 || t->out_head_stride >= head_dim) &&
@@ -1105,8 +1108,8 @@ qwa_status check_rope_side(qwa_ctx* ctx, const qwa_rope_tensor* t, int tokens, i
       (t->heads == 1 || t->out_head_stride >= (tokens - 1) * t->out_stride + head_dim);
   if (!token_major && !head_major)
     return fail(ctx, QWA_ERR_INVALID_ARG, "%s: output strides let rows overlap", name);
-  if (t->in == t->out &&
-      (t->in_stride != t->out_stride || t->in_head_stride != t->out_head_stride))
+  if (t->in == t->out && ((tokens > 1 && t->in_stride != t->out_stride) ||
+                          (t->heads > 1 && t->in_head_stride != t->out_head_stride)))
     return fail(ctx, QWA_ERR_INVALID_ARG, "%s: in place needs equal strides", name);
   return QWA_OK;
 }
@@ -1553,10 +1556,10 @@ qwa_status qwa_prefix_attention(qwa_ctx* ctx, const qwa_prefix_plan* plan, int d
     if (cache->dtype != dtype || cache->heads != s.kv_heads || cache->head_dim != kHeadDim)
       return fail(ctx, QWA_ERR_INVALID_ARG,
                   "the cache must have q's dtype, %d heads and head_dim 128", s.kv_heads);
-    if (first_slot < 0 || first_slot + s.prefix_len > cache->slots)
+    if (first_slot < 0 || first_slot > cache->slots - s.prefix_len)
       return fail(ctx, QWA_ERR_INVALID_ARG, "the prefix's slots %lld..%lld are not in the cache",
                   static_cast<long long>(first_slot),
-                  static_cast<long long>(first_slot + s.prefix_len - 1));
+                  static_cast<long long>(first_slot) + s.prefix_len - 1);
     format = cache->format;
   }
   if ((st = ensure_encode(ctx)) != QWA_OK) return st;

@@ -93,7 +93,7 @@ inline PrefixWork build_prefix_work(const PrefixShape& s, const int32_t* cu_q,
   const int total = cu_q[s.batch];
   const int P = s.prefix_len;
   // sparse_prefix reaches into the own keys by this many
-  const int own_prefix = s.sparse ? std::max(0, s.sparse_prefix - P) : 0;
+  const int64_t own_prefix = s.sparse ? std::max(0, s.sparse_prefix - P) : 0;
   w.rows.resize(total);
   std::vector<int> request_of(total);
   for (int b = 0; b < s.batch; ++b) {
@@ -196,7 +196,7 @@ inline PrefixWork build_prefix_work(const PrefixShape& s, const int32_t* cu_q,
         add_span(g.lo, g.last_hi + 1ll);
         continue;
       }
-      add_span(g.lo, std::min<int64_t>(g.last_hi + 1ll, static_cast<int64_t>(g.lo) + own_prefix));
+      add_span(g.lo, std::min<int64_t>(g.last_hi + 1ll, g.lo + own_prefix));
       add_span(std::max<int64_t>(g.lo, static_cast<int64_t>(g.first_hi) - s.window + 1),
                g.last_hi + 1ll);
     }

@@ -52,7 +52,8 @@ class KVCache:
              v_scale: Optional[torch.Tensor] = None,
              dtype: Optional[torch.dtype] = None) -> "KVCache":
         """A cache over tensors that exist already: codes (float8_e4m3fn or int8)
-        with their scales (uint8 [slots, heads]), or 16-bit values without.
+        with their scales (uint8 [slots, heads]: e + 127, where 2^e is a number of
+        ``dtype``), or 16-bit values without.
         ``dtype``: of the rows written and read (float16 unless k has one)."""
         self = cls.__new__(cls)
         if dtype is None:

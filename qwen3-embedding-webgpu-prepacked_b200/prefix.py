@@ -28,6 +28,30 @@ from .kv_cache import _DTYPES, FORMATS, KVCache
 
 
 _retired: list = []  # lists of plans that ended during a capture
+_create_lock = threading.Lock()  # a context makes one plan at a time
+
+
+def _lengths(cu) -> Optional[tuple]:
+    """Host offsets as a tuple of Python ints (of a tensor: by value)."""
+    if cu is None:
+        return None
+    return tuple(cu.tolist()) if isinstance(cu, torch.Tensor) else tuple(cu)
+
+
+def _int32(**values) -> None:
+    for name, value in values.items():
+        _need(-2 ** 31 <= value < 2 ** 31, f"{name} must be a 32-bit number")
+
+
+def _cu_arrays(cu_seqlens, cu_seqlens_k):
+    cu_q, cu_k = _lengths(cu_seqlens), _lengths(cu_seqlens_k)
+    _need(len(cu_q) >= 2, "cu_seqlens needs at least one request")
+    _need(cu_k is None or len(cu_k) == len(cu_q),
+          "cu_seqlens and cu_seqlens_k must be of the same requests")
+    for cu in (cu_q, cu_k or cu_q):
+        _int32(cu_seqlens=min(cu))
+        _int32(cu_seqlens=max(cu))
+    return _lib.cu_array(cu_q), _lib.cu_array(cu_k) if cu_k is not None else None
 
 
 class PrefixPlan:
@@ -42,20 +66,19 @@ class PrefixPlan:
                  ctx: Optional[Context] = None):
         self.ctx = ctx if ctx is not None else Context.for_device(device)
         self.handle = None
-        cu_q = _lib.cu_array(cu_seqlens)
-        cu_k = _lib.cu_array(cu_seqlens_k) if cu_seqlens_k is not None else None
-        _need(len(cu_q) >= 2, "cu_seqlens needs at least one request")
-        _need(cu_k is None or len(cu_k) == len(cu_q),
-              "cu_seqlens and cu_seqlens_k must be of the same requests")
+        cu_q, cu_k = _cu_arrays(cu_seqlens, cu_seqlens_k)
+        _int32(prefix_len=prefix_len, q_heads=q_heads, kv_heads=kv_heads, mode=mode,
+               sparse_prefix=sparse_prefix, window=window)
         _need(not _capturing(self.ctx.device),
               "a plan allocates memory: make it before the capture")
         while _retired:
             lib, old = _retired.pop()
             lib.qwa_prefix_plan_destroy(old)
         h = ctypes.c_void_p()
-        _lib.check(self.ctx.lib.qwa_prefix_plan_create(
-            self.ctx.handle, cu_q, cu_k, len(cu_q) - 1, q_heads, kv_heads, prefix_len, mode,
-            sparse_prefix, window, ctypes.byref(h)), self.ctx.handle)
+        with _create_lock:
+            _lib.check(self.ctx.lib.qwa_prefix_plan_create(
+                self.ctx.handle, cu_q, cu_k, len(cu_q) - 1, q_heads, kv_heads, prefix_len, mode,
+                sparse_prefix, window, ctypes.byref(h)), self.ctx.handle)
         self.handle = h
         self.queries = cu_q[len(cu_q) - 1]
         self.keys = cu_k[len(cu_k) - 1] if cu_k is not None else self.queries
@@ -203,20 +226,26 @@ def prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     [own keys, kv_heads, 128]. ``cu_seqlens`` (host) cuts q into requests, ``cu_seqlens_k``
     k and v (None: the same); a request's queries are the last of its keys.
     Lengths met before reuse their plan; inside a capture they must have been
-    met before it."""
+    met before it, and a captured ``stream`` must be the current one."""
     q_shape, k_shape = q.shape, k.shape
     _need(q.is_cuda and len(q_shape) == 3 and len(k_shape) == 3,
           "q and k must be CUDA tensors [tokens, heads, 128]")
     ctx = Context.for_device(q.get_device())
-    plan = _plan_for(ctx, tuple(cu_seqlens),
-                     tuple(cu_seqlens_k) if cu_seqlens_k is not None else None, prefix_len,
+    if stream is not None:
+        if not isinstance(stream, torch.cuda.Stream):
+            stream = torch.cuda.ExternalStream(int(stream), device=q.device)
+        if not _capturing(ctx.device):
+            # the graph would keep neither the plan nor a workspace
+            with torch.cuda.stream(stream):
+                _need(not torch._C._cuda_isCurrentStreamCapturing(),
+                      "a captured stream must be the current one")
+    plan = _plan_for(ctx, _lengths(cu_seqlens), _lengths(cu_seqlens_k), prefix_len,
                      q_shape[1], k_shape[1], mode, sparse_prefix, window)
     out, workspace, args = _attention_args(ctx, plan, q, k, v, out, cache, first_slot)
     _launch(ctx, stream, ctx.lib.qwa_prefix_attention, plan.handle, *args)
     if workspace is not None and stream is not None:
         # its memory must not be handed out again before that stream is done with it
-        workspace.record_stream(stream if isinstance(stream, torch.cuda.Stream) else
-                                torch.cuda.ExternalStream(int(stream), device=q.device))
+        workspace.record_stream(stream)
     return out
 
 
@@ -225,10 +254,9 @@ def prefix_attention_work(cu_seqlens: Sequence[int], prefix_len: int, q_heads: i
                           mode: int = MODE_AUTO, sparse_prefix: int = PREFIX,
                           window: int = WINDOW):
     """(kept pairs per query head, key tiles visited over all kv heads) of one call."""
-    cu_q = _lib.cu_array(cu_seqlens)
-    cu_k = _lib.cu_array(cu_seqlens_k) if cu_seqlens_k is not None else None
-    _need(cu_k is None or len(cu_k) == len(cu_q),
-          "cu_seqlens and cu_seqlens_k must be of the same requests")
+    cu_q, cu_k = _cu_arrays(cu_seqlens, cu_seqlens_k)
+    _int32(prefix_len=prefix_len, q_heads=q_heads, kv_heads=kv_heads, mode=mode,
+           sparse_prefix=sparse_prefix, window=window)
     pairs, tiles = ctypes.c_int64(), ctypes.c_int64()
     _lib.check(_lib.load().qwa_prefix_attention_work(
         cu_q, cu_k, len(cu_q) - 1, q_heads, kv_heads, prefix_len, mode, sparse_prefix, window,

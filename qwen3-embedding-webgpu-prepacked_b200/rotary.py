@@ -54,7 +54,8 @@ def rope_table(positions: int, rotary_dim: int = 128, theta: float = ROPE_THETA,
                out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
     """f32 [positions, rotary_dim / 2, 2]: (cos, sin) of positions ``first``,
     ``first`` + 1, ... with the angle in 64 bits."""
-    _need(positions >= 0 and rotary_dim >= 2, "positions must be >= 0 and rotary_dim >= 2")
+    _need(0 <= positions < 2 ** 31 and rotary_dim >= 2,
+          "positions must be in 0..2^31-1 and rotary_dim >= 2")
     if out is not None:
         _need(out.is_cuda and out.dtype == torch.float32 and out.is_contiguous()
               and out.numel() >= positions * (rotary_dim // 2) * 2,
@@ -76,7 +77,7 @@ def _side(x: torch.Tensor, y: Optional[torch.Tensor], name: str, tokens: int, di
     """Checks one of q and k with its output (None: one is made); the output and
     their qwa_rope_tensor."""
     shape = x.shape
-    if len(shape) != 3 or shape[0] != tokens or shape[2] != dim:
+    if len(shape) != 3 or shape[0] != tokens or shape[2] != dim or shape[1] >= 2 ** 31:
         raise ValueError(f"{name} must be [tokens, heads, head_dim] as the others")
     if x.dtype != dtype or x.get_device() != index:
         raise ValueError(f"{name} must agree with the others in dtype and device")
@@ -104,6 +105,8 @@ def _rope_args(ctx: Context, q, k, table, positions, q_output, k_output, layout,
     if order is None:
         raise ValueError("layout must be 'half' or 'interleaved'")
     tokens, _, dim = shape
+    if tokens >= 2 ** 31:
+        raise ValueError("at most 2^31 - 1 tokens")
     rows, half, two = table.shape
     if two != 2 or table.dtype != torch.float32 or table.get_device() != index \
             or not table.is_contiguous():

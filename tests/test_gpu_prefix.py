@@ -331,3 +331,54 @@ def test_refusals(pkg, cuda_dev):
     plan.close()
     with pytest.raises(ValueError):
         pkg.attention.encode_run(None, run.commands[0])
+    with pytest.raises(pkg._lib.QwaError):            # first_slot + 60 is past 64 bits
+        fn(q, k, v, cu, cache, 60, first_slot=2 ** 63 - 20)
+
+
+def test_two_threads_at_once(pkg, cuda_dev):
+    """Each thread makes its own plans and calls on its own stream."""
+    import threading
+    work = []
+    for seed in range(4):
+        p = problem(pkg, seed, [seed + 1, 40 + seed], [seed + 1, 40 + seed], 600, 16, 8,
+                    torch.float16, "e4m3")
+        work.append((p, check(pkg, p, 600, FULL)))
+    pkg.prefix._plans.clear()
+    torch.cuda.synchronize()
+    got, barrier = {}, threading.Barrier(4)
+
+    def run(i):
+        q, k, v, cache, _, _, cu, _ = work[i][0]
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            barrier.wait(10)
+            for _ in range(20):
+                out = pkg.prefix.prefix_attention(q, k, v, cu, cache, 600, mode=FULL)
+            stream.synchronize()
+            got[i] = out
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    for i, (_, ref) in enumerate(work):
+        assert torch.equal(got[i], ref)
+
+
+def test_captured_stream_must_be_the_current_one(pkg, cuda_dev):
+    """A graph keeps its plan and its workspace only where the capture is that of
+    the current stream."""
+    q, k, v, cache, _, _, cu, _ = problem(pkg, 1, [30] * 20, [30] * 20, 600, 16, 8, torch.float16,
+                                          "e4m3")
+    ref = pkg.prefix.prefix_attention(q, k, v, cu, cache, 600)
+    side, out = torch.cuda.Stream(), torch.empty_like(ref)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            with pytest.raises(ValueError, match="current one"):
+                pkg.prefix.prefix_attention(q, k, v, cu, cache, 600, out=out, stream=side)
+        pkg.prefix.prefix_attention(q, k, v, cu, cache, 600, out=out)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, ref)

@@ -238,3 +238,9 @@ def test_refusals(pkg, cuda_dev):
     empty = torch.zeros(0, 2, 64, dtype=torch.float16, device="cuda")
     assert rot.rope(empty, None, table, pos)[0].shape == (0, 2, 64)
     assert rot.rope_table(0, 64).shape == (0, 32, 2)
+    with pytest.raises(pkg._lib.QwaError):  # more heads than 2^20
+        rot.rope(q[:1, :1].expand(1, 2 ** 20 + 1, 64), None, table, pos)
+    # in place, where a single token has no stride of its own
+    one = q[:1]
+    assert rot.rope(one, None, table, pos, q_out=one.as_strided((1, 2, 64), (999, 64, 1)))[0] \
+        is not None
