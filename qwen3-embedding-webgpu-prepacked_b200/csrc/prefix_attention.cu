@@ -11,31 +11,43 @@
 // multiplied once for the whole block; own keys of other requests are masked.
 //
 // Warp roles:
-//   warp 0      TMA producer: Q tiles, then K_j / V_j into a 3-slot ring
+//   warp 0      TMA producer: Q, then K_j / V_j into a ring of 4 slots (16-bit
+//               prefix) or 3 (8-bit; raw prefix tiles into a ring of 3 stages). Q is
+//               loaded again once the last S of an item is done
 //   warp 1      TMEM owner; lane 0 issues every tcgen05.mma and commit
 //   warps 4-7   softmax of tile A, one thread a row
 //   warps 8-11  softmax of tile B
-//   warps 2-3 (16-bit prefix) or 12-15 (8-bit) prepare tiles: 8-bit prefix tiles
-//               are read with plain loads, converted and written to their
-//               slot; V tiles with masked keys are cleared of values that are
-//               not finite (guard, below)
+//   warps 2-3 (16-bit prefix) or 12-15 (8-bit) prepare tiles: raw 8-bit tiles are
+//               converted into their slot; V tiles with masked keys are cleared of
+//               values that are not finite (guard, below)
 // TMEM: S_A, S_B (P over them, as 16-bit pairs), O_A, O_B; 512 columns.
 // MMA order per key tile: S_A(j), PV_B(j-1), S_B(j), PV_A(j), so the softmax of
 // one tile runs under the MMAs of the other.
 // In the dual form (few blocks: each has one row tile) the key tiles of a block
 // alternate between A and B, both over the same Q, and the two O are merged in
 // tensor memory at the end. It has kernels of its own: with both forms in one, the
-// softmax warps spilled registers (4 x 5000 tokens 3% slower).
+// softmax warps spilled registers (4 x 5000 tokens 3% slower). For the same reason a launch
+// has blocks of one form only: cutting the last round's blocks into one row tile each
+// made 16 x 500 tokens 202 us instead of 195.
 //
 // Guard. A masked key has p = 0, but the MMA still multiplies: 0 * inf = NaN
 // would reach rows of other requests. So V tiles in which some row drops a key
 // are searched, values that are not finite replaced by 0, and the rows that
 // keep such a key get it back in the epilogue (found again by a slow search).
 //
-// Split. With few blocks the tiles of a block are dealt to a cluster of 2, 4 or
-// 8 CTAs, each with its own running maximum and sum; at the end every CTA
+// Split. With few blocks the tiles of a block are dealt to a cluster of 2 to 8
+// CTAs, each with its own running maximum and sum; at the end every CTA
 // leaves its O, m and l in shared memory and merges a share of the rows from
 // all of them. No workspace, one launch, and an order that does not vary.
+//
+// What bounds it (16/8 heads). Long requests: a key tile of two row tiles takes about
+// 4070 cycles, twice its MMAs: S waits for PV, as P lies over it, and the
+// exponentials of one row tile take longer than the MMAs of the other. 4 x 5000 bf16
+// tokens behind 5000: 1215 to 1340 us with the clock, 920 to 1010 TFLOP/s (0.56 to 0.62 of
+// measured). 16 x 500 f16 behind 2000 in E4M3: 195 us, 755 TFLOP/s; 504 blocks for 148
+// SMs, so the fourth round is less than half full. Small calls: latency. 16 x 1 behind 1000
+// in E4M3: 12.3 us, 16 x 15..150 behind 176: 16.1 us; loads, S, softmax, PV, merge and
+// the launch follow one another, on instructions that are not cached yet.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
