@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libqwa.so")
@@ -36,19 +37,10 @@ class RopeScalingStruct(ctypes.Structure):
                 ("high_freq_factor", F64)]
 
 
-class RopeTensor(ctypes.Structure):
-    """qwa_rope_tensor"""
-    _fields_ = [("in_", P), ("in_stride", I64), ("in_head_stride", I64), ("out", P),
-                ("out_stride", I64), ("out_head_stride", I64), ("heads", I32)]
-
-
-class KvCacheStruct(ctypes.Structure):
-    """qwa_kv_cache"""
-    _fields_ = [("dtype", I32), ("format", I32), ("heads", I32), ("head_dim", I32),
-                ("slots", I64), ("k", P), ("v", P), ("k_scale", P), ("v_scale", P)]
-
-
-RopeTensorP, KvCacheP = ctypes.POINTER(RopeTensor), ctypes.POINTER(KvCacheStruct)
+# qwa_rope_tensor and qwa_kv_cache as bytes, in the order of their fields: a call takes
+# them as a pointer, and they are made in a quarter of a ctypes structure's time
+rope_tensor = struct.Struct("@PqqPqqi4x").pack
+kv_cache = struct.Struct("@iiiiqPPPP").pack
 
 # name -> (restype, argtypes); the exported surface of include/qwa.h
 SIGNATURES = {
@@ -81,15 +73,15 @@ SIGNATURES = {
     "qwa_last_token_pool": (I32, [P, P, I32, P, I32P, I32, P]),
     "qwa_last_token_pool_padded": (I32, [P, P, P, P, I32, I32, I32, P]),
     "qwa_rope_table": (I32, [P, P, I64, I32, I32, F64, ctypes.POINTER(RopeScalingStruct), P]),
-    "qwa_rope": (I32, [P, I32, RopeTensorP, RopeTensorP, I32, I32, I32, I32, I32, P, P, I32, P]),
-    "qwa_kv_cache_write": (I32, [P, KvCacheP, P, I64, P, I64, P, I32, P]),
-    "qwa_kv_cache_read": (I32, [P, KvCacheP, P, I32, P, P, P]),
+    "qwa_rope": (I32, [P, I32, P, P, I32, I32, I32, I32, I32, P, P, I32, P]),
+    "qwa_kv_cache_write": (I32, [P, P, P, I64, P, I64, P, I32, P]),
+    "qwa_kv_cache_read": (I32, [P, P, P, I32, P, P, P]),
     "qwa_prefix_plan_create": (I32, [P, I32P, I32P, I32, I32, I32, I32, I32, I32, I32,
                                      ctypes.POINTER(P)]),
     "qwa_prefix_plan_destroy": (I32, [P]),
     "qwa_prefix_plan_deal": (I32, [P, ctypes.POINTER(I32), ctypes.POINTER(I32)]),
     "qwa_prefix_attention_workspace": (ctypes.c_size_t, [P, I32]),
-    "qwa_prefix_attention": (I32, [P, P, I32, P, I64, P, I64, P, I64, P, KvCacheP, I64, P,
+    "qwa_prefix_attention": (I32, [P, P, I32, P, I64, P, I64, P, I64, P, P, I64, P,
                                    ctypes.c_size_t, P]),
     "qwa_prefix_attention_work": (I32, [I32P, I32P, I32, I32, I32, I32, I32, I32, I32, I64P,
                                         I64P]),

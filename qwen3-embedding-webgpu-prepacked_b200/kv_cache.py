@@ -15,7 +15,6 @@ csrc/kv_cache.cu through the C ABI. The reference keeps no cache.
 """
 from __future__ import annotations
 
-import ctypes
 from typing import Optional, Tuple
 
 import torch
@@ -73,7 +72,7 @@ class KVCache:
               and v.get_device() == index and k.is_contiguous() and v.is_contiguous(),
               "k and v must be contiguous CUDA tensors [slots, heads, head_dim] of one kind")
         slots, heads, dim = shape
-        ks = vs = None
+        ks = vs = 0
         if fmt == "none":
             _need(k_scale is None and v_scale is None, "16-bit values have no scales")
         else:
@@ -87,8 +86,8 @@ class KVCache:
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.format, self.dtype, self.index = fmt, dtype, index
         self.slots, self.heads, self.head_dim = slots, heads, dim
-        self.struct = _lib.KvCacheStruct(code, FORMATS[fmt], heads, dim, slots, k.data_ptr(),
-                                         v.data_ptr(), ks, vs)
+        self.struct = _lib.kv_cache(code, FORMATS[fmt], heads, dim, slots, k.data_ptr(),
+                                    v.data_ptr(), ks, vs)
 
     @property
     def device(self) -> torch.device:
@@ -121,7 +120,7 @@ def _write_args(ctx: Context, cache: KVCache, k, v, slots) -> tuple:
     index = ctx.device
     _need(cache.index == index, "the cache must be on the kernel's device")
     n = _slots(slots, index)
-    return (ctypes.byref(cache.struct), k.data_ptr(), _rows(k, "k", cache, n, index),
+    return (cache.struct, k.data_ptr(), _rows(k, "k", cache, n, index),
             v.data_ptr(), _rows(v, "v", cache, n, index), slots.data_ptr(), n)
 
 
@@ -139,7 +138,7 @@ def _read_args(ctx: Context, cache: KVCache, slots, k_output, v_output):
         v_output = torch.empty_like(k_output)
     else:
         _need(_rows(v_output, "v_output", cache, n, index) == width, "v_output must be contiguous")
-    return k_output, v_output, (ctypes.byref(cache.struct), slots.data_ptr(), n,
+    return k_output, v_output, (cache.struct, slots.data_ptr(), n,
                                 k_output.data_ptr(), v_output.data_ptr())
 
 

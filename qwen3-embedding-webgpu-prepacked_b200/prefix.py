@@ -135,7 +135,7 @@ def _attention_args(ctx: Context, plan: PrefixPlan, q, k, v, output, cache, firs
     need = 0
     if cache is not None:
         _need(cache.index == index, "the cache must be on q's device")
-        struct = ctypes.byref(cache.struct)
+        struct = cache.struct
         need = plan.workspace[cache.format]
         if need:
             workspace = q.new_empty(need, dtype=torch.uint8)

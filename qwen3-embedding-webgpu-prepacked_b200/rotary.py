@@ -91,7 +91,7 @@ def _side(x: torch.Tensor, y: Optional[torch.Tensor], name: str, tokens: int, di
         y0, y1, y2 = y.stride()
     if x2 != 1 or y2 != 1:
         raise ValueError(f"{name}: a head's values must be contiguous")
-    return y, _lib.RopeTensor(x.data_ptr(), x0, x1, y.data_ptr(), y0, y1, shape[1])
+    return y, _lib.rope_tensor(x.data_ptr(), x0, x1, y.data_ptr(), y0, y1, shape[1])
 
 
 def _rope_args(ctx: Context, q, k, table, positions, q_output, k_output, layout, inverse):
@@ -118,10 +118,8 @@ def _rope_args(ctx: Context, q, k, table, positions, q_output, k_output, layout,
     qs = ks = None
     if q is not None:
         q_output, qs = _side(q, q_output, "q", tokens, dim, dtype, index)
-        qs = ctypes.byref(qs)
     if k is not None:
         k_output, ks = _side(k, k_output, "k", tokens, dim, dtype, index)
-        ks = ctypes.byref(ks)
     return q_output, k_output, (code, qs, ks, tokens, dim, 2 * half, order, 1 if inverse else 0,
                                 positions.data_ptr(), table.data_ptr(), rows)
 
