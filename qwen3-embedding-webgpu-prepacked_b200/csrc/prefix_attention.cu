@@ -73,6 +73,7 @@ struct Layout {
   static constexpr int kThreads = kConverts ? 512 : 384;
   static constexpr int kPrepWarp0 = kConverts ? 12 : 2;
   static constexpr int kPrepWarps = kConverts ? 4 : 2;
+  static constexpr int kSlotEmptyArrivals = slot_empty_arrivals(kPrepWarps);
   static constexpr int kRegsLaunch = kConverts ? 128 : 168;
   static constexpr int kRegsSupport = kConverts ? 72 : 104;  // producer and issuer
   static constexpr int kRegsPrep = 72;                       // of the fourth warpgroup
@@ -394,7 +395,9 @@ __device__ __forceinline__ void share_tiles(const Share& s, const PrefixItem& it
 // The preparing warps (the file's head): w counts them from 0. They follow every
 // use of the ring, because a parity says nothing to a role that is more than a
 // phase away: each waits for its slot to be empty, then converts, or (8 bits) lets
-// the producer, which runs ahead on raw tiles, load an own tile.
+// the producer, which runs ahead on raw tiles, load an own tile. A slot is empty again
+// only with an arrival of each of them, so none falls more than a phase behind
+// (slot_empty_arrivals).
 template <bool kBf16, int kFormat, bool kSplit>
 __device__ __forceinline__ void prepare_tiles(const PrefixArgs& args, const Share& share,
                                               uint32_t sbase, int w, int lane,
@@ -467,6 +470,8 @@ __device__ __forceinline__ void prepare_tiles(const PrefixArgs& args, const Shar
                     li);
           }
         }
+        // every lane is here: `wait` and `publish` gather the warp
+        if (lane == 0) mbar_arrive(bar(L::kSlotEmpty + s));
         if (++s == L::kSlots) {
           s = 0;
           parity ^= 1;
@@ -509,7 +514,7 @@ __global__ void __launch_bounds__(Layout<kFormat>::kThreads, 1)
     mbar_init(bar(L::kQEmpty), 1);
     *bad_item = 0;
     for (int i = 0; i < L::kSlots; ++i) {
-      mbar_init(bar(L::kSlotEmpty + i), 1);
+      mbar_init(bar(L::kSlotEmpty + i), L::kSlotEmptyArrivals);
       mbar_init(bar(L::kLanded + i), 1);
       mbar_init(bar(L::kReady + i), L::kPrepWarps);
       mbar_init(bar(L::kOwnGo + i), 1);

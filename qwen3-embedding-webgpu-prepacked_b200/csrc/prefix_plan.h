@@ -59,6 +59,13 @@ struct PrefixShape {
 // us.
 constexpr double kTileUs = 2.14, kDualTileUs = 1.325;
 
+// Arrivals that free a slot of the kernel's ring of key tiles: the commit of the MMAs
+// that read it, and each preparing warp's, once it is done with that use. A parity tells
+// two neighbouring phases apart and no more. Without their arrivals nothing waited
+// for the preparing warps on tiles that need no preparing, and one that was late by a
+// whole ring would have taken a phase for the one before it, and never caught up.
+constexpr int slot_empty_arrivals(int prep_warps) { return 1 + prep_warps; }
+
 struct PrefixWork {
   std::vector<PrefixItem> items;  // without the head; one per block
   std::vector<PrefixTile> tiles;
