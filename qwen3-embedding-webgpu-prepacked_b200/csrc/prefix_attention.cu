@@ -111,7 +111,8 @@ struct Layout {
   static constexpr uint32_t kLimitOff = kHolderOff + 8;
   // li + 1 of the last item with values put aside. The preparing warps may be
   // ahead of an epilogue: it takes a later item's number for its own, and its search
-  // then finds what there is.
+  // then finds what there is. They may be ahead of one another too, so the number
+  // only rises: a late warp must not take back what another has noted.
   static constexpr uint32_t kBadOff = kLimitOff + 8;
   static constexpr uint32_t kSmemUsed = kBadOff + 4;
   static constexpr uint32_t kSmemBytes = kSmemUsed;
@@ -403,7 +404,7 @@ __device__ __forceinline__ void prepare_tiles(const PrefixArgs& args, const Shar
                                               uint32_t sbase, int w, int lane,
                                               volatile int* abort_flag,
                                               const volatile unsigned long long* wait_limit,
-                                              volatile int* bad_item) {
+                                              int* bad_item) {
   using L = Layout<kFormat>;
   auto bar = [&](int i) -> uint32_t { return sbase + L::kBarOff + 8u * i; };
   // a warp-wide wait: every lane leaves it with the same answer
@@ -412,7 +413,7 @@ __device__ __forceinline__ void prepare_tiles(const PrefixArgs& args, const Shar
     return __all_sync(0xffffffffu, got);
   };
   auto publish = [&](int s, bool bad, int li) {
-    if (__any_sync(0xffffffffu, bad) && lane == 0) *bad_item = li + 1;
+    if (__any_sync(0xffffffffu, bad) && lane == 0) atomicMax(bad_item, li + 1);
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) mbar_arrive(bar(L::kReady + s));
@@ -502,7 +503,7 @@ __global__ void __launch_bounds__(Layout<kFormat>::kThreads, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kAbortOff);
   volatile unsigned long long* wait_limit =
       reinterpret_cast<volatile unsigned long long*>(smem + L::kLimitOff);
-  volatile int* bad_item = reinterpret_cast<volatile int*>(smem + L::kBadOff);
+  int* bad_item = reinterpret_cast<int*>(smem + L::kBadOff);
   auto bar = [&](int i) -> uint32_t { return sbase + L::kBarOff + 8u * i; };
 
   const int warp = threadIdx.x >> 5;
@@ -918,7 +919,8 @@ __global__ void __launch_bounds__(Layout<kFormat>::kThreads, 1)
         m_run = m;
         both = te - tb > 1;
       }
-      const bool aside = mine.hi >= 0 && *bad_item > li;  // (a row that exists keeps itself)
+      // (a row that exists keeps itself)
+      const bool aside = mine.hi >= 0 && *const_cast<volatile int*>(bad_item) > li;
       const float inv_l = 1.f / l_run;
       const int chunks = kDual ? 2 : 4, c0 = kDual ? 2 * x : 0;
       const uint32_t stage = sbase + L::kEpiOff + (warp - kSoftmaxWarp0) * 2048;
