@@ -91,6 +91,16 @@ def _raw_stream(device: int) -> int:
     return torch._C._cuda_getCurrentRawStream(device)
 
 
+def _as_stream(stream, device: int) -> torch.cuda.Stream:
+    """A stream given as torch's, by its handle, or as what has one (``cuda_stream``). What
+    a call makes for itself is made with that stream as the current one: memory of
+    another stream's pool may still be written by work that waits there."""
+    if isinstance(stream, torch.cuda.Stream):
+        _need(stream.device_index == device, "the stream must be of the tensors' device")
+        return stream
+    return torch.cuda.ExternalStream(_stream(stream), device=device)
+
+
 def _need(cond: bool, msg: str) -> None:
     if not cond:
         raise ValueError(msg)

@@ -20,7 +20,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .attention import HEAD_DIM, KV_HEADS, Context, EncodableRun, _launch, _need
+from .attention import HEAD_DIM, KV_HEADS, Context, EncodableRun, _as_stream, _launch, _need
 
 _DTYPES = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
 FORMATS = {"none": _lib.KV_PLAIN, "e4m3": _lib.KV_E4M3, "int8": _lib.KV_INT8}
@@ -179,8 +179,12 @@ def kv_cache_write(cache: KVCache, k: torch.Tensor, v: torch.Tensor, slots: torc
 def kv_cache_read(cache: KVCache, slots: torch.Tensor, k_out: Optional[torch.Tensor] = None,
                   v_out: Optional[torch.Tensor] = None, stream=None
                   ) -> Tuple[torch.Tensor, torch.Tensor]:
-    """(k, v) [tokens, heads, head_dim] of ``slots`` in the cache's dtype."""
+    """(k, v) [tokens, heads, head_dim] of ``slots`` in the cache's dtype. Outputs that
+    the call makes are of ``stream``."""
     ctx = Context.for_device(cache.index)
+    if stream is not None:
+        with torch.cuda.stream(_as_stream(stream, ctx.device)):
+            return kv_cache_read(cache, slots, k_out, v_out)
     k_out, v_out, args = _read_args(ctx, cache, slots, k_out, v_out)
     _launch(ctx, stream, ctx.lib.qwa_kv_cache_read, *args)
     return k_out, v_out

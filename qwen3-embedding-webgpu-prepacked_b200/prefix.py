@@ -23,7 +23,7 @@ import torch
 
 from . import _lib
 from .attention import (HEAD_DIM, MODE_AUTO, PREFIX, WINDOW, AttentionRun, Context, EncodableRun,
-                        _launch, _need, encode_run)
+                        _as_stream, _launch, _need, encode_run)
 from .kv_cache import _DTYPES, FORMATS, KVCache
 
 
@@ -226,14 +226,14 @@ def prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     [own keys, kv_heads, 128]. ``cu_seqlens`` (host) cuts q into requests, ``cu_seqlens_k``
     k and v (None: the same); a request's queries are the last of its keys.
     Lengths met before reuse their plan; inside a capture they must have been
-    met before it, and a captured ``stream`` must be the current one."""
+    met before it, and a captured ``stream`` must be the current one. An output that the
+    call makes is of ``stream``."""
     q_shape, k_shape = q.shape, k.shape
     _need(q.is_cuda and len(q_shape) == 3 and len(k_shape) == 3,
           "q and k must be CUDA tensors [tokens, heads, 128]")
     ctx = Context.for_device(q.get_device())
     if stream is not None:
-        if not isinstance(stream, torch.cuda.Stream):
-            stream = torch.cuda.ExternalStream(int(stream), device=q.device)
+        stream = _as_stream(stream, ctx.device)
         if not _capturing(ctx.device):
             # the graph would keep neither the plan nor a workspace
             with torch.cuda.stream(stream):
@@ -241,11 +241,16 @@ def prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                       "a captured stream must be the current one")
     plan = _plan_for(ctx, _lengths(cu_seqlens), _lengths(cu_seqlens_k), prefix_len,
                      q_shape[1], k_shape[1], mode, sparse_prefix, window)
+    if stream is not None:
+        with torch.cuda.stream(stream):
+            return _attention(ctx, plan, q, k, v, out, cache, first_slot)
+    return _attention(ctx, plan, q, k, v, out, cache, first_slot)
+
+
+def _attention(ctx: Context, plan: PrefixPlan, q, k, v, out, cache, first_slot) -> torch.Tensor:
+    """The call on the current stream, with an output and a workspace of that stream."""
     out, workspace, args = _attention_args(ctx, plan, q, k, v, out, cache, first_slot)
-    _launch(ctx, stream, ctx.lib.qwa_prefix_attention, plan.handle, *args)
-    if workspace is not None and stream is not None:
-        # its memory must not be handed out again before that stream is done with it
-        workspace.record_stream(stream)
+    _launch(ctx, None, ctx.lib.qwa_prefix_attention, plan.handle, *args)
     return out
 
 

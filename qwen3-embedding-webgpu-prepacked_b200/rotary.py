@@ -19,7 +19,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .attention import ROPE_THETA, Context, EncodableRun, _launch, _need
+from .attention import ROPE_THETA, Context, EncodableRun, _as_stream, _launch, _need
 
 _DTYPES = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
 _LAYOUTS = {"half": _lib.ROPE_HALF, "interleaved": _lib.ROPE_INTERLEAVED}
@@ -53,7 +53,8 @@ def rope_table(positions: int, rotary_dim: int = 128, theta: float = ROPE_THETA,
                scaling: Optional[RopeScaling] = None, first: int = 0, device=None,
                out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
     """f32 [positions, rotary_dim / 2, 2]: (cos, sin) of positions ``first``,
-    ``first`` + 1, ... with the angle in 64 bits."""
+    ``first`` + 1, ... with the angle in 64 bits. A table that the call makes is of
+    ``stream``."""
     _need(0 <= positions < 2 ** 31 and rotary_dim >= 2,
           "positions must be in 0..2^31-1 and rotary_dim >= 2")
     if out is not None:
@@ -63,6 +64,10 @@ def rope_table(positions: int, rotary_dim: int = 128, theta: float = ROPE_THETA,
         device = out.device
     device = torch.device("cuda") if device is None else torch.device(device)
     ctx = Context.for_device(device.index)
+    if stream is not None:
+        with torch.cuda.stream(_as_stream(stream, ctx.device)):
+            return rope_table(positions, rotary_dim, theta, scaling, first,
+                              torch.device("cuda", ctx.device), out)
     if out is None:
         out = torch.empty(positions, rotary_dim // 2, 2, dtype=torch.float32,
                           device=torch.device("cuda", ctx.device))
@@ -150,10 +155,14 @@ def rope(q: Optional[torch.Tensor], k: Optional[torch.Tensor], table: torch.Tens
          positions: torch.Tensor, layout: str = "half", inverse: bool = False,
          q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None, stream=None
          ) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
-    """(q, k) rotated at each token's position (the way back with ``inverse``)."""
+    """(q, k) rotated at each token's position (the way back with ``inverse``). Outputs
+    that the call makes are of ``stream``."""
     some = q if q is not None else k
     _need(some is not None and some.is_cuda, "q or k must be a CUDA tensor")
     ctx = Context.for_device(some.get_device())
+    if stream is not None:
+        with torch.cuda.stream(_as_stream(stream, ctx.device)):
+            return rope(q, k, table, positions, layout, inverse, q_out, k_out)
     q_out, k_out, args = _rope_args(ctx, q, k, table, positions, q_out, k_out, layout, inverse)
     _launch(ctx, stream, ctx.lib.qwa_rope, *args)
     return q_out, k_out

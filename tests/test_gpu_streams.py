@@ -1,0 +1,110 @@
+"""Calls on a stream that is not the current one. What a call makes for itself (outputs, a
+workspace) must not be memory that work waiting on the current stream still
+writes."""
+import os
+import sys
+
+import pytest
+import torch
+
+sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+from test_gpu_prefix import FULL, problem  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+SLEEP = 100_000_000  # cycles: about 50 ms
+
+
+def operators(pkg):
+    """name -> a call of stream=, returning the tensors that it makes"""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q, k, v, cache, _, _, cu, _ = problem(pkg, 1, [70, 30], [70, 30], 400, 16, 8, torch.float16,
+                                          "e4m3")
+    table = pkg.rotary.rope_table(200)
+    at = torch.randint(0, 200, (100,), generator=g, device="cuda", dtype=torch.int32)
+    return {
+        "rope": lambda stream: pkg.rotary.rope(q, k, table, at, stream=stream),
+        "rope_table": lambda stream: (pkg.rotary.rope_table(3000, stream=stream),),
+        "kv_cache_read": lambda stream: pkg.kv_cache.kv_cache_read(cache, at, stream=stream),
+        "prefix_attention": lambda stream: (pkg.prefix.prefix_attention(
+            q, k, v, cu, cache, 400, mode=FULL, stream=stream),),
+    }
+
+
+NAMES = ["rope", "rope_table", "kv_cache_read", "prefix_attention"]
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_outputs_are_not_memory_in_use_on_the_current_stream(pkg, cuda_dev, name):
+    call = operators(pkg)[name]
+    ref = call(None)
+    side = torch.cuda.Stream()
+    call(side)
+    torch.cuda.synchronize()
+    torch.cuda._sleep(SLEEP)
+    for r in ref:  # freed at once, written when the current stream gets there
+        for _ in range(4):
+            torch.empty_like(r).fill_(float("nan"))
+    got = call(side)
+    torch.cuda.synchronize()
+    for a, b in zip(got, ref):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_outputs_dropped_early_stay_of_their_stream(pkg, cuda_dev, name):
+    """The memory of an output that is dropped before its stream has written it must not
+    serve the current stream meanwhile."""
+    call = operators(pkg)[name]
+    ref = call(None)
+    side = torch.cuda.Stream()
+    call(side)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(SLEEP)
+    call(side)
+    mine = [torch.empty_like(r).fill_(3.0) for r in ref for _ in range(4)]
+    torch.cuda.synchronize()
+    assert all((t == 3).all() for t in mine)
+
+
+def test_two_calls_have_workspaces_of_their_own(pkg, cuda_dev):
+    """A long call on the current stream and one with another cache on a side stream, at
+    once: each converts its prefix into a workspace that the other does not get."""
+    work = []
+    for seed, queries, prefix in ((1, [500] * 16, 2000), (2, [500] * 8, 2000)):
+        q, k, v, cache, _, _, cu, _ = problem(pkg, seed, queries, queries, prefix, 16, 8,
+                                              torch.float16, "e4m3")
+        work.append((q, k, v, cu, cache, prefix))
+    refs = [pkg.prefix.prefix_attention(*w, mode=FULL) for w in work]
+    side = torch.cuda.Stream()
+    outs = [torch.empty_like(r) for r in refs]
+    for _ in range(20):
+        for out in outs:
+            out.zero_()
+        torch.cuda.synchronize()
+        pkg.prefix.prefix_attention(*work[0], mode=FULL, out=outs[0])
+        pkg.prefix.prefix_attention(*work[1], mode=FULL, out=outs[1], stream=side)
+        torch.cuda.synchronize()
+        for out, ref in zip(outs, refs):
+            assert torch.equal(out, ref)
+
+
+@pytest.mark.parametrize("name", ["rope", "kv_cache_read"])
+def test_a_capture_keeps_what_its_calls_made(pkg, cuda_dev, name):
+    """In a capture of a stream that is not the current one, outputs are of the graph's
+    pool: it writes them at every replay."""
+    call = operators(pkg)[name]
+    ref = call(None)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got = call(side)
+    pools = {s["address"]: tuple(s["segment_pool_id"]) for s in torch.cuda.memory_snapshot()}
+    for t in got:
+        address = max(a for a in pools if a <= t.data_ptr())
+        assert pools[address] == tuple(graph.pool())
+    graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(got, ref):
+        assert torch.equal(a, b)
