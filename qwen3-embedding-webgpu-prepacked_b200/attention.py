@@ -98,7 +98,10 @@ def _as_stream(stream, device: int) -> torch.cuda.Stream:
     if isinstance(stream, torch.cuda.Stream):
         _need(stream.device_index == device, "the stream must be of the tensors' device")
         return stream
-    return torch.cuda.ExternalStream(_stream(stream), device=device)
+    handle = _stream(stream)
+    # (torch takes a handle of 0 for none)
+    return torch.cuda.ExternalStream(handle, device=device) if handle else \
+        torch.cuda.default_stream(device)
 
 
 def _need(cond: bool, msg: str) -> None:

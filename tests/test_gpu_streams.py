@@ -68,6 +68,28 @@ def test_outputs_dropped_early_stay_of_their_stream(pkg, cuda_dev, name):
     assert all((t == 3).all() for t in mine)
 
 
+@pytest.mark.parametrize("name", NAMES)
+def test_streams_by_handle(pkg, cuda_dev, name):
+    """A stream's handle, that of the default stream (0) among them: the call runs behind
+    what waits there."""
+    call = operators(pkg)[name]
+    ref = call(None)
+    side = torch.cuda.Stream()
+    for stream in (side, side.cuda_stream, torch.cuda.default_stream().cuda_stream):
+        torch.cuda.synchronize()
+        on = side if stream else torch.cuda.default_stream()
+        with torch.cuda.stream(torch.cuda.Stream()):  # whatever the current one is
+            with torch.cuda.stream(on):
+                torch.cuda._sleep(SLEEP)
+            done = torch.cuda.Event()
+            got = call(stream)
+            done.record(on)
+            assert not done.query()
+            done.synchronize()
+            for a, b in zip(got, ref):
+                assert torch.equal(a, b)
+
+
 def test_two_calls_have_workspaces_of_their_own(pkg, cuda_dev):
     """A long call on the current stream and one with another cache on a side stream, at
     once: each converts its prefix into a workspace that the other does not get."""
