@@ -160,13 +160,22 @@ class PrefixAttentionKernel:
         """q [queries, q_heads, 128], k, v [own keys, kv_heads, 128] packed
         request after request, output as q, contiguous; the prefix is in the
         cache's slots ``first_slot`` .. ``first_slot + plan.prefix_len - 1``. A run
-        with ``owned_buffers`` is issued on one stream at a time."""
+        with ``owned_buffers`` is issued on one stream at a time (making it waits for
+        the current stream), and a captured graph needs it for as long as it is replayed."""
         _need(output is not None, "an output is required")
         _, workspace, args = _attention_args(self.ctx, plan, q, k, v, output, cache, first_slot)
-        lib, h = self.ctx.lib, self.ctx.handle
+        lib, h, device = self.ctx.lib, self.ctx.handle, self.ctx.device
+        if workspace is not None and not _capturing(device):
+            # whatever stream the run is issued on, no work must be left that writes it
+            torch.cuda.current_stream(device).synchronize()
+        used = set()
 
         def launch(stream):
             _need(plan.handle is not None, "the plan is closed")
+            if workspace is not None and stream not in used:
+                # not handed out again, once the run is gone, before that stream is done
+                workspace.record_stream(_as_stream(stream, device))
+                used.add(stream)
             return lib.qwa_prefix_attention(h, plan.handle, *args, stream)
 
         return AttentionRun([EncodableRun(launch, self.ctx, "shared-prefix attention")],

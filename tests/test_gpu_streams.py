@@ -76,11 +76,12 @@ def test_streams_by_handle(pkg, cuda_dev, name):
     ref = call(None)
     side = torch.cuda.Stream()
     for stream in (side, side.cuda_stream, torch.cuda.default_stream().cuda_stream):
+        call(stream)  # the stream's pool has memory then: allocating it may wait
         torch.cuda.synchronize()
         on = side if stream else torch.cuda.default_stream()
         with torch.cuda.stream(torch.cuda.Stream()):  # whatever the current one is
             with torch.cuda.stream(on):
-                torch.cuda._sleep(SLEEP)
+                torch.cuda._sleep(4 * SLEEP)
             done = torch.cuda.Event()
             got = call(stream)
             done.record(on)
@@ -110,6 +111,53 @@ def test_two_calls_have_workspaces_of_their_own(pkg, cuda_dev):
         torch.cuda.synchronize()
         for out, ref in zip(outs, refs):
             assert torch.equal(out, ref)
+
+
+def owned_run(pkg):
+    """(out, reference, make): make() is a run that owns a workspace"""
+    q, k, v, cache, _, _, cu, _ = problem(pkg, 5, [300] * 4, [300] * 4, 2000, 16, 8, torch.float16,
+                                          "e4m3")
+    ref = pkg.prefix.prefix_attention(q, k, v, cu, cache, 2000, mode=FULL)
+    plan = pkg.prefix.PrefixPlan(cu, 2000, 16, 8, mode=FULL)
+    kern, out = pkg.prefix.PrefixAttentionKernel(0), torch.empty_like(ref)
+
+    def make():
+        run = kern.create_run(q, k, v, out, plan, cache)
+        assert [b.numel() for b in run.owned_buffers] == [plan.workspace["e4m3"]]
+        return run
+    return kern, out, ref, make
+
+
+def test_workspace_of_a_run_is_not_in_use_elsewhere(pkg, cuda_dev):
+    kern, out, ref, make = owned_run(pkg)
+    side, nbytes = torch.cuda.Stream(), make().owned_buffers[0].numel()
+    for _ in range(10):
+        torch.cuda.synchronize()
+        torch.cuda._sleep(SLEEP // 100)
+        for _ in range(50):
+            torch.empty(nbytes, dtype=torch.uint8, device="cuda").fill_(0x7e)
+        run = make()
+        for _ in range(20):
+            kern.encode(side, run)
+        torch.cuda.synchronize()
+        assert torch.equal(out, ref)
+
+
+def test_workspace_of_a_dropped_run_stays_of_its_stream(pkg, cuda_dev):
+    kern, out, ref, make = owned_run(pkg)
+    side, run = torch.cuda.Stream(), make()
+    nbytes = run.owned_buffers[0].numel()
+    kern.encode(side, run)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(SLEEP)
+    out.zero_()
+    side.wait_stream(torch.cuda.current_stream())
+    kern.encode(side, run)
+    del run
+    mine = [torch.full((nbytes,), 3, dtype=torch.uint8, device="cuda") for _ in range(4)]
+    torch.cuda.synchronize()
+    assert all((t == 3).all() for t in mine) and torch.equal(out, ref)
 
 
 @pytest.mark.parametrize("name", ["rope", "kv_cache_read"])
