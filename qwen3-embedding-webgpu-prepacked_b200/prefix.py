@@ -216,12 +216,14 @@ def _plan_for(ctx: Context, *key) -> PrefixPlan:
     plan = PrefixPlan(cu_q, prefix_len, q_heads, kv_heads, cu_k, mode, sparse_prefix, window,
                       ctx=ctx)
     with _plans_lock:
-        _uses += 1
-        _plans[full] = [plan, _uses, False]
+        # another thread may have met the same lengths meanwhile, and captured a graph
+        # with its plan: the first one stays
+        entry = _plans.setdefault(full, [plan, 0, False])
+        _uses = entry[1] = _uses + 1
         loose = [(e[1], k) for k, e in _plans.items() if not e[2]]
         if len(loose) > MAX_PLANS:
             del _plans[min(loose)[1]]
-    return plan
+    return entry[0]
 
 
 def prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,

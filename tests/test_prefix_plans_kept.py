@@ -1,0 +1,69 @@
+"""How the shared-prefix binding keeps its plans, on the CPU: threads that meet the same
+lengths, and lists that are released. The plans are stand-ins for those of a GPU."""
+import threading
+
+import pytest
+
+
+released: list = []
+
+
+class Plan:
+    """A plan that notes when it is released; `made` is called as it is made."""
+    made = staticmethod(lambda: None)
+
+    def __init__(self, *args, **kw):
+        self.name = f"plan of {threading.current_thread().name}"
+        Plan.made()
+
+    def __del__(self):
+        released.append(self.name)
+
+
+class Ctx:
+    device = 0
+
+
+@pytest.fixture
+def prefix(pkg, monkeypatch):
+    p = pkg.prefix
+    monkeypatch.setattr(p, "_plans", {})
+    monkeypatch.setattr(p, "PrefixPlan", Plan)
+    monkeypatch.setattr(p, "_capturing", lambda device: p.captures)
+    monkeypatch.setattr(p, "captures", False, raising=False)
+    monkeypatch.setattr(Plan, "made", staticmethod(lambda: None))
+    released.clear()
+    return p
+
+
+def key(n):
+    return ((0, n), None, 10, 16, 8, 0, 176, 432)
+
+
+def test_two_threads_that_meet_the_same_lengths_share_a_plan(prefix):
+    """The plan of the first thread, which a graph may hold by then, is not replaced by that of
+    the second."""
+    got, late_made, go = {}, threading.Event(), threading.Event()
+
+    def late():
+        late_made.set()
+        go.wait(10)
+
+    Plan.made = staticmethod(late)
+    thread = threading.Thread(target=lambda: got.update(b=prefix._plan_for(Ctx, *key(5)).name),
+                              name="late")
+    thread.start()
+    late_made.wait(10)  # it has seen no plan, and makes one
+    Plan.made = staticmethod(lambda: None)
+    first = prefix._plan_for(Ctx, *key(5)).name
+    prefix.captures = True
+    assert prefix._plan_for(Ctx, *key(5)).name == first  # a graph holds it from here on
+    prefix.captures = False
+    go.set()
+    thread.join(10)
+    for n in range(prefix.MAX_PLANS + 5):  # others push out what no graph holds
+        prefix._plan_for(Ctx, *key(100 + n))
+    assert first != "plan of late" and got["b"] == first
+    assert released.count("plan of late") == 1
+    assert prefix._plan_for(Ctx, *key(5)).name == first
+    assert released.count(first) == 5  # of the others
