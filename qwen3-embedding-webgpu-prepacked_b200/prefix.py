@@ -71,8 +71,11 @@ class PrefixPlan:
                sparse_prefix=sparse_prefix, window=window)
         _need(not _capturing(self.ctx.device),
               "a plan allocates memory: make it before the capture")
-        while _retired:
-            lib, old = _retired.pop()
+        while True:
+            try:  # (threads that make plans at once share the list)
+                lib, old = _retired.pop()
+            except IndexError:
+                break
             lib.qwa_prefix_plan_destroy(old)
         h = ctypes.c_void_p()
         with _create_lock:

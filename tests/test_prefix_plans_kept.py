@@ -1,6 +1,7 @@
 """How the shared-prefix binding keeps its plans, on the CPU: threads that meet the same
 lengths, and lists that are released. The plans are stand-ins for those of a GPU."""
 import threading
+from types import SimpleNamespace
 
 import pytest
 
@@ -67,3 +68,27 @@ def test_two_threads_that_meet_the_same_lengths_share_a_plan(prefix):
     assert released.count("plan of late") == 1
     assert prefix._plan_for(Ctx, *key(5)).name == first
     assert released.count(first) == 5  # of the others
+
+
+def test_another_thread_releases_the_last_retired_plan(pkg, monkeypatch):
+    """Lists retired during a capture are released by the next plan, whichever thread makes
+    it."""
+    prefix, done = pkg.prefix, []
+
+    class Taken(list):
+        """Another thread takes the last one between a look at the list and what follows."""
+
+        def __bool__(self):
+            some = len(self) > 0
+            if len(self) == 1:
+                self.clear()
+            return some
+
+    lib = SimpleNamespace(qwa_prefix_plan_create=lambda *a: 0, qwa_prefix_plan_deal=lambda *a: 0,
+                          qwa_prefix_attention_workspace=lambda *a: 0,
+                          qwa_prefix_plan_destroy=done.append)
+    ctx = SimpleNamespace(lib=lib, handle=None, device=0)
+    monkeypatch.setattr(prefix, "_capturing", lambda device: False)
+    monkeypatch.setattr(prefix, "_retired", Taken([(lib, 1), (lib, 2)]))
+    prefix.PrefixPlan([0, 5], 10, 16, 8, ctx=ctx)
+    assert set(done) >= {2} and len(prefix._retired) == 0
