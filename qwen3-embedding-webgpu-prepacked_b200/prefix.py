@@ -218,6 +218,7 @@ def _plan_for(ctx: Context, *key) -> PrefixPlan:
     cu_q, cu_k, prefix_len, q_heads, kv_heads, mode, sparse_prefix, window = key
     plan = PrefixPlan(cu_q, prefix_len, q_heads, kv_heads, cu_k, mode, sparse_prefix, window,
                       ctx=ctx)
+    old = None
     with _plans_lock:
         # another thread may have met the same lengths meanwhile, and captured a graph
         # with its plan: the first one stays
@@ -225,7 +226,8 @@ def _plan_for(ctx: Context, *key) -> PrefixPlan:
         _uses = entry[1] = _uses + 1
         loose = [(e[1], k) for k, e in _plans.items() if not e[2]]
         if len(loose) > MAX_PLANS:
-            del _plans[min(loose)[1]]
+            old = _plans.pop(min(loose)[1])
+    del old  # outside the lock: releasing its lists waits for the device
     return entry[0]
 
 

@@ -70,6 +70,21 @@ def test_two_threads_that_meet_the_same_lengths_share_a_plan(prefix):
     assert released.count(first) == 5  # of the others
 
 
+def test_plans_are_released_outside_the_lock(prefix, monkeypatch):
+    """Releasing a plan waits for the device; calls of other threads must not wait for
+    that."""
+    held = []
+
+    class Watched(Plan):
+        def __del__(self):
+            held.append(prefix._plans_lock.locked())
+
+    monkeypatch.setattr(prefix, "PrefixPlan", Watched)
+    for n in range(prefix.MAX_PLANS + 3):
+        prefix._plan_for(Ctx, *key(n))
+    assert held == [False] * 3
+
+
 def test_another_thread_releases_the_last_retired_plan(pkg, monkeypatch):
     """Lists retired during a capture are released by the next plan, whichever thread makes
     it."""
