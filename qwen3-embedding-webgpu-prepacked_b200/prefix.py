@@ -128,6 +128,7 @@ def _attention_args(ctx: Context, plan: PrefixPlan, q, k, v, output, cache, firs
     _need(code is not None, "q must be float16 or bfloat16")
     _need(plan.ctx.device == index, "the plan must be on the kernel's device")
     _need(plan.handle is not None, "the plan is closed")
+    _need(-2 ** 63 <= first_slot < 2 ** 63, "first_slot must be a 64-bit number")
     n, hq, m, hk = plan.queries, plan.q_heads, plan.keys, plan.kv_heads
     if output is None:
         output = torch.empty_like(q, memory_format=torch.contiguous_format)

@@ -57,6 +57,8 @@ def rope_table(positions: int, rotary_dim: int = 128, theta: float = ROPE_THETA,
     ``stream``."""
     _need(0 <= positions < 2 ** 31 and rotary_dim >= 2,
           "positions must be in 0..2^31-1 and rotary_dim >= 2")
+    _need(rotary_dim < 2 ** 31 and -2 ** 63 <= first < 2 ** 63,
+          "rotary_dim must be a 32-bit number, first a 64-bit one")
     if out is not None:
         _need(out.is_cuda and out.dtype == torch.float32 and out.is_contiguous()
               and out.numel() >= positions * (rotary_dim // 2) * 2,
