@@ -343,7 +343,7 @@ typedef struct qwa_rope_scaling {
   double beta_fast, beta_slow;              /* YARN; usually 32 and 1 */
   double attention_factor;                  /* YARN; <= 0: the rule above */
   double low_freq_factor, high_freq_factor; /* LLAMA3; usually 1 and 4 */
-} qwa_rope_scaling;
+} qwa_rope_scaling; /* what a kind uses must be finite, and the angles that it gives */
 
 /* Rotary table: table[p][i] = (m cos a, m sin a), a = (first_position + p) *
  * f_i in 64 bits, f32 [positions, rotary_dim/2, 2]; scaling NULL: none. With

@@ -1060,11 +1060,16 @@ qwa_status rope_frequencies(qwa_ctx* ctx, int rotary, double theta, const qwa_ro
     };
     low = std::max(std::floor(at(s->beta_fast)), 0.0);
     high = std::min(std::ceil(at(s->beta_slow)), rotary - 1.0);
+    if (!std::isfinite(s->attention_factor))
+      return fail(ctx, QWA_ERR_INVALID_ARG, "attention_factor must be a finite number");
     if (s->attention_factor > 0.0) out->m = s->attention_factor;
     else if (factor > 1.0) out->m = 0.1 * std::log(factor) + 1.0;
   }
-  if (kind == QWA_ROPE_SCALING_LLAMA3 && !(s->high_freq_factor > s->low_freq_factor))
-    return fail(ctx, QWA_ERR_INVALID_ARG, "high_freq_factor > low_freq_factor is required");
+  if (kind == QWA_ROPE_SCALING_LLAMA3 &&
+      (!(s->high_freq_factor > s->low_freq_factor) || !std::isfinite(s->high_freq_factor) ||
+       !std::isfinite(s->low_freq_factor)))
+    return fail(ctx, QWA_ERR_INVALID_ARG,
+                "high_freq_factor > low_freq_factor is required, both finite");
   for (int i = 0; i < half; ++i) {
     double f = std::pow(base, -double(i) / half);
     if (kind == QWA_ROPE_SCALING_LINEAR) {
@@ -1080,6 +1085,9 @@ qwa_status rope_frequencies(qwa_ctx* ctx, int rotary, double theta, const qwa_ro
           1.0);
       f = (1.0 - smooth) * f / factor + smooth * f;
     }
+    // a factor at the end of its range: the angle of the last position must be finite
+    if (!std::isfinite(f * 4294967296.0) || !std::isfinite(out->m))
+      return fail(ctx, QWA_ERR_INVALID_ARG, "the scaling gives angles that are not finite");
     out->f[i] = f;
   }
   return QWA_OK;

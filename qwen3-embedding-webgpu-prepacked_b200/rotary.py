@@ -13,6 +13,7 @@ Launches are the kernels of csrc/rope.cu through the C ABI.
 from __future__ import annotations
 
 import ctypes
+import math
 from dataclasses import dataclass
 from typing import Optional, Tuple
 
@@ -41,8 +42,9 @@ class RopeScaling:
     def struct(self) -> "_lib.RopeScalingStruct":
         _need(self.kind in _lib.ROPE_SCALING,
               f"scaling kind must be one of {sorted(_lib.ROPE_SCALING)}")
-        _need(self.attention_factor is None or self.attention_factor > 0,
-              "attention_factor must be above 0")
+        _need(self.attention_factor is None
+              or (self.attention_factor > 0 and math.isfinite(self.attention_factor)),
+              "attention_factor must be a finite number above 0")
         return _lib.RopeScalingStruct(_lib.ROPE_SCALING[self.kind], self.factor,
                                       self.original_positions, self.beta_fast, self.beta_slow,
                                       self.attention_factor or 0.0, self.low_freq_factor,

@@ -24,3 +24,10 @@ def test_slots_past_64_bits(pkg, first_slot):
     assert 7 in args
     with pytest.raises(ValueError, match="bit"):
         pkg.prefix._attention_args(device, plan, q, k, k, None, None, first_slot)
+
+
+@pytest.mark.parametrize("factor", [float("inf"), float("nan"), 0.0, -1.0])
+def test_attention_factors_of_no_use(pkg, factor):
+    with pytest.raises(ValueError):
+        pkg.rotary.RopeScaling("yarn", 4.0, 4096, attention_factor=factor).struct()
+    assert pkg.rotary.RopeScaling("yarn", 4.0, 4096, attention_factor=0.5).struct()
