@@ -31,3 +31,14 @@ def test_attention_factors_of_no_use(pkg, factor):
     with pytest.raises(ValueError):
         pkg.rotary.RopeScaling("yarn", 4.0, 4096, attention_factor=factor).struct()
     assert pkg.rotary.RopeScaling("yarn", 4.0, 4096, attention_factor=0.5).struct()
+
+
+def test_rope_rows_of_the_projection_are_on_its_device(pkg):
+    def table(device=1, dtype=torch.float32, values=640, contiguous=True):
+        return SimpleNamespace(get_device=lambda: device, dtype=dtype, is_cuda=device >= 0,
+                               is_contiguous=lambda: contiguous, numel=lambda: values)
+    pkg.matmul._rope_rows(table(), 5, 1)
+    for bad in (table(device=0), table(device=-1), table(dtype=torch.float64),
+                table(values=639), table(contiguous=False)):
+        with pytest.raises(ValueError, match="rope_table"):
+            pkg.matmul._rope_rows(bad, 5, 1)
