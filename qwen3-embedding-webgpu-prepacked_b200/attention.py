@@ -120,6 +120,15 @@ def _f32_weight(t: torch.Tensor, name: str) -> None:
           f"{name} must be a contiguous CUDA float32 tensor of 128 elements")
 
 
+def _rope_rows(table: torch.Tensor, cu, device: int) -> None:
+    """Checks the rope_table of requests that ``cu`` cuts."""
+    longest = max((cu[b + 1] - cu[b] for b in range(len(cu) - 1)), default=0)
+    _need(table.get_device() == device and table.dtype == torch.float32
+          and table.is_contiguous() and table.numel() >= longest * 128,
+          "rope_table must be a contiguous float32 [positions, 64, 2] of the longest request's "
+          "positions at least, on input's device")
+
+
 def _launch(ctx: "Context", stream, fn, *args) -> None:
     """Issue a C ABI call on ``stream`` (None: the current stream of the context's
     device), without a bound run in between."""
@@ -196,6 +205,8 @@ class QKNormRopeKernel:
         _need(input.numel() >= total * input_stride, "input smaller than tokens * input_stride")
         _need(q_output.numel() >= total * Q_HEADS * HEAD_DIM, "q_output too small")
         _need(k_output.numel() >= total * KV_HEADS * HEAD_DIM, "k_output too small")
+        if rope_table is not None:
+            _rope_rows(rope_table, cu, self.ctx.device)
         lib, h = self.ctx.lib, self.ctx.handle
         args = (_ptr(input), input_stride, _ptr(q_weight), _ptr(k_weight), _ptr(q_output),
                 _ptr(k_output), cu, len(cu) - 1, epsilon, theta, _ptr(rope_table))

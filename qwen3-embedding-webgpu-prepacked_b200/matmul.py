@@ -19,7 +19,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .attention import Context, _need, _ptr, _stream
+from .attention import Context, _need, _ptr, _rope_rows, _stream
 
 LAYOUT_TILE32 = "q4_0-tile32-compact"
 
@@ -166,13 +166,6 @@ def matmul_swiglu(input: torch.Tensor, weight_interleaved: torch.Tensor,
     return out
 
 
-def _rope_rows(table: torch.Tensor, longest: int, device: int) -> None:
-    _need(table.get_device() == device and table.dtype == torch.float32
-          and table.is_contiguous() and table.numel() >= longest * 128,
-          "rope_table must be a contiguous float32 [positions, 64, 2] of the longest request's "
-          "positions at least, on input's device")
-
-
 def qkv_projection(input: torch.Tensor, weight: torch.Tensor, q_weight: torch.Tensor,
                    k_weight: torch.Tensor, cu_seqlens, eps: float = 1e-6, theta: float = 1e6,
                    q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None,
@@ -197,8 +190,7 @@ def qkv_projection(input: torch.Tensor, weight: torch.Tensor, q_weight: torch.Te
     ctx = Context.for_device(dev.index)
     cu = _lib.cu_array(cu_seqlens)
     if rope_table is not None:
-        _rope_rows(rope_table, max((cu[b + 1] - cu[b] for b in range(len(cu) - 1)), default=0),
-                   ctx.device)
+        _rope_rows(rope_table, cu, ctx.device)
     if weight.dtype == torch.uint8:
         _need(weight.is_cuda and weight.numel() >= packed_bytes(4096, k),
               "packed weight must be a CUDA tile32-compact buffer of [4096, k]")

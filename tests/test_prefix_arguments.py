@@ -33,12 +33,29 @@ def test_attention_factors_of_no_use(pkg, factor):
     assert pkg.rotary.RopeScaling("yarn", 4.0, 4096, attention_factor=0.5).struct()
 
 
-def test_rope_rows_of_the_projection_are_on_its_device(pkg):
+def test_rope_rows_are_on_the_device_and_enough(pkg):
+    """Of the projection and of the Q/K norm, whose requests of `cu` begin behind a prefix."""
     def table(device=1, dtype=torch.float32, values=640, contiguous=True):
         return SimpleNamespace(get_device=lambda: device, dtype=dtype, is_cuda=device >= 0,
                                is_contiguous=lambda: contiguous, numel=lambda: values)
-    pkg.matmul._rope_rows(table(), 5, 1)
+    cu = [0, 2, 7, 8]  # at most five positions
+    pkg.attention._rope_rows(table(), cu, 1)
     for bad in (table(device=0), table(device=-1), table(dtype=torch.float64),
                 table(values=639), table(contiguous=False)):
         with pytest.raises(ValueError, match="rope_table"):
-            pkg.matmul._rope_rows(bad, 5, 1)
+            pkg.attention._rope_rows(bad, cu, 1)
+
+
+def test_qk_norm_takes_no_short_rope_table(pkg, monkeypatch):
+    """It read past the table's end."""
+    attn = pkg.attention
+    for name in ("_f16_cuda", "_f32_weight"):
+        monkeypatch.setattr(attn, name, lambda *a: None)
+    kern = attn.QKNormRopeKernel.__new__(attn.QKNormRopeKernel)
+    kern.ctx = SimpleNamespace(device=-1, lib=None, handle=None)  # of CPU tensors
+    x = torch.zeros(9, 4096)
+    args = (x, x, x, x, x, [0, 4, 9])
+    kern.create_run_varlen(*args, input_stride=4096, rope_table=torch.zeros(5, 64, 2))
+    for bad in (torch.zeros(4, 64, 2), torch.zeros(5, 64, 2, dtype=torch.float64)):
+        with pytest.raises(ValueError, match="rope_table"):
+            kern.create_run_varlen(*args, input_stride=4096, rope_table=bad)
