@@ -272,6 +272,9 @@ def qk_norm_rope(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tens
                  q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None,
                  stream=None):
     """Normed + roped q [T,16,128] and k [T,8,128] (f16) from qkv [T, stride]."""
+    if stream is not None and (q_out is None or k_out is None):
+        with torch.cuda.stream(_as_stream(stream, qkv.get_device())):
+            return qk_norm_rope(qkv, q_weight, k_weight, cu_seqlens, eps, theta, q_out, k_out)
     T = int(cu_seqlens[-1])
     q_out = q_out if q_out is not None else torch.empty(T, Q_HEADS, HEAD_DIM, dtype=torch.float16,
                                                         device=qkv.device)
@@ -287,6 +290,9 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: Seq
               value_stride: int = 1024, value_offset: int = 0, mode: int = MODE_AUTO,
               prefix: int = PREFIX, window: int = WINDOW, out: Optional[torch.Tensor] = None,
               stream=None) -> torch.Tensor:
+    if stream is not None and out is None:
+        with torch.cuda.stream(_as_stream(stream, q.get_device())):
+            return attention(q, k, v, cu_seqlens, value_stride, value_offset, mode, prefix, window)
     T = int(cu_seqlens[-1])
     out = out if out is not None else torch.empty(T, Q_HEADS, HEAD_DIM, dtype=torch.float16,
                                                   device=q.device)
@@ -303,6 +309,10 @@ def prefill_attention_layer(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight:
                             stream=None, ctx: Optional[Context] = None) -> torch.Tensor:
     """Prologue + attention of one layer (model.ts:94-95): qkv [T, 4096] f16.
     ``ctx``: the context to launch on (default: the device's shared one)."""
+    if stream is not None and (q_buf is None or k_buf is None or out is None):
+        with torch.cuda.stream(_as_stream(stream, qkv.get_device())):
+            return prefill_attention_layer(qkv, q_weight, k_weight, cu_seqlens, mode, prefix,
+                                           window, eps, theta, q_buf, k_buf, out, ctx=ctx)
     _f16_cuda(qkv, "qkv")
     _f32_weight(q_weight, "q_weight")
     _f32_weight(k_weight, "k_weight")

@@ -11,7 +11,7 @@ from typing import Optional
 
 import torch
 
-from .attention import Context, EncodableRun, _need, _ptr, encode_run
+from .attention import Context, EncodableRun, _as_stream, _need, _ptr, encode_run
 
 
 def _f16(t: torch.Tensor, name: str, n: int) -> None:
@@ -68,6 +68,9 @@ class EmbeddingLookupKernel:
 
 def swiglu(combined: torch.Tensor, width: int, out: Optional[torch.Tensor] = None,
            stream=None) -> torch.Tensor:
+    if stream is not None and out is None:
+        with torch.cuda.stream(_as_stream(stream, combined.get_device())):
+            return swiglu(combined, width)
     rows = combined.shape[0]
     out = out if out is not None else torch.empty(rows, width, dtype=torch.float16,
                                                   device=combined.device)
@@ -78,6 +81,9 @@ def swiglu(combined: torch.Tensor, width: int, out: Optional[torch.Tensor] = Non
 def embedding_lookup(ids: torch.Tensor, table: torch.Tensor, width: int = 1024,
                      vocab: Optional[int] = None, out: Optional[torch.Tensor] = None,
                      stream=None) -> torch.Tensor:
+    if stream is not None and out is None:
+        with torch.cuda.stream(_as_stream(stream, ids.get_device())):
+            return embedding_lookup(ids, table, width, vocab)
     n = ids.numel()
     out = out if out is not None else torch.empty(n, width, dtype=torch.float16, device=ids.device)
     encode_run(stream, EmbeddingLookupKernel(ids.device.index).create_run(ids, table, out, n,

@@ -19,7 +19,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .attention import Context, _need, _ptr, _rope_rows, _stream
+from .attention import Context, _as_stream, _need, _ptr, _rope_rows, _stream
 
 LAYOUT_TILE32 = "q4_0-tile32-compact"
 
@@ -104,6 +104,9 @@ class QuantMatmulKernel:
 def q40_dequantize(packed: torch.Tensor, n: int, k: int, out: Optional[torch.Tensor] = None,
                    stream=None) -> torch.Tensor:
     """f16 W [n, k] from a tile32-compact buffer."""
+    if stream is not None and out is None:
+        with torch.cuda.stream(_as_stream(stream, packed.get_device())):
+            return q40_dequantize(packed, n, k)
     _need(packed.is_cuda and packed.dtype == torch.uint8 and packed.numel() >= packed_bytes(n, k),
           "packed must be a CUDA uint8 tile32-compact buffer")
     out = out if out is not None else torch.empty(n, k, dtype=torch.float16, device=packed.device)
@@ -119,6 +122,9 @@ def q40_matmul(input: torch.Tensor, packed: torch.Tensor, n: int, k: int,
     """f16 [m, n] = input [m, k] @ W^T with W the Q4_0 tile32 matrix ``packed``
     (quant-matmul.ts:495-540): m <= 64 rows on n <= 2048 read the records
     directly; other shapes use the context's cached f16 copy."""
+    if stream is not None and out is None:
+        with torch.cuda.stream(_as_stream(stream, input.get_device())):
+            return q40_matmul(input, packed, n, k)
     kern = QuantMatmulKernel(input.device.index)
     run = kern.create_run_from_buffers(input, packed, input.shape[0], n, k, out)
     kern.encode(stream, run)
@@ -128,6 +134,9 @@ def q40_matmul(input: torch.Tensor, packed: torch.Tensor, n: int, k: int,
 def matmul(input: torch.Tensor, weight: torch.Tensor, out: Optional[torch.Tensor] = None,
            stream=None) -> torch.Tensor:
     """f16 [m, n] = input [m, k] @ weight [n, k]^T on the tensor cores."""
+    if stream is not None and out is None:
+        with torch.cuda.stream(_as_stream(stream, input.get_device())):
+            return matmul(input, weight)
     m, k = input.shape
     n = weight.shape[0]
     _f16(input, "input", m * k)
@@ -153,6 +162,9 @@ def matmul_swiglu(input: torch.Tensor, weight_interleaved: torch.Tensor,
     """f16 [m, n/2] = SwiGLU of input [m, k] @ gate_up^T, the SwiGLU applied in
     the GEMM's epilogue (bit for bit ``swiglu(matmul(...))``); the weight is
     ``interleave_gate_up(gate_up)``."""
+    if stream is not None and out is None:
+        with torch.cuda.stream(_as_stream(stream, input.get_device())):
+            return matmul_swiglu(input, weight_interleaved)
     m, k = input.shape
     n = weight_interleaved.shape[0]
     _f16(input, "input", m * k)
@@ -174,6 +186,10 @@ def qkv_projection(input: torch.Tensor, weight: torch.Tensor, q_weight: torch.Te
     """attn_qkv projection fused with the per-head Q/K RMSNorm + RoPE
     (src/webgpu/model.ts:93-94). ``weight`` is f16 [4096, k] or a uint8 Q4_0
     tile32-compact buffer; returns (q [T,16,128], k [T,8,128], v [T,1024])."""
+    if stream is not None and (q_out is None or k_out is None or v_out is None):
+        with torch.cuda.stream(_as_stream(stream, input.get_device())):
+            return qkv_projection(input, weight, q_weight, k_weight, cu_seqlens, eps, theta, q_out,
+                                  k_out, v_out, rope_table)
     T, k = input.shape
     _need(T == int(cu_seqlens[-1]), "input rows must equal cu_seqlens[-1]")
     _f16(input, "input", T * k)

@@ -12,7 +12,7 @@ from typing import Optional
 
 import torch
 
-from .attention import EPSILON, Context, EncodableRun, _need, _ptr, encode_run
+from .attention import EPSILON, Context, EncodableRun, _as_stream, _need, _ptr, encode_run
 
 
 def _f16(t: torch.Tensor, name: str, n: int) -> None:
@@ -48,6 +48,9 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
              eps: float = EPSILON, out: Optional[torch.Tensor] = None,
              stream=None) -> torch.Tensor:
     """normalized f16 [rows, width]; with ``residual``, x += residual in place."""
+    if stream is not None and out is None:
+        with torch.cuda.stream(_as_stream(stream, x.get_device())):
+            return rms_norm(x, weight, residual, eps)
     rows, width = x.shape
     out = out if out is not None else torch.empty_like(x)
     kern = RmsNormKernel(x.device.index)

@@ -15,7 +15,7 @@ from typing import Optional, Sequence
 import torch
 
 from . import _lib
-from .attention import Context, EncodableRun, _need, _ptr, encode_run
+from .attention import Context, EncodableRun, _as_stream, _need, _ptr, encode_run
 
 WIDTH = 1024  # hidden size of Qwen3-Embedding-0.6B, ops.ts:361 default
 
@@ -69,6 +69,9 @@ class LastTokenPoolKernel:
 def last_token_pool(hidden: torch.Tensor, cu_seqlens: Sequence[int],
                     out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
     """f32 [B, width] L2-normalised last-token rows of packed hidden [T, width]."""
+    if stream is not None and out is None:
+        with torch.cuda.stream(_as_stream(stream, hidden.get_device())):
+            return last_token_pool(hidden, cu_seqlens)
     width = hidden.shape[-1]
     batch = len(cu_seqlens) - 1
     out = out if out is not None else torch.empty(batch, width, dtype=torch.float32,

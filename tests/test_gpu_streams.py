@@ -4,8 +4,11 @@ writes."""
 import os
 import sys
 
+import numpy as np
 import pytest
 import torch
+
+from oracle import q40 as oracle_q40
 
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
 from test_gpu_prefix import FULL, problem  # noqa: E402
@@ -34,10 +37,50 @@ def operators(pkg):
 NAMES = ["rope", "rope_table", "kv_cache_read", "prefix_attention"]
 
 
-@pytest.mark.parametrize("name", NAMES)
+def layer_operators(pkg):
+    """The same of the framework's other calls with stream="""
+    g = torch.Generator(device="cuda").manual_seed(2)
+    x = torch.randn(300, 4096, generator=g, device="cuda").half()
+    w = (torch.randn(4096, 1024, generator=g, device="cuda") / 32).half()
+    hidden, ones, cu = x[:, :1024].contiguous(), torch.ones(128, device="cuda"), [0, 100, 300]
+    q, k = pkg.attention.qk_norm_rope(x, ones, ones, cu)
+    rng = np.random.default_rng(3)
+    q40, _, _ = oracle_q40.pack_q40_tile32([(oracle_q40.random_q40_rows(rng, 1024, 1024), 1024)])
+    packed = torch.from_numpy(q40).cuda()
+    table = torch.from_numpy(np.frombuffer(pkg.prepacked.random_q6k_rows(rng, 64, 1024),
+                                           np.uint8).copy()).cuda()
+    ids = torch.randint(0, 64, (300,), generator=g, device="cuda", dtype=torch.int32)
+    mm, att = pkg.matmul, pkg.attention
+
+    def one(fn, *args):
+        return lambda stream: (fn(*args, stream=stream),)
+    return {
+        "qk_norm_rope": lambda stream: att.qk_norm_rope(x, ones, ones, cu, stream=stream),
+        "attention": one(att.attention, q, k, hidden, cu),
+        "prefill_attention_layer": one(att.prefill_attention_layer, x, ones, ones, cu),
+        "rms_norm": one(pkg.norm.rms_norm, hidden, torch.ones(1024, device="cuda")),
+        "swiglu": one(pkg.ffn.swiglu, x, 2048),
+        "embedding_lookup": one(pkg.ffn.embedding_lookup, ids, table),
+        "last_token_pool": one(pkg.pooling.last_token_pool, hidden, cu),
+        "q40_dequantize": one(mm.q40_dequantize, packed, 1024, 1024),
+        "q40_matmul": one(mm.q40_matmul, hidden, packed, 1024, 1024),
+        "matmul": one(mm.matmul, hidden, w),
+        "matmul_swiglu": one(mm.matmul_swiglu, hidden, mm.interleave_gate_up(w)),
+        "qkv_projection": lambda stream: mm.qkv_projection(hidden, w, ones, ones, cu,
+                                                           stream=stream),
+    }
+
+
+LAYER_NAMES = ["qk_norm_rope", "attention", "prefill_attention_layer", "rms_norm", "swiglu",
+               "embedding_lookup", "last_token_pool", "q40_dequantize", "q40_matmul", "matmul",
+               "matmul_swiglu", "qkv_projection"]
+
+
+@pytest.mark.parametrize("name", NAMES + LAYER_NAMES)
 def test_outputs_are_not_memory_in_use_on_the_current_stream(pkg, cuda_dev, name):
-    call = operators(pkg)[name]
+    call = (operators if name in NAMES else layer_operators)(pkg)[name]
     ref = call(None)
+    torch.cuda.synchronize()
     side = torch.cuda.Stream()
     call(side)
     torch.cuda.synchronize()
@@ -51,12 +94,13 @@ def test_outputs_are_not_memory_in_use_on_the_current_stream(pkg, cuda_dev, name
         assert torch.equal(a, b)
 
 
-@pytest.mark.parametrize("name", NAMES)
+@pytest.mark.parametrize("name", NAMES + LAYER_NAMES)
 def test_outputs_dropped_early_stay_of_their_stream(pkg, cuda_dev, name):
     """The memory of an output that is dropped before its stream has written it must not
     serve the current stream meanwhile."""
-    call = operators(pkg)[name]
+    call = (operators if name in NAMES else layer_operators)(pkg)[name]
     ref = call(None)
+    torch.cuda.synchronize()
     side = torch.cuda.Stream()
     call(side)
     torch.cuda.synchronize()
