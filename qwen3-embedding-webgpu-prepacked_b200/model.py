@@ -28,15 +28,15 @@ here, so embeddings are not the trained model's.
 """
 from __future__ import annotations
 
-from typing import List, Optional, Sequence
-
+import warnings
 from dataclasses import dataclass
+from typing import List, Optional, Sequence
 
 import numpy as np
 import torch
 
 from . import attention as attn
-from . import ffn, matmul, norm, prepacked, rotary
+from . import ffn, matmul, norm, prepacked, rotary, sharding
 from .kv_cache import KVCache, kv_cache_write
 from .pooling import last_token_pool
 from .prefix import _capturing, prefix_attention
@@ -87,10 +87,25 @@ def synthetic_model_file(layers: int = LAYERS, vocab: int = 4096, seed: int = 0)
 @dataclass
 class CachedPrefix:
     """The keys and values of a text that requests begin with, by layer, and
-    the attention mode that it was computed in."""
+    the attention mode that it was computed in (``auto``: as AUTO resolved it)."""
     length: int
     mode: int
     caches: List[KVCache]
+    auto: bool = False
+
+    def mode_for(self, longest: int) -> int:
+        """The mode of requests of up to ``longest`` tokens behind the text; warns where
+        AUTO on the whole requests would be another, and with it their embeddings."""
+        if self.auto and longest > 0:
+            whole = attn.MODE_SPARSE if sharding.resolve_sparse(
+                attn.MODE_AUTO, [self.length + longest]) else attn.MODE_FULL
+            if whole != self.mode:
+                warnings.warn(
+                    f"requests of {longest} tokens behind a prefix of {self.length} keep its "
+                    "sparse attention, as AUTO resolved it on the prefix; computed whole they "
+                    "would have full attention. Cache the prefix with mode=MODE_FULL for that.",
+                    stacklevel=3)
+        return self.mode
 
     def nbytes(self) -> int:
         return sum(c.nbytes() for c in self.caches)
@@ -162,16 +177,18 @@ class Qwen3EmbeddingModel:
         """Compute the text that requests will begin with (``ids``, CUDA int32)
         once and keep its keys and values of every layer in ``format`` ("none":
         float16, "e4m3" or "int8"). AUTO resolves the attention mode on the
-        prefix alone, and requests behind it keep that mode."""
+        prefix alone, and requests behind it keep that mode: it is sparse for prefixes up to 8192
+        tokens, and requests that are longer with the prefix differ from whole ones
+        (``forward`` warns)."""
         length = int(ids.numel())
         if length < 1:
             raise ValueError("a prefix has at least one token")
-        if mode == attn.MODE_AUTO:
-            from . import sharding
+        auto = mode == attn.MODE_AUTO
+        if auto:
             mode = attn.MODE_SPARSE if sharding.resolve_sparse(mode, [length]) else attn.MODE_FULL
         caches = [KVCache(length, format, device=self.device) for _ in range(self.layers)]
         self.forward(ids, [0, length], mode, store=caches)
-        return CachedPrefix(length, mode, caches)
+        return CachedPrefix(length, mode, caches, auto)
 
     def with_prefix(self, prefix: CachedPrefix) -> "PrefixedModel":
         """A runtime whose requests all stand behind ``prefix``."""
@@ -195,6 +212,7 @@ class Qwen3EmbeddingModel:
                                  f"{self.layers}")
             longest = max((int(b) - int(a) for a, b in zip(cu_seqlens[:-1], cu_seqlens[1:])),
                           default=0)
+            mode = prefix.mode_for(longest)
             rope_rows = self._rope_rows(prefix.length, longest)
         if store is not None:
             if len(store) < self.layers or any(c.slots < T for c in store):
@@ -218,7 +236,7 @@ class Qwen3EmbeddingModel:
                 kv_cache_write(store[l], k, v.view(T, 8, 128), slots)
             if prefix is not None:
                 prefix_attention(q, k, v.view(T, 8, 128), cu_seqlens, prefix.caches[l],
-                                 prefix.length, mode=prefix.mode, out=o)
+                                 prefix.length, mode=mode, out=o)
             else:
                 attn.attention(q, k, v, cu_seqlens, value_stride=1024, value_offset=0, mode=mode,
                                out=o)
