@@ -403,7 +403,9 @@ typedef struct qwa_kv_cache {
  * for which the largest magnitude is at most 448 * 2^e (E4M3) or 127 * 2^e
  * (INT8), 2^0 for a row of zeros; code = x * 2^-e rounded to nearest, ties to even.
  * An infinity is stored as the largest code; NaN stays NaN in E4M3 and becomes 0 in
- * INT8, and does not count for e. e is at least -15 / -24 (f16) and -117 / -126 (bf16),
+ * INT8, and does not count for e. e is at least -15 / -24 (f16: the smallest code then
+ * stands for the smallest subnormal, 2^-24) and -117 / -126 (bf16: for the smallest normal,
+ * 2^-126, so smaller values are rounded to its multiples),
  * and where 256 * 2^e (64 * 2^e) is out of the 16-bit type's range, codes end at 240 (63): what
  * is read back is always finite unless a NaN was written. Slots of one call must
  * differ: of two rows for one slot, values of both may remain. */

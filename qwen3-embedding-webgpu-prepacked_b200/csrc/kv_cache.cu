@@ -13,9 +13,12 @@
 // stored numbers. E4M3 loses nothing by it (a floating format has the same
 // relative step under any scale); INT8 loses up to one of its 7 bits.
 //
-// e stops at `low`, where code * 2^e still is a multiple of the type's
-// smallest subnormal, and at the top, where 256 * 2^e (64 * 2^e) would leave
-// the type's range, codes stop one step lower (240, 63).
+// e stops at `low`, where the smallest code times 2^e is the smallest value that is
+// left whole: f16's smallest subnormal 2^-24, which attention and conversions keep, but
+// bf16's smallest normal 2^-126, so that no value read back depends on how products
+// treat f32 subnormals (bf16's range is f32's). Smaller bf16 values are rounded to
+// multiples of 2^-126. At the top, where 256 * 2^e (64 * 2^e) would leave the type's
+// range, codes stop one step lower (240, 63).
 #include <cuda_bf16.h>
 
 #include "convert.cuh"
