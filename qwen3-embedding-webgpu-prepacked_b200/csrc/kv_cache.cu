@@ -143,8 +143,9 @@ __device__ __forceinline__ Where where(const KvCacheArgs& a, uint32_t vec) {
 
 // head_dim / 16 lanes hold a vector, 16 values each (two loads, one 16-byte
 // store of codes). HBM-bound: a thread's kVectors loads are in flight together, and
-// wait for nothing. 80000 tokens of 8 heads into INT8: 81 us, 6.1 TB/s (0.95 of measured; 91 us with
-// divisions by `heads`, which made it bound by its arithmetic); 16 tokens: 1.7 us.
+// wait for nothing. 80000 tokens of 8 heads into INT8: 81 to 87 us with the clock, 5.7 to 6.1
+// TB/s (0.88 to 0.95 of measured; 91 us with divisions by `heads`, which made it bound by
+// its arithmetic); 16 tokens: 1.7 us.
 template <bool kBf16, int kFormat, int kVectors>
 __global__ void __launch_bounds__(kThreads) kv_write_kernel(const KvCacheArgs a) {
   using C = Code<kBf16, kFormat == kKvPlain ? kKvE4M3 : kFormat>;
@@ -220,7 +221,7 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(const KvCacheArgs a)
 }
 
 // The way back: 16 codes a lane (one load, two stores). 8000 scattered slots of 8
-// heads from E4M3: 10.8 us, 4.6 TB/s (0.71 of measured; 2 us of it are the launch).
+// heads from E4M3: 10.8 to 11.2 us, 4.5 TB/s (0.70 of measured; 2 us of it are the launch).
 template <bool kBf16, int kFormat, int kVectors>
 __global__ void __launch_bounds__(kThreads) kv_read_kernel(const KvCacheArgs a) {
   const int lanes = a.head_dim / 16, per_pass = kThreads / lanes;

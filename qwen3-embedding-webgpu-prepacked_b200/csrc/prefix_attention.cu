@@ -40,14 +40,20 @@
 // leaves its O, m and l in shared memory and merges a share of the rows from
 // all of them. No workspace, one launch, and an order that does not vary.
 //
+// Bits. Scores, m, l and O are f32. P is rounded once to the 16-bit type of V, as both operands
+// of a tcgen05 f16 MMA have one type: at most half a step of p (2^-11, bf16 2^-8) for
+// each key, against l of the unrounded values. The relative error against 64 bits (rms) grows
+// from the output's own rounding, 0.00021 in f16 and 0.0017 in bf16, to 0.00029 and 0.0023; a P of 32
+// bits would take the tf32 form, at half the rate, with V as 32 bits too.
+//
 // What bounds it (16/8 heads). Long requests: a key tile of two row tiles takes about
-// 4070 cycles, twice its MMAs: S waits for PV, as P lies over it, and the
-// exponentials of one row tile take longer than the MMAs of the other. 4 x 5000 bf16
-// tokens behind 5000: 1215 to 1340 us with the clock, 920 to 1010 TFLOP/s (0.56 to 0.62 of
-// measured). 16 x 500 f16 behind 2000 in E4M3: 195 us, 755 TFLOP/s; 504 blocks for 148
-// SMs, so the fourth round is less than half full. Small calls: latency. 16 x 1 behind 1000
-// in E4M3: 12.3 us, 16 x 15..150 behind 176: 16.1 us; loads, S, softmax, PV, merge and
-// the launch follow one another, on instructions that are not cached yet.
+// 4070 cycles, 1.4 times what its MMAs need (about 2900): S waits for PV, as P lies over
+// it, and the exponentials of one row tile take longer than the MMAs of the other. 4 x 5000
+// bf16 tokens behind 5000: 1215 to 1380 us with the clock, 890 to 1010 TFLOP/s (0.55 to
+// 0.62 of measured). 16 x 500 f16 behind 2000 in E4M3: 193 to 196 us, 755 TFLOP/s; 504 blocks
+// for 148 SMs, so the fourth round is less than half full. Small calls: latency. 16 x 1 behind
+// 1000 in E4M3: 12.3 to 12.9 us, 16 x 15..150 behind 176: 16.1 to 16.8 us; loads, S, softmax,
+// PV, merge and the launch follow one another, on instructions that are not cached yet.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

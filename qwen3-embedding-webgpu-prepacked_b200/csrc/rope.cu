@@ -59,8 +59,9 @@ __host__ __device__ constexpr int rope_table_bytes(int half) { return (half * 8 
 // One block a token: what turns passes through shared memory, so pairs of any
 // distance and rows of any stride and alignment are served. kUnits: rows of whole 16-byte
 // units, moved as such; the units behind the rotated part go straight through.
-// 8000 tokens of 16 + 8 heads of 128, 34 in halves: 31 us, 3.2 TB/s (118 value by value):
-// bound by its passes through shared memory.
+// 8000 tokens of 16 + 8 heads of 128, 34 in halves: 31 us, 3.2 TB/s; rows of an odd stride, value
+// by value: 113 us, 0.87 TB/s (all 128 in halves 118). Bound by its passes through shared memory,
+// value by value by 2-byte accesses.
 template <typename T, bool kUnits>
 __global__ void __launch_bounds__(kRopeThreads) rope_any_kernel(const RopeArgs a) {
   extern __shared__ __align__(16) uint8_t rope_smem[];

@@ -11,7 +11,10 @@ reference's, on absolute positions.
 
 Launches are the kernel of csrc/prefix_attention.cu through the C ABI. A
 ``PrefixPlan`` holds the work lists of given lengths; ``prefix_attention``
-keeps the last few plans.
+keeps the last few plans. Lengths that were not met before cost their plan: lists made on the
+host, an allocation and a copy, and as it allocates it waits for what runs on the device
+(16 ragged requests: 83 us of the host's time a call instead of 17; 16 of about 500 tokens
+behind 2000: 219 instead of 22, in the shade of a kernel of 193). A model's layers share one.
 """
 from __future__ import annotations
 
